@@ -13,6 +13,8 @@ LIB_PATH = os.path.join(HERE, "libhfuse_b200.so")
 
 HFUSE_MAX_HITS = 256
 HFUSE_NOALLOC_MAX_CHANNELS = 1024
+HFUSE_F32, HFUSE_BF16, HFUSE_F16 = 0, 1, 2
+HFUSE_RECURRENCE_CHUNK = 256
 
 _p, _i, _f = C.c_void_p, C.c_int, C.c_float
 _i64, _u64, _u32, _sz = C.c_int64, C.c_uint64, C.c_uint32, C.c_size_t
@@ -23,6 +25,13 @@ MAXPOOL = [_p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p]
 BNSTATS = [_p, _i, _i, _i, _f, _p, _p, _p, _p, _sz]
 UPSAMPLE = [_p, _i, _i, _i, _i, _i, _i, _i, _p]
 HISTC = [_p, _i64, _i, _f, _f, _p]
+# language-model operators
+LAYERNORM = [_p, _i64, _i, _i64, _i, _p, _p, _i, _f, _p, _p, _p]
+LAYERNORM_BWD = [_p, _i64, _p, _i64, _i64, _i, _i, _p, _p, _p, _i, _p, _p, _p, _p, _sz]
+EMBEDDING = [_p, _i64, _i, _i, _p, _i64, _i, _f, _p]
+EMBEDDING_BWD = [_p, _p, _i64, _i, _i64, _i, _i, _f, _i64, _p, _p, _sz]
+RECURRENCE = [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i, _i, _p, _p, _p, _p]
+RECURRENCE_BWD = [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _p, _p, _p]
 SEARCH = [C.c_char_p, _u64, _u64, C.c_char_p, _p]                 # header80, start, count, target32, hits
 ETHASH = [_p, _u32, C.c_char_p, _u64, _u64, C.c_char_p, _p]       # dag, items, header_hash32, start, count, target32, hits
 
@@ -47,6 +56,9 @@ CRYPTO_PAIRS = {
     "sia_ethash": ("sia", "ethash"), "blake256_sha256d": ("blake256", "sha256d"),
     "blake256_sia": ("blake256", "sia"), "sha256d_sia": ("sha256d", "sia"),
 }
+LM_OPS = {"hfuse_layernorm": LAYERNORM, "hfuse_layernorm_backward": LAYERNORM_BWD, "hfuse_embedding": EMBEDDING,
+          "hfuse_embedding_backward": EMBEDDING_BWD, "hfuse_gated_recurrence": RECURRENCE,
+          "hfuse_gated_recurrence_backward": RECURRENCE_BWD}
 
 
 class Hits(C.Structure):
@@ -69,6 +81,8 @@ def exported_symbols() -> list[str]:
               "hfuse_histc_allreduce_counts", "hfuse_dag_broadcast", "hfuse_blake256_sha256d_search_sharded",
               "hfuse_sia_ethash_search_sharded"]
     names += ["hfuse_maxpool2d_backward_f32", "hfuse_bn_backward_f32", "hfuse_maxpool_backward_bn_backward_f32"]
+    names += list(LM_OPS) + ["hfuse_layernorm_backward_workspace_bytes", "hfuse_embedding_backward_workspace_bytes",
+                             "hfuse_gated_recurrence_chunks"]
     names += ["hfuse_error_string", "hfuse_version", "hfuse_bnstats_workspace_bytes", "hfuse_bnstats_noalloc_f32",
               "hfuse_bnstats_finalize_f64", "hfuse_hits_reset", "hfuse_hash_batch", "hfuse_tune_set",
               "hfuse_tune_describe", "hfuse_tune_default", "hfuse_tune_set_share", "hfuse_tune_option", "hfuse_xoshiro256ss_fill", "hfuse_int32_probe", "hfuse_hbm_probe", "hfuse_hbm_probe_bulk", "hfuse_shard_range"]
@@ -131,6 +145,14 @@ def lib() -> C.CDLL:
     L.hfuse_bn_backward_f32.restype, L.hfuse_bn_backward_f32.argtypes = _i, BNB + [_p]
     L.hfuse_maxpool_backward_bn_backward_f32.restype = _i
     L.hfuse_maxpool_backward_bn_backward_f32.argtypes = MPB + BNB + [_p]
+    for sym, params in LM_OPS.items():
+        fn = getattr(L, sym)
+        fn.restype, fn.argtypes = _i, params + [_p]
+    L.hfuse_layernorm_backward_workspace_bytes.restype = _sz
+    L.hfuse_layernorm_backward_workspace_bytes.argtypes = [_i64, _i]
+    L.hfuse_embedding_backward_workspace_bytes.restype = _sz
+    L.hfuse_embedding_backward_workspace_bytes.argtypes = [_i64, _i64, _i]
+    L.hfuse_gated_recurrence_chunks.restype, L.hfuse_gated_recurrence_chunks.argtypes = _i64, [_i64]
     L.hfuse_comm_unique_id.restype, L.hfuse_comm_unique_id.argtypes = _i, [C.c_char_p]
     L.hfuse_comm_create.restype, L.hfuse_comm_create.argtypes = _i, [_i, _i, C.c_char_p, C.POINTER(_p)]
     L.hfuse_comm_destroy.restype, L.hfuse_comm_destroy.argtypes = _i, [_p]

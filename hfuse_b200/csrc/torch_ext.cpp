@@ -1,4 +1,5 @@
-// PyTorch extension: torch.ops.hfuse_b200.* for the five DL kernels and their ten fused pairs.
+// PyTorch extension: torch.ops.hfuse_b200.* for the five DL kernels, their ten fused pairs and the
+// language-model operators.
 //
 // Stands in for the torch C++ extension the reference's Python harness calls
 // (TorchKernel's build.sh / call_{1080,v100}.py, README.md:68,84-95 of aoli-al/HFuse).  It only
@@ -11,6 +12,7 @@
 
 #include <map>
 #include <mutex>
+#include <optional>
 #include <tuple>
 
 #include "../../include/hfuse_b200.h"
@@ -234,6 +236,177 @@ std::tuple<Tensor, Tensor, Tensor> histc_bnstats(const Tensor& x, int64_t bins, 
     return {a.counts, b.mean, b.invstd};
 }
 
+// ---- operators of a language model's token path ---------------------------------------------------------
+using OptTensor = const std::optional<Tensor>&;
+
+int lm_type(const Tensor& t, const char* what) {
+    TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor: hfuse_b200 has no CPU path");
+    switch (t.scalar_type()) {
+    case at::kFloat: return HFUSE_F32;
+    case at::kBFloat16: return HFUSE_BF16;
+    case at::kHalf: return HFUSE_F16;
+    default: break;
+    }
+    TORCH_CHECK(false, what, " must be float32, bfloat16 or float16");
+    return -1;
+}
+void check_unit(const Tensor& t, const char* what) {
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, what, " must have a last dimension of at least 1");
+    TORCH_CHECK(t.size(-1) == 1 || t.stride(-1) == 1, what, " must have stride 1 in its last dimension");
+    TORCH_CHECK(t.size(-1) <= INT32_MAX, what, " has too long rows");
+}
+void check_like(const Tensor& t, const Tensor& like, at::ScalarType type, const char* what) {
+    TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor: hfuse_b200 has no CPU path");
+    TORCH_CHECK(t.device() == like.device(), what, " must be on ", like.device(), ", is on ", t.device());
+    TORCH_CHECK(t.scalar_type() == type, what, " must be ", type, ", is ", t.scalar_type());
+}
+void check_vec(const Tensor& t, const Tensor& like, at::ScalarType type, at::IntArrayRef shape, const char* what) {
+    check_like(t, like, type, what);
+    TORCH_CHECK(t.sizes() == shape, what, " must have shape ", shape, ", has ", t.sizes());
+    TORCH_CHECK(t.is_contiguous(), what, " must be contiguous");
+}
+const void* opt_ptr(OptTensor t) { return t ? t->data_ptr() : nullptr; }
+const float* opt_f32(OptTensor t) { return t ? t->data_ptr<float>() : nullptr; }
+
+// elements between two rows (all dimensions but the last, which must follow each other evenly)
+int64_t row_stride(const Tensor& t, const char* what) {
+    int64_t ld = -1, span = 0;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (ld < 0) ld = t.stride(d);
+        else TORCH_CHECK(t.stride(d) == span, what, " must have rows that are evenly spaced in memory");
+        span = t.stride(d) * t.size(d);
+    }
+    if (ld < 0) return t.size(-1);
+    TORCH_CHECK(ld >= t.size(-1), what, " must have rows that do not overlap");
+    return ld;
+}
+// type of weight and bias (the input's where there is neither)
+at::ScalarType norm_params(const Tensor& x, OptTensor weight, OptTensor bias) {
+    const auto type = weight ? weight->scalar_type() : bias ? bias->scalar_type() : x.scalar_type();
+    TORCH_CHECK(type == x.scalar_type() || type == at::kFloat, "weight and bias must have the input's type or float32");
+    const int64_t D[1] = {x.size(-1)};
+    if (weight) check_vec(*weight, x, type, D, "weight");
+    if (bias) check_vec(*bias, x, type, D, "bias");
+    return type;
+}
+int code_of(at::ScalarType t) { return t == at::kFloat ? HFUSE_F32 : t == at::kBFloat16 ? HFUSE_BF16 : HFUSE_F16; }
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm(const Tensor& x, OptTensor weight, OptTensor bias, double eps) {
+    const int type = lm_type(x, "layer_norm input");
+    check_unit(x, "layer_norm input");
+    TORCH_CHECK(eps >= 0, "layer_norm: eps must not be negative");
+    const auto wt = norm_params(x, weight, bias);
+    const int64_t D = x.size(-1), ld = row_stride(x, "layer_norm input");
+    c10::cuda::CUDAGuard g(x.device());
+    Tensor y = at::empty(x.sizes(), x.options());
+    Tensor mean = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat)), invstd = at::empty_like(mean);
+    ok(hfuse_layernorm(x.data_ptr(), x.numel() / D, i32(D), ld, type, opt_ptr(weight), opt_ptr(bias), code_of(wt), (float)eps,
+                       y.data_ptr(), mean.data_ptr<float>(), invstd.data_ptr<float>(), stream()), "hfuse_layernorm");
+    return {y, mean, invstd};
+}
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& x, const Tensor& grad_out, const Tensor& mean,
+                                                       const Tensor& invstd, OptTensor weight) {
+    const int type = lm_type(x, "layer_norm input");
+    check_unit(x, "layer_norm input");
+    check_like(grad_out, x, x.scalar_type(), "layer_norm grad_out");
+    TORCH_CHECK(grad_out.sizes() == x.sizes(), "layer_norm grad_out must have the shape of the input");
+    check_unit(grad_out, "layer_norm grad_out");
+    check_vec(mean, x, at::kFloat, x.sizes().slice(0, x.dim() - 1), "mean");
+    check_vec(invstd, x, at::kFloat, x.sizes().slice(0, x.dim() - 1), "invstd");
+    const auto wt = norm_params(x, weight, std::nullopt);
+    const int64_t D = x.size(-1), rows = x.numel() / D;
+    const int64_t ldx = row_stride(x, "layer_norm input"), ldg = row_stride(grad_out, "layer_norm grad_out");
+    c10::cuda::CUDAGuard g(x.device());
+    Tensor dx = at::empty(x.sizes(), x.options());
+    Tensor dw = at::empty({D}, x.options().dtype(wt)), db = at::empty({D}, x.options().dtype(wt));
+    Tensor ws = at::empty({(int64_t)hfuse_layernorm_backward_workspace_bytes(rows, i32(D))}, x.options().dtype(at::kByte));
+    ok(hfuse_layernorm_backward(x.data_ptr(), ldx, grad_out.data_ptr(), ldg, rows, i32(D), type, mean.data_ptr<float>(),
+                                invstd.data_ptr<float>(), opt_ptr(weight), code_of(wt), dx.data_ptr(), dw.data_ptr(),
+                                db.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), stream()), "hfuse_layernorm_backward");
+    return {dx, dw, db};
+}
+
+void check_ids(const Tensor& ids, const Tensor& like) {
+    TORCH_CHECK(ids.is_cuda(), "ids must be a CUDA tensor: hfuse_b200 has no CPU path");
+    TORCH_CHECK(ids.device() == like.device(), "ids must be on ", like.device(), ", is on ", ids.device());
+    TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "ids must be int64 or int32");
+    TORCH_CHECK(ids.is_contiguous(), "ids must be contiguous");
+}
+Tensor embedding(const Tensor& table, const Tensor& ids, double scale) {
+    const int type = lm_type(table, "embedding table");
+    TORCH_CHECK(table.dim() == 2 && table.numel() > 0 && table.is_contiguous(), "embedding table must be 2-D, contiguous and not empty");
+    TORCH_CHECK(table.size(1) <= INT32_MAX, "embedding table has too long rows");
+    check_ids(ids, table);
+    c10::cuda::CUDAGuard g(table.device());
+    auto shape = ids.sizes().vec();
+    shape.push_back(table.size(1));
+    Tensor out = at::empty(shape, table.options());
+    ok(hfuse_embedding(table.data_ptr(), table.size(0), i32(table.size(1)), type, ids.data_ptr(), ids.numel(),
+                       i32(ids.element_size()), (float)scale, out.data_ptr(), stream()), "hfuse_embedding");
+    return out;
+}
+Tensor embedding_backward(const Tensor& grad_out, const Tensor& ids, int64_t rows, double scale, int64_t padding_id) {
+    const int type = lm_type(grad_out, "embedding grad_out");
+    check_ids(ids, grad_out);
+    TORCH_CHECK(grad_out.dim() == ids.dim() + 1 && grad_out.sizes().slice(0, ids.dim()) == ids.sizes() && grad_out.size(-1) >= 1,
+                "embedding grad_out must have the shape of ids and one dimension more");
+    TORCH_CHECK(grad_out.is_contiguous(), "embedding grad_out must be contiguous");
+    TORCH_CHECK(rows >= 1, "embedding_backward: rows must be positive");
+    const int64_t D = grad_out.size(-1), n = ids.numel();
+    TORCH_CHECK(D <= INT32_MAX, "embedding grad_out has too long rows");
+    c10::cuda::CUDAGuard g(grad_out.device());
+    Tensor grad = at::empty({rows, D}, grad_out.options());
+    Tensor ws = at::empty({(int64_t)hfuse_embedding_backward_workspace_bytes(n, rows, i32(D))}, grad_out.options().dtype(at::kByte));
+    ok(hfuse_embedding_backward(grad_out.data_ptr(), ids.data_ptr(), n, i32(ids.element_size()), rows, i32(D), type, (float)scale,
+                                padding_id, grad.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), stream()),
+       "hfuse_embedding_backward");
+    return grad;
+}
+
+int check_steps(const Tensor& t, const char* what) {
+    const int type = lm_type(t, what);
+    TORCH_CHECK(t.dim() == 3 && t.numel() > 0, what, " must be 3-D and not empty");
+    check_unit(t, what);
+    return type;
+}
+void check_steps_like(const Tensor& t, const Tensor& like, const char* what) {
+    check_like(t, like, like.scalar_type(), what);
+    TORCH_CHECK(t.sizes() == like.sizes(), what, " must have shape ", like.sizes(), ", has ", t.sizes());
+    check_unit(t, what);
+}
+std::tuple<Tensor, Tensor, Tensor> gated_recurrence(const Tensor& gate, const Tensor& x, OptTensor h0, bool save_states) {
+    const int type = check_steps(gate, "gate");
+    check_steps_like(x, gate, "x");
+    const int64_t B = x.size(0), T = x.size(1), D = x.size(2), BD[2] = {B, D};
+    if (h0) check_vec(*h0, x, at::kFloat, BD, "h0");
+    c10::cuda::CUDAGuard g(x.device());
+    const auto f32 = x.options().dtype(at::kFloat);
+    Tensor out = at::empty(x.sizes(), x.options()), last = at::empty({B, D}, f32);
+    Tensor states = save_states ? at::empty({B, hfuse_gated_recurrence_chunks(T), D}, f32) : at::empty({0}, f32);
+    ok(hfuse_gated_recurrence(gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), B, T, i32(D),
+                              type, opt_f32(h0), out.data_ptr(), last.data_ptr<float>(),
+                              save_states ? states.data_ptr<float>() : nullptr, stream()), "hfuse_gated_recurrence");
+    return {out, last, states};
+}
+std::tuple<Tensor, Tensor, Tensor> gated_recurrence_backward(const Tensor& gate, const Tensor& x, const Tensor& states,
+                                                             const Tensor& grad_out, OptTensor grad_last) {
+    const int type = check_steps(gate, "gate");
+    check_steps_like(x, gate, "x");
+    check_steps_like(grad_out, gate, "grad_out");
+    const int64_t B = x.size(0), T = x.size(1), D = x.size(2), BD[2] = {B, D}, S[3] = {B, hfuse_gated_recurrence_chunks(T), D};
+    check_vec(states, x, at::kFloat, S, "states");
+    if (grad_last) check_vec(*grad_last, x, at::kFloat, BD, "grad_last");
+    c10::cuda::CUDAGuard g(x.device());
+    Tensor dgate = at::empty(x.sizes(), x.options()), dx = at::empty(x.sizes(), x.options());
+    Tensor dh0 = at::empty({B, D}, x.options().dtype(at::kFloat));
+    ok(hfuse_gated_recurrence_backward(gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1),
+                                       states.data_ptr<float>(), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
+                                       opt_f32(grad_last), B, T, i32(D), type, dgate.data_ptr(), dx.data_ptr(),
+                                       dh0.data_ptr<float>(), stream()), "hfuse_gated_recurrence_backward");
+    return {dgate, dx, dh0};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(hfuse_b200, m) {
@@ -252,4 +425,10 @@ TORCH_LIBRARY(hfuse_b200, m) {
     m.def("histc_upsample(Tensor x, int bins, float min, float max, Tensor y, int[2] output_size, bool align_corners) -> (Tensor, Tensor)", &histc_upsample);
     m.def("upsample_bnstats(Tensor x, int[2] output_size, bool align_corners, Tensor y, float eps) -> (Tensor, Tensor, Tensor)", &upsample_bnstats);
     m.def("histc_bnstats(Tensor x, int bins, float min, float max, Tensor y, float eps) -> (Tensor, Tensor, Tensor)", &histc_bnstats);
+    m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)", &layer_norm);
+    m.def("layer_norm_backward(Tensor x, Tensor grad_out, Tensor mean, Tensor invstd, Tensor? weight) -> (Tensor, Tensor, Tensor)", &layer_norm_backward);
+    m.def("embedding(Tensor table, Tensor ids, float scale) -> Tensor", &embedding);
+    m.def("embedding_backward(Tensor grad_out, Tensor ids, int rows, float scale, int padding_id) -> Tensor", &embedding_backward);
+    m.def("gated_recurrence(Tensor gate, Tensor x, Tensor? h0, bool save_states) -> (Tensor, Tensor, Tensor)", &gated_recurrence);
+    m.def("gated_recurrence_backward(Tensor gate, Tensor x, Tensor states, Tensor grad_out, Tensor? grad_last) -> (Tensor, Tensor, Tensor)", &gated_recurrence_backward);
 }

@@ -10,6 +10,10 @@ An operator is described by a small object (`Im2col`, `MaxPool`, `BnStats`,
 `Upsample`, `Histc`) that owns its output buffers; `run(op)` launches the
 standalone kernel, `run_pair(a, b)` launches the fused pair named after the
 two halves (the ten pairs of the reference's configs/ml_fusion.yaml).
+
+The operators of a language model's token path (`layer_norm`, `embedding`,
+`gated_recurrence` and their backward functions) are plain functions that
+allocate their results; gradients are explicit calls, as for pooling and batch norm.
 """
 from __future__ import annotations
 
@@ -311,3 +315,213 @@ def run_backward_pair(mp: MaxPoolBackward, bn: BnBackward, stream=None):
     _lib.check(_lib.lib().hfuse_maxpool_backward_bn_backward_f32(*mp.c_args(), *bn.c_args(), _stream_ptr(stream)),
                "hfuse_maxpool_backward_bn_backward_f32")
     return mp.grad_in, (bn.dx, bn.grad_weight, bn.grad_bias)
+
+
+# ---- operators of a language model's token path (forward and backward; f32, bf16 and f16) ----------
+_LM_TYPES = {torch.float32: _lib.HFUSE_F32, torch.bfloat16: _lib.HFUSE_BF16, torch.float16: _lib.HFUSE_F16}
+
+
+def _check_lm(x, name, dim=None, dtypes=None, shape=None, like=None):
+    """Argument checks shared by the language-model operators; the innermost dimension has stride 1."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor: hfuse_b200 has no CPU path")
+    if x.dtype not in (dtypes or _LM_TYPES):
+        raise TypeError(f"{name} must be {' or '.join(str(t)[6:] for t in (dtypes or _LM_TYPES))}, got {x.dtype}")
+    if like is not None and x.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}, is on {x.device}")
+    if dim is not None and x.dim() != dim:
+        raise ValueError(f"{name} must be {dim}-D")
+    if shape is not None and tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, has {tuple(x.shape)}")
+    if x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{name} must have stride 1 in its last dimension")
+    return x
+
+
+def _contiguous(x, name):
+    if not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return x
+
+
+def _row_stride(x, name):
+    """Elements between two rows (all dimensions but the last one, which must follow each other evenly)."""
+    ld, span = None, None
+    for d in range(x.dim() - 2, -1, -1):
+        if x.shape[d] == 1:
+            continue
+        if ld is None:
+            ld = x.stride(d)
+        elif x.stride(d) != span:
+            raise ValueError(f"{name} must have rows that are evenly spaced in memory")
+        span = x.stride(d) * x.shape[d]
+    if ld is None:
+        return x.shape[-1]
+    if ld < x.shape[-1]:
+        raise ValueError(f"{name} must have rows that do not overlap")
+    return ld
+
+
+def _ptr(x):
+    return None if x is None else x.data_ptr()
+
+
+class _on:
+    """Device and stream of a call: buffers made inside belong to the stream that the kernels run on."""
+
+    def __init__(self, x, stream):
+        self.stream = stream if stream is not None else torch.cuda.current_stream(x.device)
+
+    def __enter__(self):
+        self.ctx = torch.cuda.stream(self.stream)
+        self.ctx.__enter__()
+        return self.stream.cuda_stream
+
+    def __exit__(self, *exc):
+        return self.ctx.__exit__(*exc)
+
+
+def _check_norm_params(x, weight, bias):
+    D = x.shape[-1]
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _contiguous(_check_lm(t, name, dtypes=(x.dtype, torch.float32), shape=(D,), like=x), name)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError("weight and bias must have the same type")
+    given = weight if weight is not None else bias
+    return x.dtype if given is None else given.dtype
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, stream=None):
+    """x [..., D] -> (y [..., D], mean [...], invstd [...]); mean and invstd are float32."""
+    _check_lm(x, "layer_norm input")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layer_norm input must have a last dimension of at least 1")
+    if not eps >= 0:
+        raise ValueError("layer_norm: eps must not be negative")
+    wt = _check_norm_params(x, weight, bias)
+    D, ld = x.shape[-1], _row_stride(x, "layer_norm input")
+    with _on(x, stream) as s:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        invstd = torch.empty_like(mean)
+        _lib.check(_lib.lib().hfuse_layernorm(x.data_ptr(), x.numel() // D, D, ld, _LM_TYPES[x.dtype], _ptr(weight), _ptr(bias),
+                                              _LM_TYPES[wt], float(eps), y.data_ptr(), mean.data_ptr(), invstd.data_ptr(), s),
+                   "hfuse_layernorm")
+    return y, mean, invstd
+
+
+def layer_norm_backward(x, grad_out, mean, invstd, weight=None, stream=None):
+    """Gradients (grad_in, grad_weight, grad_bias) of layer_norm from what it saved.  grad_weight and grad_bias have
+    the weight's type (the input's without a weight)."""
+    _check_lm(x, "layer_norm input")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layer_norm input must have a last dimension of at least 1")
+    _check_lm(grad_out, "layer_norm grad_out", dtypes=(x.dtype,), shape=x.shape, like=x)
+    for t, name in ((mean, "mean"), (invstd, "invstd")):
+        _contiguous(_check_lm(t, name, dtypes=(torch.float32,), shape=x.shape[:-1], like=x), name)
+    wt = _check_norm_params(x, weight, None)
+    D, rows = x.shape[-1], x.numel() // x.shape[-1]
+    ldx, ldg = _row_stride(x, "layer_norm input"), _row_stride(grad_out, "layer_norm grad_out")
+    L = _lib.lib()
+    with _on(x, stream) as s:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw, db = (torch.empty(D, dtype=wt, device=x.device) for _ in range(2))
+        ws = torch.empty(L.hfuse_layernorm_backward_workspace_bytes(rows, D), dtype=torch.uint8, device=x.device)
+        _lib.check(L.hfuse_layernorm_backward(x.data_ptr(), ldx, grad_out.data_ptr(), ldg, rows, D, _LM_TYPES[x.dtype],
+                                              mean.data_ptr(), invstd.data_ptr(), _ptr(weight), _LM_TYPES[wt], dx.data_ptr(),
+                                              dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(), s),
+                   "hfuse_layernorm_backward")
+    return dx, dw, db
+
+
+def _check_ids(ids, like):
+    return _contiguous(_check_lm(ids, "ids", dtypes=(torch.int64, torch.int32), like=like), "ids")
+
+
+def embedding(table, ids, scale=1.0, stream=None):
+    """scale * table[ids]: table [rows, D], ids of any shape (int64 or int32) -> ids.shape + [D]; an id outside the
+    table gives zeros."""
+    _contiguous(_check_lm(table, "embedding table", dim=2), "embedding table")
+    if 0 in table.shape:
+        raise ValueError("embedding table must not be empty")
+    _check_ids(ids, table)
+    rows, D = table.shape
+    with _on(table, stream) as s:
+        out = torch.empty(tuple(ids.shape) + (D,), dtype=table.dtype, device=table.device)
+        _lib.check(_lib.lib().hfuse_embedding(table.data_ptr(), rows, D, _LM_TYPES[table.dtype], ids.data_ptr(), ids.numel(),
+                                              ids.element_size(), float(scale), out.data_ptr(), s), "hfuse_embedding")
+    return out
+
+
+def embedding_backward(grad_out, ids, rows, scale=1.0, padding_id=-1, stream=None):
+    """Gradient [rows, D] of embedding's table; ids outside [0, rows) and padding_id (-1: none) give none."""
+    _contiguous(_check_lm(grad_out, "embedding grad_out"), "embedding grad_out")
+    _check_ids(ids, grad_out)
+    if grad_out.dim() < 1 or grad_out.shape[-1] < 1 or tuple(grad_out.shape[:-1]) != tuple(ids.shape):
+        raise ValueError("embedding grad_out must have the shape of ids and one dimension more")
+    if rows < 1:
+        raise ValueError("embedding_backward: rows must be positive")
+    D, n, L = grad_out.shape[-1], ids.numel(), _lib.lib()
+    with _on(grad_out, stream) as s:
+        grad = torch.empty(rows, D, dtype=grad_out.dtype, device=grad_out.device)
+        ws = torch.empty(L.hfuse_embedding_backward_workspace_bytes(n, rows, D), dtype=torch.uint8, device=grad_out.device)
+        _lib.check(L.hfuse_embedding_backward(grad_out.data_ptr(), ids.data_ptr(), n, ids.element_size(), rows, D,
+                                              _LM_TYPES[grad_out.dtype], float(scale), int(padding_id), grad.data_ptr(),
+                                              ws.data_ptr(), ws.numel(), s), "hfuse_embedding_backward")
+    return grad
+
+
+def _check_steps(x, name, like=None):
+    _check_lm(x, name, dim=3, dtypes=None if like is None else (like.dtype,), shape=None if like is None else like.shape, like=like)
+    if 0 in x.shape:
+        raise ValueError(f"{name} must not be empty")
+    return x
+
+
+def _check_state(h, name, x):
+    if h is not None:
+        _contiguous(_check_lm(h, name, dtypes=(torch.float32,), shape=(x.shape[0], x.shape[2]), like=x), name)
+    return h
+
+
+def gated_recurrence(gate, x, h0=None, save_states=False, stream=None):
+    """h_t = sigmoid(gate_t) h_{t-1} + (1 - sigmoid(gate_t)) x_t along dimension 1 of gate, x [B, T, D] ->
+    (h [B, T, D], the last state [B, D] in float32, states for gated_recurrence_backward or an empty tensor)."""
+    _check_steps(gate, "gate")
+    _check_steps(x, "x", gate)
+    _check_state(h0, "h0", x)
+    B, T, D = x.shape
+    L = _lib.lib()
+    with _on(x, stream) as s:
+        out = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+        last = torch.empty((B, D), dtype=torch.float32, device=x.device)
+        states = torch.empty((B, L.hfuse_gated_recurrence_chunks(T), D) if save_states else (0,), dtype=torch.float32,
+                             device=x.device)
+        _lib.check(L.hfuse_gated_recurrence(gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0),
+                                            x.stride(1), B, T, D, _LM_TYPES[x.dtype], _ptr(h0), out.data_ptr(), last.data_ptr(),
+                                            states.data_ptr() if save_states else None, s), "hfuse_gated_recurrence")
+    return out, last, states
+
+
+def gated_recurrence_backward(gate, x, states, grad_out, grad_last=None, stream=None):
+    """Gradients (grad_gate, grad_x, grad_h0) of gated_recurrence from the states that it saved; grad_last [B, D] is the
+    gradient of the last state."""
+    _check_steps(gate, "gate")
+    _check_steps(x, "x", gate)
+    _check_steps(grad_out, "grad_out", gate)
+    _check_state(grad_last, "grad_last", x)
+    B, T, D = x.shape
+    L = _lib.lib()
+    _contiguous(_check_lm(states, "states", dtypes=(torch.float32,), shape=(B, L.hfuse_gated_recurrence_chunks(T), D), like=x),
+                "states")
+    with _on(x, stream) as s:
+        dgate, dx = (torch.empty((B, T, D), dtype=x.dtype, device=x.device) for _ in range(2))
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=x.device)
+        _lib.check(L.hfuse_gated_recurrence_backward(
+            gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), states.data_ptr(),
+            grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1), _ptr(grad_last), B, T, D, _LM_TYPES[x.dtype],
+            dgate.data_ptr(), dx.data_ptr(), dh0.data_ptr(), s), "hfuse_gated_recurrence_backward")
+    return dgate, dx, dh0

@@ -12,7 +12,8 @@
  *
  * Conventions
  *   - every pointer is a device pointer on the current CUDA device unless its comment
- *     says "host"; float buffers are contiguous NCHW fp32, 16-byte aligned;
+ *     says "host"; float buffers are contiguous NCHW fp32, 16-byte aligned (the language-model
+ *     operators have their own types and strides, see there);
  *   - `stream` is a cudaStream_t passed as void* (NULL = the default stream);
  *   - return value: HFUSE_OK or a negative HFUSE_ERR_* code; nothing is thrown;
  *   - calls are asynchronous with respect to the host;
@@ -184,6 +185,78 @@ HFUSE_API int hfuse_maxpool_backward_bn_backward_f32(
     int sh, int sw, int ph, int pw, int dh, int dw, float* p_grad_in, const float* x, const float* grad_out, int N, int C,
     int HW, const float* weight, const float* mean, const float* invstd, float* grad_in, float* grad_weight,
     float* grad_bias, hfuse_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Operators of a language model's token path that are no matrix product (no counterpart in the
+ * reference, whose deep-learning kernels are those of an image model): layer norm beside batch
+ * norm, the embedding lookup and its gradient beside pooling by saved indices, and a gated linear
+ * recurrence.  Each comes with its backward pass.
+ *   - `dtype` is one of HFUSE_F32, HFUSE_BF16, HFUSE_F16; arithmetic, statistics and states are
+ *     32-bit floating point, a 16-bit result is rounded once when it is stored;
+ *   - pointers need the alignment of their element type only; buffers and rows that are 16-byte
+ *     aligned (recurrence: channel counts and strides that are multiples of 4 bytes) run faster;
+ *   - outputs and workspaces must not overlap inputs or each other; a workspace needs no
+ *     initialisation and holds nothing between calls; two calls that overlap on the GPU must not
+ *     share one;
+ *   - results do not depend on timing: the same call gives the same bits.
+ * ------------------------------------------------------------------------------------- */
+enum { HFUSE_F32 = 0, HFUSE_BF16 = 1, HFUSE_F16 = 2 };
+
+/* Layer norm over rows of D elements: mean = sum(x)/D, invstd = 1/sqrt(sum((x-mean)^2)/D + eps),
+ * y = (x-mean) invstd weight + bias.  Row r of x begins at x + r * ld_x elements (ld_x >= D; row
+ * stride of a slice of a wider buffer); y is [rows][D] without gaps.  weight and bias (each may be
+ * NULL: 1, 0) are [D] of type weight_dtype, which is dtype or HFUSE_F32.  mean and invstd
+ * [rows] are kept for the backward pass.  rows = 0 is allowed and does nothing. */
+HFUSE_API int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype, const void* weight,
+                              const void* bias, int weight_dtype, float eps, void* y, float* mean, float* invstd,
+                              hfuse_stream_t stream);
+/* With xh = (x-mean) invstd and g = grad_out weight:
+ *   grad_in = invstd (g - mean_D(g) - xh mean_D(g xh)) [rows][D], grad_weight = sum over rows of
+ *   grad_out xh, grad_bias = sum over rows of grad_out (both [D] of type weight_dtype; with
+ *   rows = 0 they are zero).  grad_in, grad_weight and grad_bias may each be NULL.  The workspace
+ *   (16-byte aligned) may be NULL when grad_weight and grad_bias both are. */
+HFUSE_API size_t hfuse_layernorm_backward_workspace_bytes(int64_t rows, int D);
+HFUSE_API int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, int64_t ld_grad_out, int64_t rows,
+                                       int D, int dtype, const float* mean, const float* invstd, const void* weight,
+                                       int weight_dtype, void* grad_in, void* grad_weight, void* grad_bias, void* workspace,
+                                       size_t workspace_bytes, hfuse_stream_t stream);
+
+/* Embedding lookup: out[i] = scale table[ids[i]], table [rows][D], out [n][D].  ids are 32- or
+ * 64-bit signed integers (id_bytes 4 or 8).  An id outside [0, rows) gives a row of zeros.
+ * n = 0 is allowed and does nothing. */
+HFUSE_API int hfuse_embedding(const void* table, int64_t rows, int D, int dtype, const void* ids, int64_t n, int id_bytes,
+                              float scale, void* out, hfuse_stream_t stream);
+/* Its gradient: grad_table[v] = scale times the sum of grad_out[i] over the tokens i with
+ * ids[i] = v, added in 32 bits in a fixed order; every row of grad_table [rows][D] is written, rows
+ * without a token with zeros.  Ids outside [0, rows) and tokens whose id is padding_id (-1: none)
+ * give no gradient. */
+HFUSE_API size_t hfuse_embedding_backward_workspace_bytes(int64_t n, int64_t rows, int D);
+HFUSE_API int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, int id_bytes, int64_t rows, int D,
+                                       int dtype, float scale, int64_t padding_id, void* grad_table, void* workspace,
+                                       size_t workspace_bytes, hfuse_stream_t stream);
+
+/* Gated linear recurrence along T steps, for B sequences of D channels each:
+ *   a_t = sigmoid(gate_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  out_t = h_t
+ * gate and x: element (b, t, d) at b * stride_b + t * stride_t + d (strides in elements, not
+ * negative), so both may be halves of one wider buffer; out is [B][T][D] without gaps.  h0
+ * [B][D] (float; NULL: zeros) is the state before the first step, h_last [B][D] (float) the state
+ * after the last one: a sequence may be worked off in pieces, down to single steps.  `states` (float, may
+ * be NULL: not wanted) receives what the backward pass needs, [B][hfuse_gated_recurrence_chunks(T)][D]:
+ * the state before every step that is a multiple of HFUSE_RECURRENCE_CHUNK.  A gate of -infinity
+ * starts afresh (h_t = x_t), one of +infinity holds the state. */
+#define HFUSE_RECURRENCE_CHUNK 256
+HFUSE_API int64_t hfuse_gated_recurrence_chunks(int64_t T);
+HFUSE_API int hfuse_gated_recurrence(const void* gate, int64_t gate_stride_b, int64_t gate_stride_t, const void* x,
+                                     int64_t x_stride_b, int64_t x_stride_t, int64_t B, int64_t T, int D, int dtype,
+                                     const float* h0, void* out, float* h_last, float* states, hfuse_stream_t stream);
+/* With e_t = grad_out_t + a_{t+1} e_{t+1}, e_T including grad_h_last ([B][D] float, may be NULL):
+ *   grad_x_t = (1 - a_t) e_t, grad_gate_t = e_t (h_{t-1} - x_t) a_t (1 - a_t) (both [B][T][D]), grad_h0 = a_1 e_1
+ *   ([B][D] float).  `states` as the forward call wrote it. */
+HFUSE_API int hfuse_gated_recurrence_backward(const void* gate, int64_t gate_stride_b, int64_t gate_stride_t, const void* x,
+                                              int64_t x_stride_b, int64_t x_stride_t, const float* states,
+                                              const void* grad_out, int64_t grad_out_stride_b, int64_t grad_out_stride_t,
+                                              const float* grad_h_last, int64_t B, int64_t T, int D, int dtype,
+                                              void* grad_gate, void* grad_x, float* grad_h0, hfuse_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Multi-GPU batch-norm statistics with the cross-GPU sum inside the kernel (no counterpart

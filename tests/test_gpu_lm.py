@@ -1,0 +1,335 @@
+"""The language-model operators against their 64-bit definitions, inside the bounds that 32-bit arithmetic gives."""
+import pytest
+import torch
+
+from hfuse_b200 import _lib, ops
+from oracle import lm
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def within(got, exact, bound, dtype=None):
+    """got is of type dtype and no further from exact than the bound and one rounding to that type allow"""
+    dtype = dtype or got.dtype
+    assert got.dtype == dtype and got.shape == exact.shape
+    off, may = (got.double() - exact).abs(), lm.store(bound, exact, dtype)
+    assert (off <= may).all(), f"{(off / may).max().item():.3g} times the bound"
+
+
+@pytest.fixture(params=["harness", "extension"])
+def api(request):
+    """Both Python entry points with one signature."""
+    if request.param == "harness":
+        return ops
+    from hfuse_b200 import torch_ops
+
+    class Extension:
+        layer_norm = staticmethod(lambda x, w=None, b=None, eps=1e-5: torch_ops.ops.layer_norm(x, w, b, eps))
+        layer_norm_backward = staticmethod(lambda x, dy, m, r, w=None: torch_ops.ops.layer_norm_backward(x, dy, m, r, w))
+        embedding = staticmethod(lambda t, i, s=1.0: torch_ops.ops.embedding(t, i, s))
+        embedding_backward = staticmethod(lambda dy, i, rows, s=1.0, pad=-1: torch_ops.ops.embedding_backward(dy, i, rows, s, pad))
+        gated_recurrence = staticmethod(lambda g, x, h=None, save=False: torch_ops.ops.gated_recurrence(g, x, h, save))
+        gated_recurrence_backward = staticmethod(lambda g, x, s, dy, dl=None: torch_ops.ops.gated_recurrence_backward(g, x, s, dy, dl))
+
+    return Extension
+
+
+# ---- layer norm -------------------------------------------------------------------------------------------------
+NORM_SHAPES = [(1, 1), (1, 4096), (3, 7), (5, 32), (700, 64), (37, 129), (2, 1001), (333, 1000), (64, 2048), (300, 512), (9, 8192),
+               (5, 8190), (3, 16384), (3, 20000), (2, 70001), (2500, 96), (5000, 24), (1200, 256), (450, 1024), (301, 4095)]
+
+
+def _norm_inputs(dev, rows, D, t, wt, seed, offset=0.3):
+    g = _gen(dev, seed)
+    x = (offset + torch.randn(rows, D, generator=g, device=dev) * (0.5 + torch.rand(rows, 1, generator=g, device=dev))).to(t)
+    w = (1 + 0.3 * torch.randn(D, generator=g, device=dev)).to(wt)
+    b = (0.3 * torch.randn(D, generator=g, device=dev)).to(wt)
+    return x, w, b, torch.randn(rows, D, generator=g, device=dev).to(t)
+
+
+def _check_norm(api, x, w, b, dy, eps=1e-5):
+    y, mean, invstd = api.layer_norm(x, w, b, eps)
+    wt = w.dtype if w is not None else b.dtype if b is not None else x.dtype
+    for got, exact, bound, t in zip((y, mean, invstd), lm.layer_norm(x, w, b, eps), lm.layer_norm_bound(x, w, b, eps),
+                                    (x.dtype, torch.float32, torch.float32)):
+        within(got, exact, bound, t)
+    grads = api.layer_norm_backward(x, dy, mean, invstd, w)
+    wt = w.dtype if w is not None else x.dtype
+    for got, exact, bound, t in zip(grads, lm.layer_norm_backward(x, dy, mean, invstd, w),
+                                    lm.layer_norm_backward_bound(x, dy, mean, invstd, w), (x.dtype, wt, wt)):
+        within(got, exact, bound, t)
+    return (y, mean, invstd) + tuple(grads)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,D", NORM_SHAPES)
+def test_layer_norm(dev, rows, D, kind):
+    x, w, b, dy = _norm_inputs(dev, rows, D, TYPES[kind], TYPES[kind], 11)
+    _check_norm(ops, x, w, b, dy)
+
+
+@pytest.mark.parametrize("rows,D,kind", [(40, 768, "bf16"), (7, 1001, "f16"), (1500, 64, "bf16"), (3, 20000, "f16")])
+def test_layer_norm_under_float_weights(dev, api, rows, D, kind):
+    x, w, b, dy = _norm_inputs(dev, rows, D, TYPES[kind], torch.float32, 12)
+    _check_norm(api, x, w, b, dy)
+
+
+@pytest.mark.parametrize("D", [64, 33, 2048])
+def test_layer_norm_without_weight_or_bias(dev, api, D):
+    x, w, b, dy = _norm_inputs(dev, 50, D, torch.bfloat16, torch.bfloat16, 13)
+    _check_norm(api, x, None, None, dy)
+    _check_norm(api, x, None, b, dy)
+    _check_norm(api, x, w, None, dy)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("at,D,wide", [(8, 64, 192), (3, 64, 200), (64, 1024, 2048), (1, 1024, 1500), (0, 129, 131)])
+def test_layer_norm_of_a_slice_of_wider_rows(dev, api, at, D, wide, kind):
+    big, _, _, dbig = _norm_inputs(dev, 6 * 35, wide, TYPES[kind], TYPES[kind], 14)
+    _, w, b, _ = _norm_inputs(dev, 1, D, TYPES[kind], TYPES[kind], 15)
+    x, dy = big.view(6, 35, wide)[..., at:at + D], dbig.view(6, 35, wide)[..., at:at + D]
+    got = _check_norm(api, x, w, b, dy)
+    assert got[0].is_contiguous() and got[0].shape == x.shape
+    with pytest.raises((ValueError, RuntimeError), match="evenly spaced"):
+        api.layer_norm(big.view(6, 35, wide)[:, :20, at:at + D], w, b)
+    with pytest.raises((ValueError, RuntimeError), match="stride 1"):
+        api.layer_norm(big.t(), None, None)
+
+
+def test_layer_norm_far_from_zero_and_of_constant_rows(dev):
+    x, w, b, dy = _norm_inputs(dev, 64, 1024, torch.float32, torch.float32, 16, offset=1000.0)
+    _check_norm(ops, x, w, b, dy)
+    y, mean, invstd = ops.layer_norm(torch.full((4, 512), 3.0, device=dev), None, None, 1e-5)
+    assert (y == 0).all() and (mean == 3).all()
+    torch.testing.assert_close(invstd, torch.full((4,), 1e-5 ** -0.5, device=dev), rtol=4 * lm.U, atol=0)
+
+
+def test_layer_norm_keeps_a_bad_row_to_itself(dev):
+    x, w, b, dy = _norm_inputs(dev, 90, 256, torch.bfloat16, torch.bfloat16, 17)
+    good = ops.layer_norm(x, w, b)
+    bad = x.clone()
+    bad[7, 3], bad[50, 0], bad[89, 255] = float("nan"), float("inf"), float("-inf")
+    y, mean, invstd = ops.layer_norm(bad, w, b)
+    rows = torch.tensor([7, 50, 89], device=dev)
+    keep = torch.ones(90, dtype=torch.bool, device=dev)
+    keep[rows] = False
+    assert y[rows].isnan().all() and torch.equal(y[keep], good[0][keep]) and torch.equal(mean[keep], good[1][keep])
+    dx, dw, db = ops.layer_norm_backward(bad, dy, mean, invstd, w)
+    ref = ops.layer_norm_backward(x, dy, good[1], good[2], w)
+    assert torch.equal(dx[keep], ref[0][keep]) and dx[rows].isnan().all() and torch.equal(db, ref[2])
+
+
+def test_layer_norm_of_no_rows(dev, api):
+    x, w = torch.empty(0, 16, device=dev), torch.ones(16, device=dev)
+    y, mean, invstd = api.layer_norm(x, w, None)
+    assert y.shape == (0, 16) and mean.shape == (0,)
+    dx, dw, db = api.layer_norm_backward(x, x, mean, invstd, w)
+    assert dx.shape == (0, 16) and (dw == 0).all() and (db == 0).all()
+
+
+def test_layer_norm_shapes_and_refusals(dev, api):
+    x = torch.randn(2, 3, 5, 16, device=dev)
+    y, mean, _ = api.layer_norm(x)
+    assert y.shape == x.shape and mean.shape == (2, 3, 5)
+    v, vm, _ = api.layer_norm(x[0, 0, 0])
+    assert v.shape == (16,) and vm.shape == () and torch.equal(v, y[0, 0, 0])
+    w = torch.ones(16, device=dev)
+    for bad in (lambda: api.layer_norm(x, w[:15]), lambda: api.layer_norm(x, w.double()), lambda: api.layer_norm(x.int()),
+                lambda: api.layer_norm(x.bfloat16(), w.half()), lambda: api.layer_norm(x, w, None, -1.0),
+                lambda: api.layer_norm(x, w.cpu()), lambda: api.layer_norm(x[..., :1].expand(2, 3, 5, 16)),
+                lambda: api.layer_norm(x[:1, :1, :1].expand(2, 3, 5, 16)),
+                lambda: api.layer_norm_backward(x, x[:1], mean, mean, w), lambda: api.layer_norm_backward(x, x, mean[0], mean, w),
+                lambda: api.layer_norm_backward(x, x.half(), mean, mean, w),
+                lambda: api.layer_norm_backward(x, x, mean.half(), mean, w)):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            bad()
+
+
+# ---- embedding --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,V,D", [((1,), 1, 1), ((3, 5), 7, 8), ((1000,), 300, 33), ((64,), 32000, 1024), ((7, 129), 1001, 250),
+                                       ((5000,), 50, 64), ((2,), 5, 20000)])
+def test_embedding(dev, api, shape, V, D, kind):
+    g = _gen(dev, 21)
+    table = torch.randn(V, D, generator=g, device=dev).to(TYPES[kind])
+    ids = torch.randint(0, V, shape, generator=g, device=dev)
+    want = (table[ids].float() * 1.7).to(table.dtype)              # one product, one rounding: the same bits
+    scale = float(torch.tensor(1.7, dtype=torch.float32))
+    assert torch.equal(api.embedding(table, ids, scale), want)
+    assert torch.equal(api.embedding(table, ids.int(), scale), want)
+    within(want, lm.embedding(table, ids, scale), lm.U * lm.embedding(table, ids, scale).abs())
+
+
+def test_embedding_ids_outside_the_table(dev, api):
+    table = torch.randn(10, 24, device=dev)
+    ids = torch.tensor([0, -1, 9, 10, 1 << 40, -(1 << 40), 5], device=dev)
+    out = api.embedding(table, ids, 2.0)
+    assert torch.equal(out, lm.embedding(table, ids, 2.0).float())
+    assert api.embedding(table, ids[:0], 2.0).shape == (0, 24)
+    dy = torch.randn(7, 24, device=dev)
+    grad = api.embedding_backward(dy, ids, 10, 2.0)
+    assert torch.equal(grad, lm.embedding_backward(dy, ids, 10, 2.0).float())
+    assert (api.embedding_backward(dy[:0], ids[:0], 10, 2.0) == 0).all()
+
+
+def _ids(dev, n, V, how, seed):
+    g = _gen(dev, seed)
+    if how == "one":
+        return torch.full((n,), V // 2, device=dev, dtype=torch.int64)
+    if how == "rising":
+        return torch.arange(n, device=dev) % V
+    if how == "text":
+        r = torch.exp(torch.rand(n, generator=g, device=dev, dtype=torch.float64) * torch.log(torch.tensor(V + 1.0))) - 1
+        return torch.randperm(V, generator=g, device=dev)[r.long().clamp(0, V - 1)]
+    return torch.randint(0, V, (n,), generator=g, device=dev)
+
+
+@pytest.mark.parametrize("n,V,D,how,kind", [
+    (1, 1, 1, "one", "f32"), (2, 511, 8, "even", "bf16"), (31, 512, 16, "even", "f16"), (32, 513, 33, "one", "bf16"),
+    (33, 3, 64, "one", "f32"), (64, 2, 8, "rising", "f32"), (65, 64, 8, "rising", "f16"), (2047, 1000, 40, "text", "f32"),
+    (2048, 262143, 8, "even", "bf16"), (2049, 262144, 8, "even", "f32"), (4100, 50257, 1001, "text", "f16"),
+    (5000, 100, 128, "text", "bf16"), (70000, 30000, 64, "text", "bf16"), (40000, 4, 24, "one", "f32"), (300000, 1000, 8, "text", "f32"),
+    (300000, 7, 8, "even", "bf16"), (777, 1 << 20, 9, "even", "f32"), (16384, 32000, 512, "text", "f16"), (9000, 9000, 2048, "rising", "bf16")])
+def test_embedding_backward(dev, n, V, D, how, kind):
+    ids = _ids(dev, n, V, how, 22)
+    dy = torch.randn(n, D, generator=_gen(dev, 23), device=dev).to(TYPES[kind])
+    got = ops.embedding_backward(dy, ids, V, 0.5)
+    within(got, lm.embedding_backward(dy, ids, V, 0.5), lm.embedding_backward_bound(dy, ids, V, 0.5), TYPES[kind])
+    assert torch.equal(got, ops.embedding_backward(dy, ids.int(), V, 0.5))           # the same bits every time
+
+
+@pytest.mark.parametrize("pad", [0, 17, 99])
+def test_embedding_backward_padding_and_unused_ids(dev, api, pad):
+    ids = _ids(dev, 6000, 100, "text", 24)
+    ids[::3] = pad
+    ids[1::50], ids[2::70] = -5, 100
+    dy = torch.randn(6000, 72, generator=_gen(dev, 25), device=dev).bfloat16()
+    got = api.embedding_backward(dy.view(60, 100, 72), ids.view(60, 100), 100, 3.0, pad)
+    within(got, lm.embedding_backward(dy, ids, 100, 3.0, pad), lm.embedding_backward_bound(dy, ids, 100, 3.0, pad))
+    assert (got[pad] == 0).all()
+
+
+def test_embedding_backward_of_padding_alone(dev, api):
+    ids = torch.full((3000,), 4, device=dev)
+    assert (api.embedding_backward(torch.randn(3000, 16, device=dev), ids, 9, 1.0, 4) == 0).all()
+
+
+def test_embedding_refusals(dev, api):
+    table, ids = torch.randn(10, 24, device=dev), torch.zeros(4, dtype=torch.int64, device=dev)
+    dy = torch.randn(4, 24, device=dev)
+    for bad in (lambda: api.embedding(table.t(), ids), lambda: api.embedding(table[0], ids), lambda: api.embedding(table, ids.short()),
+                lambda: api.embedding(table, ids.cpu()), lambda: api.embedding(table, torch.zeros(8, dtype=torch.int64, device=dev)[::2]),
+                lambda: api.embedding(table[:0], ids), lambda: api.embedding(table.double(), ids),
+                lambda: api.embedding_backward(dy, ids[:3], 10), lambda: api.embedding_backward(dy, ids, 0),
+                lambda: api.embedding_backward(dy[:, ::2], ids, 10), lambda: api.embedding_backward(dy.double(), ids, 10)):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            bad()
+
+
+# ---- gated recurrence -------------------------------------------------------------------------------------------
+def _rec_inputs(dev, B, T, D, t, seed):
+    g = _gen(dev, seed)
+    gate = (2 + 2.5 * torch.randn(B, T, D, generator=g, device=dev)).to(t)
+    x, dy = (torch.randn(B, T, D, generator=g, device=dev).to(t) for _ in range(2))
+    h0, dl = (torch.randn(B, D, generator=g, device=dev) for _ in range(2))
+    return gate, x, dy, h0, dl
+
+
+def _check_rec(api, gate, x, dy, h0, dl):
+    h, last, states = api.gated_recurrence(gate, x, h0, True)
+    eh, before, elast = lm.gated_recurrence(gate, x, h0)
+    bh, bbefore, blast = lm.gated_recurrence_bound(gate, x, h0)
+    within(h, eh, bh, x.dtype)
+    within(last, elast, blast, torch.float32)
+    step = _lib.HFUSE_RECURRENCE_CHUNK
+    within(states, before[:, ::step], bbefore[:, ::step], torch.float32)
+    plain = api.gated_recurrence(gate, x, h0)
+    assert torch.equal(plain[0], h) and torch.equal(plain[1], last) and plain[2].numel() == 0
+    grads = api.gated_recurrence_backward(gate, x, states, dy, dl)
+    for got, exact, bound, t in zip(grads, lm.gated_recurrence_backward(gate, x, h0, dy, dl),
+                                    lm.gated_recurrence_backward_bound(gate, x, h0, dy, dl), (x.dtype, x.dtype, torch.float32)):
+        within(got, exact, bound, t)
+    return h, last, states
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,D", [(1, 1, 1), (2, 1, 64), (64, 1, 257), (1, 2, 3), (3, 15, 32), (2, 16, 33), (5, 17, 34), (3, 255, 33),
+                                   (2, 256, 64), (2, 257, 40), (1, 513, 130), (300, 5, 8), (4, 700, 96), (1, 3001, 8), (2, 1500, 66)])
+def test_gated_recurrence(dev, B, T, D, kind):
+    gate, x, dy, h0, dl = _rec_inputs(dev, B, T, D, TYPES[kind], 31)
+    _check_rec(ops, gate, x, dy, h0, dl)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_gated_recurrence_from_nothing(dev, api, kind):
+    gate, x, dy, _, _ = _rec_inputs(dev, 2, 300, 48, TYPES[kind], 32)
+    _check_rec(api, gate, x, dy, None, None)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("D,at", [(64, 0), (64, 3), (33, 0), (250, 2)])
+def test_gated_recurrence_of_halves_of_one_buffer(dev, api, D, at, kind):
+    g = _gen(dev, 33)
+    both = torch.randn(2, 333, 2 * D + 6, generator=g, device=dev).to(TYPES[kind])
+    gate, x = both[..., at:at + D], both[..., at + D:at + 2 * D]
+    dy = torch.randn(333, 2, D, generator=g, device=dev).to(TYPES[kind]).transpose(0, 1)
+    h0, dl = (torch.randn(2, D, generator=g, device=dev) for _ in range(2))
+    _check_rec(api, gate, x, dy, h0, dl)
+    # a gate that all sequences share
+    _check_rec(api, gate[:1].expand(2, 333, D), x, dy, h0, dl)
+
+
+def test_gated_recurrence_in_pieces_and_single_steps(dev, api):
+    gate, x, _, h0, _ = _rec_inputs(dev, 3, 600, 80, torch.bfloat16, 34)
+    whole, last, _ = api.gated_recurrence(gate, x, h0)
+    bound = lm.gated_recurrence_bound(gate, x, h0)
+    exact = lm.gated_recurrence(gate, x, h0)
+    h, out = h0, []
+    for a, b in ((0, 1), (1, 2), (2, 300), (300, 557), (557, 600)):
+        y, h, _ = api.gated_recurrence(gate[:, a:b], x[:, a:b], h)
+        out.append(y)
+    within(torch.cat(out, 1), exact[0], bound[0])
+    within(h, exact[2], bound[2])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_gates_of_infinity(dev, api, kind):
+    gate, x, dy, h0, dl = _rec_inputs(dev, 2, 530, 36, TYPES[kind], 35)
+    gate[:, 100], gate[:, 256], gate[0, 511] = float("-inf"), float("-inf"), float("-inf")
+    gate[:, 101:140], gate[1, 300:400] = float("inf"), float("inf")
+    h, _, _ = _check_rec(api, gate, x, dy, h0, dl)
+    assert torch.equal(h[:, 100], x[:, 100]) and torch.equal(h[:, 139], x[:, 100]) and torch.equal(h[:, 256], x[:, 256])
+
+
+def test_gated_recurrence_keeps_a_bad_channel_to_itself(dev):
+    gate, x, dy, h0, dl = _rec_inputs(dev, 2, 400, 70, torch.float32, 36)
+    h, last, states = ops.gated_recurrence(gate, x, h0, True)
+    ref = ops.gated_recurrence_backward(gate, x, states, dy, dl)
+    bg, bx = gate.clone(), x.clone()
+    bg[0, 50, 3], bx[1, 399, 69] = float("nan"), float("inf")
+    h2, last2, states2 = ops.gated_recurrence(bg, bx, h0, True)
+    keep = torch.ones(2, 70, dtype=torch.bool, device=dev)
+    keep[0, 3] = keep[1, 69] = False
+    pick = keep[:, None, :].expand(2, 400, 70)
+    assert torch.equal(h2[pick], h[pick]) and torch.equal(last2[keep], last[keep])
+    assert torch.equal(h2[0, :50, 3], h[0, :50, 3]) and h2[0, 50:, 3].isnan().all()
+    got = ops.gated_recurrence_backward(bg, bx, states2, dy, dl)
+    assert torch.equal(got[0][pick], ref[0][pick]) and torch.equal(got[1][pick], ref[1][pick])
+
+
+def test_gated_recurrence_refusals(dev, api):
+    g = torch.randn(2, 5, 8, device=dev)
+    st = torch.zeros(2, 1, 8, device=dev)
+    for bad in (lambda: api.gated_recurrence(g, g[:, :4]), lambda: api.gated_recurrence(g, g.half()), lambda: api.gated_recurrence(g[0], g[0]),
+                lambda: api.gated_recurrence(g, g, torch.zeros(2, 7, device=dev)), lambda: api.gated_recurrence(g, g, st[:, 0].half()),
+                lambda: api.gated_recurrence(g[:, :0], g[:, :0]), lambda: api.gated_recurrence(g.transpose(1, 2), g.transpose(1, 2)),
+                lambda: api.gated_recurrence(g, g.cpu()), lambda: api.gated_recurrence_backward(g, g, st[:, :, :7], g),
+                lambda: api.gated_recurrence_backward(g, g, st, g[:1]), lambda: api.gated_recurrence_backward(g, g, st, g, st)):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            bad()
