@@ -4,6 +4,18 @@
 //   e_t = dout_t + a_{t+1} e_{t+1},  dx_t = (1 - a_t) e_t,  dgate_t = e_t (h_{t-1} - x_t) a_t (1 - a_t),  dh_0 = a_1 e_1
 //
 // A gate of -infinity starts afresh (h_t = x_t), one of +infinity holds the state.
+//
+// Steps s .. t together map a state h to A h + H with A the product of their a and H their result from zero, and two
+// such maps make one: (A2, H2) after (A1, H1) is (A2 A1, A2 H1 + H2).  So a block takes 32 lanes' worth of channels
+// of one sequence, each of its warps runs kSteps steps of them from zero in registers, the warps' maps meet in
+// shared memory, and each warp adds what the state before its first step contributes: A_t times that state.  One
+// pass over the data: gate and x are read once and out is written once; the block moves on through the sequence
+// with the state in registers.  The backward pass does the same from the end (its maps are e -> A e + E),
+// with the states before each step run again from the ones that the forward pass saved every 256 steps.
+//
+// The next pieces of the sequence are on their way into shared memory (cp.async) while one is worked on.  Where there
+// are fewer groups of channels than the GPU has room for, a cluster of blocks shares a group: each takes a piece in turn
+// and the blocks' maps are exchanged through distributed shared memory.
 #include "launch.cuh"
 #include "lm_common.cuh"
 
@@ -12,6 +24,7 @@ using namespace hfuse;
 namespace {
 
 constexpr int kSaved = HFUSE_RECURRENCE_CHUNK;
+constexpr int kMaxCluster = 8;
 
 struct RecArgs {
     const void *gate, *x, *dy;
@@ -20,67 +33,432 @@ struct RecArgs {
     float *last, *states, *dh0;
     long long gate_b, gate_t, x_b, x_t, dy_b, dy_t;       // strides of a batch item and of a step
     int B, T, D, chunks;
+    int groups;              // groups of channels per sequence
+    int split;               // blocks that share a group
 };
 
-// a = sigmoid(g) and 1 - a, the smaller of the two without cancellation; a NaN stays one
+// a = sigmoid(g) and z = 1 - a = sigmoid(-g), both to a few units in their last place: with e = exp(-g),
+// a = 1 / (1 + e) and z = e a.  The exponent stops at 126 so that e a cannot be infinity times zero (the
+// subtraction then makes an a of 2^-126 the zero that a gate of -infinity stands for); a NaN stays one.
 __device__ __forceinline__ void gates(float g, float& a, float& z) {
-    const float e = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + e), s = e * r;
-    a = g >= 0.f ? r : s;
-    z = g >= 0.f ? s : r;
+    float t = g * -1.4426950408889634f, e;
+    asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(a) : "f"(1.f + e));
+    z = e * a;
+    a -= 0x1p-126f;
 }
 
-template <class T>
-__global__ void __launch_bounds__(128) rec_fwd(const RecArgs p) {
-    for (long long i = (long long)blockIdx.x * 128 + threadIdx.x; i < (long long)p.B * p.D; i += (long long)gridDim.x * 128) {
-        const long long b = i / p.D, d = i - b * p.D;
-        const T* g = static_cast<const T*>(p.gate) + b * p.gate_b + d;
-        const T* x = static_cast<const T*>(p.x) + b * p.x_b + d;
-        T* y = static_cast<T*>(p.y) + b * p.T * p.D + d;
-        float h = p.h0 ? p.h0[i] : 0.f;
-        for (int t = 0; t < p.T; ++t) {
-            if (p.states && t % kSaved == 0) p.states[(b * p.chunks + t / kSaved) * p.D + d] = h;
-            float a, z;
-            gates(to_f32(g[t * p.gate_t]), a, z);
-            h = fmaf(a, h, z * to_f32(x[t * p.x_t]));
-            y[(long long)t * p.D] = from_f32<T>(h);
+// ---- staging: `rows` steps of 32 * CPL channels into shared memory ----------------------------------------
+// ALIGN: bytes that every row's begin and the number of channels are a multiple of (16, 4, or one 16-bit element)
+__device__ __forceinline__ void cp_async16(void* s, const void* g) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s)), "l"(g) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void* s, const void* g) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(s)), "l"(g) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Steps from T on get `beyond` (a gate of +infinity and an x of zero leave the state as it is), channels from D on are
+// left alone: no result of theirs is stored.
+template <class T, int CPL, int ALIGN>
+__device__ __forceinline__ void stage_rows(T* dst, const T* src, long long stride, int t0, int rows, int d0, int T_end, int D,
+                                           float beyond) {
+    constexpr int C = 32 * CPL, E = ALIGN >= (int)sizeof(T) ? ALIGN / (int)sizeof(T) : 1, PER = C / E;
+    for (int i = threadIdx.x; i < rows * PER; i += blockDim.x) {
+        const int r = i / PER, k = (i - r * PER) * E;
+        if (d0 + k >= D) continue;
+        T* to = dst + r * C + k;
+        if (t0 + r < T_end) {
+            const T* from = src + (t0 + r) * stride + d0 + k;
+            if constexpr (ALIGN == 16) cp_async16(to, from);
+            else if constexpr (ALIGN == 4) cp_async4(to, from);
+            else *to = *from;
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) to[j] = from_f32<T>(beyond);
         }
-        p.last[i] = h;
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(128) rec_bwd(const RecArgs p) {
-    for (long long i = (long long)blockIdx.x * 128 + threadIdx.x; i < (long long)p.B * p.D; i += (long long)gridDim.x * 128) {
-        const long long b = i / p.D, d = i - b * p.D;
-        const T* g = static_cast<const T*>(p.gate) + b * p.gate_b + d;
-        const T* x = static_cast<const T*>(p.x) + b * p.x_b + d;
-        const T* dy = static_cast<const T*>(p.dy) + b * p.dy_b + d;
-        T* dg = static_cast<T*>(p.dgate) + b * p.T * p.D + d;
-        T* dx = static_cast<T*>(p.dx) + b * p.T * p.D + d;
-        float e = p.dlast ? p.dlast[i] : 0.f;
-        float before[kSaved];                              // the state before each step of the chunk, run again
-        for (int c = p.chunks - 1; c >= 0; --c) {
-            const int t0 = c * kSaved, t1 = min(p.T, t0 + kSaved);
-            float h = p.states[(b * p.chunks + c) * p.D + d], a, z;
-            for (int t = t0; t < t1; ++t) {
-                before[t - t0] = h;
-                gates(to_f32(g[t * p.gate_t]), a, z);
-                h = fmaf(a, h, z * to_f32(x[t * p.x_t]));
-            }
-            for (int t = t1 - 1; t >= t0; --t) {
-                gates(to_f32(g[t * p.gate_t]), a, z);
-                e += to_f32(dy[t * p.dy_t]);
-                dx[(long long)t * p.D] = from_f32<T>(e * z);
-                dg[(long long)t * p.D] = from_f32<T>(e * (before[t - t0] - to_f32(x[t * p.x_t])) * (a * z));
-                e *= a;
-            }
-        }
-        p.dh0[i] = e;
+template <class T, int CPL>
+__device__ __forceinline__ void read_row(const T* row, float (&v)[CPL]) {
+    const Pack<T, CPL> p = *reinterpret_cast<const Pack<T, CPL>*>(row);
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) v[c] = to_f32(p.v[c]);
+}
+template <class T, int CPL, bool WHOLE>
+__device__ __forceinline__ void write_out(T* p, const float (&v)[CPL], int left) {
+    if constexpr (WHOLE) {                 // rows keep the alignment of CPL elements, D is a multiple of CPL
+        Pack<T, CPL> r;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) r.v[c] = from_f32<T>(v[c]);
+        if (left > 0) store_stream<T, CPL>(p, r);
+    } else {
+#pragma unroll
+        for (int c = 0; c < CPL; ++c)
+            if (c < left) p[c] = from_f32<T>(v[c]);
     }
 }
+template <int CPL>
+__device__ __forceinline__ void read_state(const float* p, float (&v)[CPL], int left) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) v[c] = p && c < left ? p[c] : 0.f;
+}
+template <int CPL>
+__device__ __forceinline__ void write_state(float* p, const float (&v)[CPL], int left) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c)
+        if (c < left) p[c] = v[c];
+}
+
+// ---- cluster: the blocks that share a group of channels --------------------------------------------------
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void store_peer(float* p, int rank, float v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+
+// shared memory of a block: two stages of `tensors` tiles, two sets of the warps' maps (`maps` floats per channel), two
+// sets of the blocks' maps
+template <class T, int CPL>
+size_t rec_smem(int warps, int steps, int tensors, int maps, int split) {
+    const size_t C = 32 * CPL;
+    return 2 * (size_t)tensors * warps * steps * C * sizeof(T) + 2 * (size_t)maps * warps * C * 4 +
+           (split > 1 ? 2 * (size_t)kMaxCluster * 2 * C * 4 : 0);
+}
+
+template <class T, int CPL, int S, int ALIGN>
+__global__ void __launch_bounds__(512) rec_fwd(const RecArgs p) {
+    constexpr int C = 32 * CPL;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
+    T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x][rows][C]
+    float* maps = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T));   // [2][A, H][W][C]
+    float* peers = maps + 4 * W * C;                                          // [2][block][A, H][C]
+    const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
+    const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
+    const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
+    const T* x = static_cast<const T*>(p.x) + b * p.x_b;
+    T* y = static_cast<T*>(p.y) + (long long)b * p.T * p.D + d;
+    const int n = (p.T + rows * p.split - 1) / (rows * p.split);
+    const long long at_state = (long long)b * p.D + d;
+
+    auto issue = [&](int it) {
+        if (it < n) {
+            T* s = stage + (it & 1) * 2 * rows * C;
+            const int t0 = (it * p.split + rank) * rows;
+            stage_rows<T, CPL, ALIGN>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
+            stage_rows<T, CPL, ALIGN>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
+        }
+        cp_commit();
+    };
+    issue(0);
+    issue(1);
+    float carry[CPL];                                     // the state before the cluster's next piece
+    read_state<CPL>(p.h0 ? p.h0 + at_state : nullptr, carry, left);
+    if (p.split > 1) cluster_sync();                      // the peers' shared memory is there
+    for (int it = 0; it < n; ++it) {
+        const int t0 = (it * p.split + rank) * rows + warp * S;
+        const T* sg = stage + (it & 1) * 2 * rows * C + warp * S * C + lane * CPL;
+        const T* sx = sg + rows * C;
+        float* mA = maps + (it & 1) * 2 * W * C + lane * CPL;
+        float* mH = mA + W * C;
+        cp_wait<1>();
+        __syncthreads();
+        float h[S][CPL], a[S][CPL], H[CPL], A[CPL];
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) { H[c] = 0.f; A[c] = 1.f; }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float g[CPL], v[CPL];
+            read_row<T, CPL>(sg + s * C, g);
+            read_row<T, CPL>(sx + s * C, v);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                float at, zt;
+                gates(g[c], at, zt);
+                H[c] = fmaf(at, H[c], zt * v[c]);
+                A[c] *= at;
+                h[s][c] = H[c];
+                a[s][c] = A[c];
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) {
+            mA[warp * C + c] = A[c];
+            mH[warp * C + c] = H[c];
+        }
+        __syncthreads();
+        issue(it + 2);                                    // every warp has read this stage
+        float preA[CPL], preH[CPL];
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) { A[c] = preA[c] = 1.f; H[c] = preH[c] = 0.f; }
+        for (int w = 0; w < W; ++w) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                if (w == warp) { preA[c] = A[c]; preH[c] = H[c]; }
+                const float aw = mA[w * C + c];
+                H[c] = fmaf(aw, H[c], mH[w * C + c]);
+                A[c] *= aw;
+            }
+        }
+        float in[CPL];
+        if (p.split == 1) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                in[c] = fmaf(preA[c], carry[c], preH[c]);
+                carry[c] = fmaf(A[c], carry[c], H[c]);
+            }
+        } else {
+            float* set = peers + (it & 1) * kMaxCluster * 2 * C + lane * CPL;
+            for (int j = warp; j < p.split; j += W)
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) {
+                    store_peer(set + (2 * rank) * C + c, j, A[c]);
+                    store_peer(set + (2 * rank + 1) * C + c, j, H[c]);
+                }
+            cluster_sync();
+            for (int j = 0; j < p.split; ++j)
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) {
+                    if (j == rank) in[c] = fmaf(preA[c], carry[c], preH[c]);
+                    carry[c] = fmaf(set[(2 * j) * C + c], carry[c], set[(2 * j + 1) * C + c]);
+                }
+        }
+        if (p.states && t0 < p.T && t0 % kSaved == 0)
+            write_state<CPL>(p.states + ((long long)b * p.chunks + t0 / kSaved) * p.D + d, in, left);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) h[s][c] = fmaf(a[s][c], in[c], h[s][c]);
+            if (t0 + s < p.T) write_out<T, CPL, (ALIGN >= 4)>(y + (long long)(t0 + s) * p.D, h[s], left);
+        }
+    }
+    if (warp == 0 && rank == 0) write_state<CPL>(p.last + at_state, carry, left);
+}
+
+template <class T, int CPL, int S, int ALIGN>
+__global__ void __launch_bounds__(512) rec_bwd(const RecArgs p) {
+    constexpr int C = 32 * CPL;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
+    T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x, dy][rows][C]
+    float* maps = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T));   // [2][A, H, E][W][C]
+    float* peers = maps + 6 * W * C;                                          // [2][block][A, E][C]
+    const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
+    const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
+    const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
+    const T* x = static_cast<const T*>(p.x) + b * p.x_b;
+    const T* dy = static_cast<const T*>(p.dy) + b * p.dy_b;
+    T* dgate = static_cast<T*>(p.dgate) + (long long)b * p.T * p.D + d;
+    T* dx = static_cast<T*>(p.dx) + (long long)b * p.T * p.D + d;
+    const int n = (p.T + rows * p.split - 1) / (rows * p.split);
+    const long long at_state = (long long)b * p.D + d;
+
+    auto issue = [&](int k) {                              // the k-th piece from the end
+        if (k < n) {
+            T* s = stage + (k & 1) * 3 * rows * C;
+            const int t0 = ((n - 1 - k) * p.split + rank) * rows;
+            stage_rows<T, CPL, ALIGN>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
+            stage_rows<T, CPL, ALIGN>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
+            stage_rows<T, CPL, ALIGN>(s + 2 * rows * C, dy, p.dy_t, t0, rows, d0, p.T, p.D, 0.f);
+        }
+        cp_commit();
+    };
+    issue(0);
+    float carry[CPL];                                     // a e of the step after the cluster's next piece
+    read_state<CPL>(p.dlast ? p.dlast + at_state : nullptr, carry, left);
+    if (p.split > 1) cluster_sync();
+    for (int k = 0; k < n; ++k) {
+        const int first = ((n - 1 - k) * p.split + rank) * rows, t0 = first + warp * S;
+        const T* sg = stage + (k & 1) * 3 * rows * C + warp * S * C + lane * CPL;
+        const T* sx = sg + rows * C;
+        const T* sd = sx + rows * C;
+        float* mA = maps + (k & 1) * 3 * W * C + lane * CPL;
+        float* mH = mA + W * C;
+        float* mE = mH + W * C;
+        cp_wait<0>();
+        __syncthreads();                                  // the stage is there, and the other one has been read
+        issue(k + 1);
+        // a block's piece begins where the forward pass saved a state
+        float hb[CPL];
+        read_state<CPL>(first < p.T ? p.states + ((long long)b * p.chunks + first / kSaved) * p.D + d : nullptr, hb, left);
+        float a[S][CPL], z[S][CPL], A[CPL], H[CPL], E[CPL];
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = E[c] = 0.f; }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float g[CPL], v[CPL];
+            read_row<T, CPL>(sg + s * C, g);
+            read_row<T, CPL>(sx + s * C, v);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                gates(g[c], a[s][c], z[s][c]);
+                H[c] = fmaf(a[s][c], H[c], z[s][c] * v[c]);
+                A[c] *= a[s][c];
+            }
+        }
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) {
+            float v[CPL];
+            read_row<T, CPL>(sd + s * C, v);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) E[c] = (E[c] + v[c]) * a[s][c];
+        }
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) {
+            mA[warp * C + c] = A[c];
+            mH[warp * C + c] = H[c];
+            mE[warp * C + c] = E[c];
+        }
+        __syncthreads();
+        for (int w = 0; w < warp; ++w)
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) hb[c] = fmaf(mA[w * C + c], hb[c], mH[w * C + c]);
+        float preA[CPL], preE[CPL];
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) { A[c] = preA[c] = 1.f; E[c] = preE[c] = 0.f; }
+        for (int w = W - 1; w >= 0; --w) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                if (w == warp) { preA[c] = A[c]; preE[c] = E[c]; }
+                const float aw = mA[w * C + c];
+                E[c] = fmaf(aw, E[c], mE[w * C + c]);
+                A[c] *= aw;
+            }
+        }
+        float e[CPL];
+        if (p.split == 1) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                e[c] = fmaf(preA[c], carry[c], preE[c]);
+                carry[c] = fmaf(A[c], carry[c], E[c]);
+            }
+        } else {
+            float* set = peers + (k & 1) * kMaxCluster * 2 * C + lane * CPL;
+            for (int j = warp; j < p.split; j += W)
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) {
+                    store_peer(set + (2 * rank) * C + c, j, A[c]);
+                    store_peer(set + (2 * rank + 1) * C + c, j, E[c]);
+                }
+            cluster_sync();
+            for (int j = p.split - 1; j >= 0; --j)
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) {
+                    if (j == rank) e[c] = fmaf(preA[c], carry[c], preE[c]);
+                    carry[c] = fmaf(set[(2 * j) * C + c], carry[c], set[(2 * j + 1) * C + c]);
+                }
+        }
+        // dgate's factor (h_{t-1} - x_t) a z of each step, the states run again
+        float f[S][CPL];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float v[CPL];
+            read_row<T, CPL>(sx + s * C, v);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                f[s][c] = (hb[c] - v[c]) * (a[s][c] * z[s][c]);
+                hb[c] = fmaf(a[s][c], hb[c], z[s][c] * v[c]);
+            }
+        }
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) {
+            float v[CPL], dg[CPL], dv[CPL];
+            read_row<T, CPL>(sd + s * C, v);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+                e[c] += v[c];
+                dg[c] = e[c] * f[s][c];
+                dv[c] = e[c] * z[s][c];
+                e[c] *= a[s][c];
+            }
+            if (t0 + s < p.T) {
+                write_out<T, CPL, (ALIGN >= 4)>(dgate + (long long)(t0 + s) * p.D, dg, left);
+                write_out<T, CPL, (ALIGN >= 4)>(dx + (long long)(t0 + s) * p.D, dv, left);
+            }
+        }
+    }
+    if (warp == 0 && rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+constexpr int kStepsFwd = 16, kStepsBwd = 16;
 
 bool rec_shape_ok(int64_t B, int64_t T, int D) { return B > 0 && T > 0 && D > 0; }
 constexpr long long kMax32 = (1LL << 31) - 1;
+
+template <class... KArgs, class... Args>
+int launch_cluster(void (*kern)(KArgs...), int grid, int block, size_t smem, int cluster, cudaStream_t s, Args&&... args) {
+    if (cluster == 1) return launch_kernel(kern, grid, block, smem, s, false, args...);
+    allow_dynamic_smem((const void*)kern, smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return HFUSE_ERR_LAUNCH;
+    }
+    return check_launch();
+}
+
+// the largest of 16, 4 and the element size that divides every row's begin and the number of channels
+int rec_align(int es, int D, std::initializer_list<const void*> ptrs, std::initializer_list<long long> strides) {
+    uintptr_t all = (uintptr_t)D * es;
+    for (const void* q : ptrs) all |= reinterpret_cast<uintptr_t>(q);
+    for (long long s : strides) all |= (uintptr_t)(s * es);
+    return (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : es;
+}
+
+template <class T, int CPL, int ALIGN, bool BWD>
+int rec_launch(RecArgs a, cudaStream_t s) {
+    constexpr int S = BWD ? kStepsBwd : kStepsFwd;
+    DeviceFacts f;
+    if (int rc = device_facts(f)) return rc;
+    const int C = 32 * CPL, W = a.T >= 16 * S ? 16 : (a.T + S - 1) / S;
+    a.groups = (a.D + C - 1) / C;
+    const long long groups = (long long)a.B * a.groups;
+    const int pieces = (a.T + W * S - 1) / (W * S);
+    int split = 1;
+    if (groups < f.sms) {
+        split = (int)(f.sms / groups);
+        split = split > kMaxCluster ? kMaxCluster : split;
+        split = split > pieces ? pieces : split;
+    }
+    a.split = split;
+    const size_t smem = rec_smem<T, CPL>(W, S, BWD ? 3 : 2, BWD ? 3 : 2, split);
+    if (groups * split > kMax32) return HFUSE_ERR_TOO_LARGE;
+    if constexpr (BWD) return launch_cluster(rec_bwd<T, CPL, S, ALIGN>, (int)(groups * split), W * 32, smem, split, s, a);
+    else return launch_cluster(rec_fwd<T, CPL, S, ALIGN>, (int)(groups * split), W * 32, smem, split, s, a);
+}
+
+template <bool BWD>
+int rec_dispatch(const RecArgs& a, int dtype, int align, cudaStream_t s) {
+    return by_type(dtype, [&](auto t) {
+        using T = typename decltype(t)::type;
+        if constexpr (sizeof(T) == 4) {
+            return align == 16 ? rec_launch<T, 1, 16, BWD>(a, s) : rec_launch<T, 1, 4, BWD>(a, s);
+        } else {
+            if (align == 16) return rec_launch<T, 2, 16, BWD>(a, s);
+            if (align == 4) return rec_launch<T, 2, 4, BWD>(a, s);
+            return rec_launch<T, 2, 2, BWD>(a, s);
+        }
+    });
+}
 
 }  // namespace
 
@@ -94,21 +472,16 @@ int hfuse_gated_recurrence(const void* gate, int64_t gate_stride_b, int64_t gate
     if (!lm_type_ok(dtype) || !rec_shape_ok(B, T, D) || !gate || !x || !out || !h_last) return HFUSE_ERR_BAD_ARG;
     if (gate_stride_b < 0 || gate_stride_t < 0 || x_stride_b < 0 || x_stride_t < 0) return HFUSE_ERR_BAD_ARG;
     if (B > kMax32 || T > kMax32 - 65536 || B * D > kMax32) return HFUSE_ERR_TOO_LARGE;
-    const size_t es = lm_type_size(dtype);
+    const int es = lm_type_size(dtype);
     if (!aligned_to(gate, es) || !aligned_to(x, es) || !aligned_to(out, es) || !aligned_to(h0, 4) || !aligned_to(h_last, 4) ||
         !aligned_to(states, 4))
         return HFUSE_ERR_ALIGNMENT;
-    DeviceFacts f;
-    if (int rc = device_facts(f)) return rc;
     RecArgs a{};
     a.gate = gate; a.x = x; a.h0 = h0; a.y = out; a.last = h_last; a.states = states;
     a.gate_b = gate_stride_b; a.gate_t = gate_stride_t; a.x_b = x_stride_b; a.x_t = x_stride_t;
     a.B = (int)B; a.T = (int)T; a.D = D; a.chunks = (int)hfuse_gated_recurrence_chunks(T);
-    return by_type(dtype, [&](auto t) {
-        using E = typename decltype(t)::type;
-        const long long want = (B * D + 127) / 128, most = f.sms * 16LL;
-        return launch_kernel(rec_fwd<E>, (int)(want < most ? want : most), 128, 0, static_cast<cudaStream_t>(stream), false, a);
-    });
+    const int align = rec_align(es, D, {gate, x, out}, {gate_stride_b, gate_stride_t, x_stride_b, x_stride_t});
+    return rec_dispatch<false>(a, dtype, align, static_cast<cudaStream_t>(stream));
 }
 
 int hfuse_gated_recurrence_backward(const void* gate, int64_t gate_stride_b, int64_t gate_stride_t, const void* x,
@@ -121,23 +494,19 @@ int hfuse_gated_recurrence_backward(const void* gate, int64_t gate_stride_b, int
     if (gate_stride_b < 0 || gate_stride_t < 0 || x_stride_b < 0 || x_stride_t < 0 || grad_out_stride_b < 0 || grad_out_stride_t < 0)
         return HFUSE_ERR_BAD_ARG;
     if (B > kMax32 || T > kMax32 - 65536 || B * D > kMax32) return HFUSE_ERR_TOO_LARGE;
-    const size_t es = lm_type_size(dtype);
+    const int es = lm_type_size(dtype);
     if (!aligned_to(gate, es) || !aligned_to(x, es) || !aligned_to(grad_out, es) || !aligned_to(grad_gate, es) ||
         !aligned_to(grad_x, es) || !aligned_to(states, 4) || !aligned_to(grad_h_last, 4) || !aligned_to(grad_h0, 4))
         return HFUSE_ERR_ALIGNMENT;
-    DeviceFacts f;
-    if (int rc = device_facts(f)) return rc;
     RecArgs a{};
     a.gate = gate; a.x = x; a.dy = grad_out; a.dlast = grad_h_last; a.states = const_cast<float*>(states);
     a.dgate = grad_gate; a.dx = grad_x; a.dh0 = grad_h0;
     a.gate_b = gate_stride_b; a.gate_t = gate_stride_t; a.x_b = x_stride_b; a.x_t = x_stride_t;
     a.dy_b = grad_out_stride_b; a.dy_t = grad_out_stride_t;
     a.B = (int)B; a.T = (int)T; a.D = D; a.chunks = (int)hfuse_gated_recurrence_chunks(T);
-    return by_type(dtype, [&](auto t) {
-        using E = typename decltype(t)::type;
-        const long long want = (B * D + 127) / 128, most = f.sms * 16LL;
-        return launch_kernel(rec_bwd<E>, (int)(want < most ? want : most), 128, 0, static_cast<cudaStream_t>(stream), false, a);
-    });
+    const int align = rec_align(es, D, {gate, x, grad_out, grad_gate, grad_x},
+                                {gate_stride_b, gate_stride_t, x_stride_b, x_stride_t, grad_out_stride_b, grad_out_stride_t});
+    return rec_dispatch<true>(a, dtype, align, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
