@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace hfuse {
@@ -88,6 +90,30 @@ __device__ __forceinline__ void store_stream(T* p, const Pack<T, N>& r) {
         memcpy(&u, &r, 2);
         asm volatile("st.global.cs.u16 [%0], %1;" ::"l"(p), "h"(u) : "memory");
     }
+}
+
+// N floats rounded to T
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> pack_f32(const float (&v)[N]) {
+    Pack<T, N> r;
+    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 h = __floats2half2_rn(v[k], v[k + 1]);
+                r.v[k] = h.x;
+                r.v[k + 1] = h.y;
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[k], v[k + 1]);
+                r.v[k] = h.x;
+                r.v[k + 1] = h.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) r.v[k] = from_f32<T>(v[k]);
+    }
+    return r;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {

@@ -43,8 +43,8 @@ struct RecArgs {
 __device__ __forceinline__ void gates(float g, float& a, float& z) {
     float t = g * -1.4426950408889634f, e;
     asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
-    asm("rcp.approx.f32 %0, %1;" : "=f"(a) : "f"(1.f + e));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.f + e));
     z = e * a;
     a -= 0x1p-126f;
 }
@@ -67,16 +67,22 @@ template <class T, int CPL, int ALIGN>
 __device__ __forceinline__ void stage_rows(T* dst, const T* src, long long stride, int t0, int rows, int d0, int T_end, int D,
                                            float beyond) {
     constexpr int C = 32 * CPL, E = ALIGN >= (int)sizeof(T) ? ALIGN / (int)sizeof(T) : 1, PER = C / E;
-    for (int i = threadIdx.x; i < rows * PER; i += blockDim.x) {
-        const int r = i / PER, k = (i - r * PER) * E;
+    static_assert(PER <= 64 && 32 % (PER < 32 ? PER : 32) == 0, "a thread stays in its column");
+    constexpr int COLS = PER < 32 ? PER : 32;                // columns that a warp covers at a time
+    const int step = blockDim.x / COLS;
+    for (int k0 = 0; k0 < PER; k0 += COLS) {
+        const int k = (k0 + threadIdx.x % COLS) * E;
         if (d0 + k >= D) continue;
+        int r = threadIdx.x / COLS;
+        const T* from = src + (long long)(t0 + r) * stride + d0 + k;
         T* to = dst + r * C + k;
-        if (t0 + r < T_end) {
-            const T* from = src + (t0 + r) * stride + d0 + k;
+        const int in = min(rows, T_end - t0);
+        for (; r < in; r += step, from += step * stride, to += step * C) {
             if constexpr (ALIGN == 16) cp_async16(to, from);
             else if constexpr (ALIGN == 4) cp_async4(to, from);
             else *to = *from;
-        } else {
+        }
+        for (; r < rows; r += step, to += step * C) {
 #pragma unroll
             for (int j = 0; j < E; ++j) to[j] = from_f32<T>(beyond);
         }
@@ -92,10 +98,7 @@ __device__ __forceinline__ void read_row(const T* row, float (&v)[CPL]) {
 template <class T, int CPL, bool WHOLE>
 __device__ __forceinline__ void write_out(T* p, const float (&v)[CPL], int left) {
     if constexpr (WHOLE) {                 // rows keep the alignment of CPL elements, D is a multiple of CPL
-        Pack<T, CPL> r;
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) r.v[c] = from_f32<T>(v[c]);
-        if (left > 0) store_stream<T, CPL>(p, r);
+        if (left > 0) store_stream<T, CPL>(p, pack_f32<T, CPL>(v));
     } else {
 #pragma unroll
         for (int c = 0; c < CPL; ++c)
@@ -114,6 +117,31 @@ __device__ __forceinline__ void write_state(float* p, const float (&v)[CPL], int
         if (c < left) p[c] = v[c];
 }
 
+// ---- maps h -> A h + H of one stretch of steps in shared memory: {A, H} per channel ------------------------
+template <int CPL>
+__device__ __forceinline__ void write_map(float* m, const float (&A)[CPL], const float (&H)[CPL]) {
+    Pack<float, 2 * CPL> r;
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) { r.v[2 * c] = A[c]; r.v[2 * c + 1] = H[c]; }
+    *reinterpret_cast<Pack<float, 2 * CPL>*>(m) = r;
+}
+template <int CPL>
+__device__ __forceinline__ void apply_map(const float* m, float (&h)[CPL]) {
+    const Pack<float, 2 * CPL> r = *reinterpret_cast<const Pack<float, 2 * CPL>*>(m);
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) h[c] = fmaf(r.v[2 * c], h[c], r.v[2 * c + 1]);
+}
+// the map of the steps so far, then m's
+template <int CPL>
+__device__ __forceinline__ void join_map(const float* m, float (&A)[CPL], float (&H)[CPL]) {
+    const Pack<float, 2 * CPL> r = *reinterpret_cast<const Pack<float, 2 * CPL>*>(m);
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+        H[c] = fmaf(r.v[2 * c], H[c], r.v[2 * c + 1]);
+        A[c] *= r.v[2 * c];
+    }
+}
+
 // ---- cluster: the blocks that share a group of channels --------------------------------------------------
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -124,23 +152,23 @@ __device__ __forceinline__ void store_peer(float* p, int rank, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
 
-// shared memory of a block: two stages of `tensors` tiles, two sets of the warps' maps (`maps` floats per channel), two
-// sets of the blocks' maps
+// shared memory of a block: two stages of `tensors` tiles, the warps' maps (`maps` per channel; the barrier at the top of a
+// piece is behind their last reader), two sets of the blocks' maps
 template <class T, int CPL>
 size_t rec_smem(int warps, int steps, int tensors, int maps, int split) {
     const size_t C = 32 * CPL;
-    return 2 * (size_t)tensors * warps * steps * C * sizeof(T) + 2 * (size_t)maps * warps * C * 4 +
-           (split > 1 ? 2 * (size_t)kMaxCluster * 2 * C * 4 : 0);
+    return 2 * (size_t)tensors * warps * steps * C * sizeof(T) + (size_t)maps * warps * C * 8 +
+           (split > 1 ? 2 * (size_t)kMaxCluster * C * 8 : 0);
 }
 
 template <class T, int CPL, int S, int ALIGN>
-__global__ void __launch_bounds__(512) rec_fwd(const RecArgs p) {
+__global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
     constexpr int C = 32 * CPL;
     extern __shared__ __align__(128) unsigned char smem[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
     T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x][rows][C]
-    float* maps = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T));   // [2][A, H][W][C]
-    float* peers = maps + 4 * W * C;                                          // [2][block][A, H][C]
+    float* maps = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T));   // [W][C]{A, H}
+    float* peers = maps + 2 * W * C;                                          // [2][block][C]{A, H}
     const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
     const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
     const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
@@ -167,8 +195,7 @@ __global__ void __launch_bounds__(512) rec_fwd(const RecArgs p) {
         const int t0 = (it * p.split + rank) * rows + warp * S;
         const T* sg = stage + (it & 1) * 2 * rows * C + warp * S * C + lane * CPL;
         const T* sx = sg + rows * C;
-        float* mA = maps + (it & 1) * 2 * W * C + lane * CPL;
-        float* mH = mA + W * C;
+        float* map = maps + lane * CPL * 2;           // {A, H} of each channel, a warp in 2 C floats
         cp_wait<1>();
         __syncthreads();
         float h[S][CPL], a[S][CPL], H[CPL], A[CPL];
@@ -189,68 +216,58 @@ __global__ void __launch_bounds__(512) rec_fwd(const RecArgs p) {
                 a[s][c] = A[c];
             }
         }
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-            mA[warp * C + c] = A[c];
-            mH[warp * C + c] = H[c];
-        }
+        write_map<CPL>(map + warp * 2 * C, A, H);
         __syncthreads();
         issue(it + 2);                                    // every warp has read this stage
-        float preA[CPL], preH[CPL];
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) { A[c] = preA[c] = 1.f; H[c] = preH[c] = 0.f; }
-        for (int w = 0; w < W; ++w) {
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                if (w == warp) { preA[c] = A[c]; preH[c] = H[c]; }
-                const float aw = mA[w * C + c];
-                H[c] = fmaf(aw, H[c], mH[w * C + c]);
-                A[c] *= aw;
-            }
-        }
         float in[CPL];
         if (p.split == 1) {
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                in[c] = fmaf(preA[c], carry[c], preH[c]);
-                carry[c] = fmaf(A[c], carry[c], H[c]);
-            }
+            for (int c = 0; c < CPL; ++c) in[c] = carry[c];
+            for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) carry[c] = in[c];
+            for (int w = warp; w < W; ++w) apply_map<CPL>(map + w * 2 * C, carry);
         } else {
-            float* set = peers + (it & 1) * kMaxCluster * 2 * C + lane * CPL;
-            for (int j = warp; j < p.split; j += W)
+            float* set = peers + ((it & 1) * kMaxCluster * C + lane * CPL) * 2;
+            if (warp < p.split) {                         // W >= split: see rec_launch
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = 0.f; }
+                for (int w = 0; w < W; ++w) join_map<CPL>(map + w * 2 * C, A, H);
 #pragma unroll
                 for (int c = 0; c < CPL; ++c) {
-                    store_peer(set + (2 * rank) * C + c, j, A[c]);
-                    store_peer(set + (2 * rank + 1) * C + c, j, H[c]);
+                    store_peer(set + rank * 2 * C + 2 * c, warp, A[c]);
+                    store_peer(set + rank * 2 * C + 2 * c + 1, warp, H[c]);
                 }
+            }
             cluster_sync();
-            for (int j = 0; j < p.split; ++j)
+            for (int j = 0; j < rank; ++j) apply_map<CPL>(set + j * 2 * C, carry);
 #pragma unroll
-                for (int c = 0; c < CPL; ++c) {
-                    if (j == rank) in[c] = fmaf(preA[c], carry[c], preH[c]);
-                    carry[c] = fmaf(set[(2 * j) * C + c], carry[c], set[(2 * j + 1) * C + c]);
-                }
+            for (int c = 0; c < CPL; ++c) in[c] = carry[c];
+            for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
+            for (int j = rank; j < p.split; ++j) apply_map<CPL>(set + j * 2 * C, carry);
         }
         if (p.states && t0 < p.T && t0 % kSaved == 0)
             write_state<CPL>(p.states + ((long long)b * p.chunks + t0 / kSaved) * p.D + d, in, left);
+        T* to = y + (long long)t0 * p.D;
+        const int steps = p.T - t0;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
+        for (int s = 0; s < S; ++s, to += p.D) {
 #pragma unroll
             for (int c = 0; c < CPL; ++c) h[s][c] = fmaf(a[s][c], in[c], h[s][c]);
-            if (t0 + s < p.T) write_out<T, CPL, (ALIGN >= 4)>(y + (long long)(t0 + s) * p.D, h[s], left);
+            if (s < steps) write_out<T, CPL, (ALIGN >= 4)>(to, h[s], left);
         }
     }
     if (warp == 0 && rank == 0) write_state<CPL>(p.last + at_state, carry, left);
 }
 
 template <class T, int CPL, int S, int ALIGN>
-__global__ void __launch_bounds__(512) rec_bwd(const RecArgs p) {
+__global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
     constexpr int C = 32 * CPL;
     extern __shared__ __align__(128) unsigned char smem[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
     T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x, dy][rows][C]
-    float* maps = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T));   // [2][A, H, E][W][C]
-    float* peers = maps + 6 * W * C;                                          // [2][block][A, E][C]
+    float* maps = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T));   // [H, E][W][C]{A, H or E}
+    float* peers = maps + 4 * W * C;                                          // [2][block][C]{A, E}
     const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
     const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
     const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
@@ -280,9 +297,8 @@ __global__ void __launch_bounds__(512) rec_bwd(const RecArgs p) {
         const T* sg = stage + (k & 1) * 3 * rows * C + warp * S * C + lane * CPL;
         const T* sx = sg + rows * C;
         const T* sd = sx + rows * C;
-        float* mA = maps + (k & 1) * 3 * W * C + lane * CPL;
-        float* mH = mA + W * C;
-        float* mE = mH + W * C;
+        float* mapH = maps + lane * CPL * 2;        // {A, H}, then {A, E}
+        float* mapE = mapH + 2 * W * C;
         cp_wait<0>();
         __syncthreads();                                  // the stage is there, and the other one has been read
         issue(k + 1);
@@ -311,50 +327,36 @@ __global__ void __launch_bounds__(512) rec_bwd(const RecArgs p) {
 #pragma unroll
             for (int c = 0; c < CPL; ++c) E[c] = (E[c] + v[c]) * a[s][c];
         }
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-            mA[warp * C + c] = A[c];
-            mH[warp * C + c] = H[c];
-            mE[warp * C + c] = E[c];
-        }
+        write_map<CPL>(mapH + warp * 2 * C, A, H);
+        write_map<CPL>(mapE + warp * 2 * C, A, E);
         __syncthreads();
-        for (int w = 0; w < warp; ++w)
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) hb[c] = fmaf(mA[w * C + c], hb[c], mH[w * C + c]);
-        float preA[CPL], preE[CPL];
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) { A[c] = preA[c] = 1.f; E[c] = preE[c] = 0.f; }
-        for (int w = W - 1; w >= 0; --w) {
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                if (w == warp) { preA[c] = A[c]; preE[c] = E[c]; }
-                const float aw = mA[w * C + c];
-                E[c] = fmaf(aw, E[c], mE[w * C + c]);
-                A[c] *= aw;
-            }
-        }
+        for (int w = 0; w < warp; ++w) apply_map<CPL>(mapH + w * 2 * C, hb);
         float e[CPL];
         if (p.split == 1) {
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                e[c] = fmaf(preA[c], carry[c], preE[c]);
-                carry[c] = fmaf(A[c], carry[c], E[c]);
-            }
+            for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+            for (int w = W - 1; w > warp; --w) apply_map<CPL>(mapE + w * 2 * C, e);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) carry[c] = e[c];
+            for (int w = warp; w >= 0; --w) apply_map<CPL>(mapE + w * 2 * C, carry);
         } else {
-            float* set = peers + (k & 1) * kMaxCluster * 2 * C + lane * CPL;
-            for (int j = warp; j < p.split; j += W)
+            float* set = peers + ((k & 1) * kMaxCluster * C + lane * CPL) * 2;
+            if (warp < p.split) {
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) { A[c] = 1.f; E[c] = 0.f; }
+                for (int w = W - 1; w >= 0; --w) join_map<CPL>(mapE + w * 2 * C, A, E);
 #pragma unroll
                 for (int c = 0; c < CPL; ++c) {
-                    store_peer(set + (2 * rank) * C + c, j, A[c]);
-                    store_peer(set + (2 * rank + 1) * C + c, j, E[c]);
+                    store_peer(set + rank * 2 * C + 2 * c, warp, A[c]);
+                    store_peer(set + rank * 2 * C + 2 * c + 1, warp, E[c]);
                 }
+            }
             cluster_sync();
-            for (int j = p.split - 1; j >= 0; --j)
+            for (int j = p.split - 1; j > rank; --j) apply_map<CPL>(set + j * 2 * C, carry);
 #pragma unroll
-                for (int c = 0; c < CPL; ++c) {
-                    if (j == rank) e[c] = fmaf(preA[c], carry[c], preE[c]);
-                    carry[c] = fmaf(set[(2 * j) * C + c], carry[c], set[(2 * j + 1) * C + c]);
-                }
+            for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+            for (int w = W - 1; w > warp; --w) apply_map<CPL>(mapE + w * 2 * C, e);
+            for (int j = rank; j >= 0; --j) apply_map<CPL>(set + j * 2 * C, carry);
         }
         // dgate's factor (h_{t-1} - x_t) a z of each step, the states run again
         float f[S][CPL];
@@ -368,8 +370,11 @@ __global__ void __launch_bounds__(512) rec_bwd(const RecArgs p) {
                 hb[c] = fmaf(a[s][c], hb[c], z[s][c] * v[c]);
             }
         }
+        const int steps = p.T - t0;
+        const long long end = (long long)(t0 + S - 1) * p.D;
+        T *to_g = dgate + end, *to_x = dx + end;
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
+        for (int s = S - 1; s >= 0; --s, to_g -= p.D, to_x -= p.D) {
             float v[CPL], dg[CPL], dv[CPL];
             read_row<T, CPL>(sd + s * C, v);
 #pragma unroll
@@ -379,9 +384,9 @@ __global__ void __launch_bounds__(512) rec_bwd(const RecArgs p) {
                 dv[c] = e[c] * z[s][c];
                 e[c] *= a[s][c];
             }
-            if (t0 + s < p.T) {
-                write_out<T, CPL, (ALIGN >= 4)>(dgate + (long long)(t0 + s) * p.D, dg, left);
-                write_out<T, CPL, (ALIGN >= 4)>(dx + (long long)(t0 + s) * p.D, dv, left);
+            if (s < steps) {
+                write_out<T, CPL, (ALIGN >= 4)>(to_g, dg, left);
+                write_out<T, CPL, (ALIGN >= 4)>(to_x, dv, left);
             }
         }
     }
@@ -389,7 +394,8 @@ __global__ void __launch_bounds__(512) rec_bwd(const RecArgs p) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
-constexpr int kStepsFwd = 16, kStepsBwd = 16;
+constexpr int kWarpsFwd = 8, kWarpsBwd = 16, kSteps = 16;     // a whole piece of the backward pass is kSaved steps
+static_assert(kWarpsBwd * kSteps == kSaved && kSaved % kSteps == 0, "pieces begin where states are saved");
 
 bool rec_shape_ok(int64_t B, int64_t T, int D) { return B > 0 && T > 0 && D > 0; }
 constexpr long long kMax32 = (1LL << 31) - 1;
@@ -426,21 +432,20 @@ int rec_align(int es, int D, std::initializer_list<const void*> ptrs, std::initi
 
 template <class T, int CPL, int ALIGN, bool BWD>
 int rec_launch(RecArgs a, cudaStream_t s) {
-    constexpr int S = BWD ? kStepsBwd : kStepsFwd;
+    constexpr int S = kSteps, MAXW = BWD ? kWarpsBwd : kWarpsFwd;
     DeviceFacts f;
     if (int rc = device_facts(f)) return rc;
-    const int C = 32 * CPL, W = a.T >= 16 * S ? 16 : (a.T + S - 1) / S;
+    const int C = 32 * CPL, W = a.T >= MAXW * S ? MAXW : (a.T + S - 1) / S;
     a.groups = (a.D + C - 1) / C;
     const long long groups = (long long)a.B * a.groups;
     const int pieces = (a.T + W * S - 1) / (W * S);
+    // blocks that share a group: a power of two that the GPU has room for all at once and that all get work; a
+    // sequence of several pieces has MAXW >= kMaxCluster warps in a block
+    const long long room = (long long)f.sms * (BWD ? 1 : 2);
     int split = 1;
-    if (groups < f.sms) {
-        split = (int)(f.sms / groups);
-        split = split > kMaxCluster ? kMaxCluster : split;
-        split = split > pieces ? pieces : split;
-    }
+    while (2 * split <= kMaxCluster && 2 * split <= pieces && groups * 2 * split <= room) split *= 2;
     a.split = split;
-    const size_t smem = rec_smem<T, CPL>(W, S, BWD ? 3 : 2, BWD ? 3 : 2, split);
+    const size_t smem = rec_smem<T, CPL>(W, S, BWD ? 3 : 2, BWD ? 2 : 1, split);
     if (groups * split > kMax32) return HFUSE_ERR_TOO_LARGE;
     if constexpr (BWD) return launch_cluster(rec_bwd<T, CPL, S, ALIGN>, (int)(groups * split), W * 32, smem, split, s, a);
     else return launch_cluster(rec_fwd<T, CPL, S, ALIGN>, (int)(groups * split), W * 32, smem, split, s, a);
