@@ -63,28 +63,30 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 
 // Steps from T on get `beyond` (a gate of +infinity and an x of zero leave the state as it is), channels from D on are
 // left alone: no result of theirs is stored.
-template <class T, int CPL, int ALIGN>
+template <class T, int CPL, int ALIGN, int S>
 __device__ __forceinline__ void stage_rows(T* dst, const T* src, long long stride, int t0, int rows, int d0, int T_end, int D,
                                            float beyond) {
     constexpr int C = 32 * CPL, E = ALIGN >= (int)sizeof(T) ? ALIGN / (int)sizeof(T) : 1, PER = C / E;
-    static_assert(PER <= 64 && 32 % (PER < 32 ? PER : 32) == 0, "a thread stays in its column");
-    constexpr int COLS = PER < 32 ? PER : 32;                // columns that a warp covers at a time
-    const int step = blockDim.x / COLS;
+    constexpr int COLS = PER < 32 ? PER : 32;                // accesses of a row that a warp has in its lanes
+    const int step = blockDim.x / COLS, r0 = threadIdx.x / COLS, in = T_end - t0;
+#pragma unroll
     for (int k0 = 0; k0 < PER; k0 += COLS) {
         const int k = (k0 + threadIdx.x % COLS) * E;
         if (d0 + k >= D) continue;
-        int r = threadIdx.x / COLS;
-        const T* from = src + (long long)(t0 + r) * stride + d0 + k;
-        T* to = dst + r * C + k;
-        const int in = min(rows, T_end - t0);
-        for (; r < in; r += step, from += step * stride, to += step * C) {
-            if constexpr (ALIGN == 16) cp_async16(to, from);
-            else if constexpr (ALIGN == 4) cp_async4(to, from);
-            else *to = *from;
-        }
-        for (; r < rows; r += step, to += step * C) {
+        const T* from = src + (long long)(t0 + r0) * stride + d0 + k;
+        T* to = dst + r0 * C + k;
 #pragma unroll
-            for (int j = 0; j < E; ++j) to[j] = from_f32<T>(beyond);
+        for (int j = 0; j < S * COLS / 32; ++j) {            // rows / step
+            if (r0 + j * step < in) {
+                if constexpr (ALIGN == 16) cp_async16(to, from);
+                else if constexpr (ALIGN == 4) cp_async4(to, from);
+                else *to = *from;
+            } else {
+#pragma unroll
+                for (int q = 0; q < E; ++q) to[q] = from_f32<T>(beyond);
+            }
+            from += step * stride;
+            to += step * C;
         }
     }
 }
@@ -146,19 +148,61 @@ __device__ __forceinline__ void join_map(const float* m, float (&A)[CPL], float 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void store_peer(float* p, int rank, float v) {
+__device__ __forceinline__ uint32_t at_peer(const void* p, int rank) {
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+    return at;
 }
+// one channel's map into a peer's shared memory; its 8 bytes are counted on the peer's mbarrier, so neither side needs
+// a fence or a barrier of the whole cluster
+__device__ __forceinline__ void send_map(uint32_t to, uint32_t bar, float A, float H) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(A), "f"(H),
+                 "r"(bar)
+                 : "memory");
+}
+constexpr unsigned long long kPeerWaitNs = 2000000000ull;
+
+// The maps of all blocks of the cluster: sets of maps that alternate, each with an mbarrier.  A block sends a set only
+// after all its warps have read the last one, and it receives a set only after every block has sent the one before,
+// so no set is written while it is read.
+template <int CPL>
+struct Peers {
+    static constexpr int C = 32 * CPL;
+    float* sets;                   // [2][kMaxCluster][C]{A, H}
+    unsigned long long* bars;      // [2]
+    int split, rank;
+    bool lost = false;             // a wait ran out: results become NaN
+
+    __device__ __forceinline__ void begin() {
+        if (threadIdx.x == 0) {
+            mbar_init(bars, 1);
+            mbar_init(bars + 1, 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+        cluster_sync();            // every block's barriers are there
+    }
+    // called by the warps below `split`: warp j sends to block j
+    __device__ __forceinline__ void send(int it, int warp, int lane, const float (&A)[CPL], const float (&H)[CPL]) {
+        if (threadIdx.x == 0) mbar_expect_tx(bars + (it & 1), (uint32_t)(split * C * 8));
+        const uint32_t bar = at_peer(bars + (it & 1), warp);
+        const uint32_t to = at_peer(sets + (((it & 1) * kMaxCluster + rank) * C + lane * CPL) * 2, warp);
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) send_map(to + 8 * c, bar, A[c], H[c]);
+    }
+    __device__ __forceinline__ const float* receive(int it, int lane) {
+        if (!lost) lost = !mbar_wait<true>(bars + (it & 1), (it >> 1) & 1, kPeerWaitNs);
+        return sets + ((it & 1) * kMaxCluster * C + lane * CPL) * 2;
+    }
+};
 
 // shared memory of a block: two stages of `tensors` tiles, the warps' maps (`maps` per channel; the barrier at the top of a
-// piece is behind their last reader), two sets of the blocks' maps
+// piece is behind their last reader), the state that goes on to the next piece, the blocks' maps
 template <class T, int CPL>
 size_t rec_smem(int warps, int steps, int tensors, int maps, int split) {
     const size_t C = 32 * CPL;
-    return 2 * (size_t)tensors * warps * steps * C * sizeof(T) + (size_t)maps * warps * C * 8 +
-           (split > 1 ? 2 * (size_t)kMaxCluster * C * 8 : 0);
+    return 2 * (size_t)tensors * warps * steps * C * sizeof(T) + (size_t)maps * warps * C * 8 + C * 4 +
+           (split > 1 ? 2 * (size_t)kMaxCluster * C * 8 + 16 : 0);
 }
 
 template <class T, int CPL, int S, int ALIGN>
@@ -167,9 +211,11 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
     extern __shared__ __align__(128) unsigned char smem[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
     T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x][rows][C]
-    float* maps = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T));   // [W][C]{A, H}
-    float* peers = maps + 2 * W * C;                                          // [2][block][C]{A, H}
+    float* map = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T)) + lane * CPL * 2;   // [W][C]{A, H}
+    float* next = map - lane * CPL * 2 + 2 * W * C + lane * CPL;              // [C]
     const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
+    Peers<CPL> peers{next - lane * CPL + C, nullptr, p.split, rank};
+    peers.bars = reinterpret_cast<unsigned long long*>(peers.sets + 2 * kMaxCluster * C * 2);
     const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
     const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
     const T* x = static_cast<const T*>(p.x) + b * p.x_b;
@@ -181,8 +227,8 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
         if (it < n) {
             T* s = stage + (it & 1) * 2 * rows * C;
             const int t0 = (it * p.split + rank) * rows;
-            stage_rows<T, CPL, ALIGN>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
-            stage_rows<T, CPL, ALIGN>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
+            stage_rows<T, CPL, ALIGN, S>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
+            stage_rows<T, CPL, ALIGN, S>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
         }
         cp_commit();
     };
@@ -190,14 +236,14 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
     issue(1);
     float carry[CPL];                                     // the state before the cluster's next piece
     read_state<CPL>(p.h0 ? p.h0 + at_state : nullptr, carry, left);
-    if (p.split > 1) cluster_sync();                      // the peers' shared memory is there
+    if (p.split > 1) peers.begin();
     for (int it = 0; it < n; ++it) {
         const int t0 = (it * p.split + rank) * rows + warp * S;
         const T* sg = stage + (it & 1) * 2 * rows * C + warp * S * C + lane * CPL;
         const T* sx = sg + rows * C;
-        float* map = maps + lane * CPL * 2;           // {A, H} of each channel, a warp in 2 C floats
         cp_wait<1>();
         __syncthreads();
+        if (p.split == 1 && it > 0) read_row<float, CPL>(next, carry);
         float h[S][CPL], a[S][CPL], H[CPL], A[CPL];
 #pragma unroll
         for (int c = 0; c < CPL; ++c) { H[c] = 0.f; A[c] = 1.f; }
@@ -223,28 +269,33 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
         if (p.split == 1) {
 #pragma unroll
             for (int c = 0; c < CPL; ++c) in[c] = carry[c];
+#pragma unroll 4
             for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
+            if (warp == W - 1) {                          // what the block's last step leaves
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) carry[c] = in[c];
-            for (int w = warp; w < W; ++w) apply_map<CPL>(map + w * 2 * C, carry);
+                for (int c = 0; c < CPL; ++c) next[c] = carry[c] = fmaf(A[c], in[c], H[c]);
+            }
         } else {
-            float* set = peers + ((it & 1) * kMaxCluster * C + lane * CPL) * 2;
             if (warp < p.split) {                         // W >= split: see rec_launch
 #pragma unroll
                 for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = 0.f; }
+#pragma unroll 4
                 for (int w = 0; w < W; ++w) join_map<CPL>(map + w * 2 * C, A, H);
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) {
-                    store_peer(set + rank * 2 * C + 2 * c, warp, A[c]);
-                    store_peer(set + rank * 2 * C + 2 * c + 1, warp, H[c]);
-                }
+                peers.send(it, warp, lane, A, H);
             }
-            cluster_sync();
+            const float* set = peers.receive(it, lane);
+#pragma unroll 4
             for (int j = 0; j < rank; ++j) apply_map<CPL>(set + j * 2 * C, carry);
 #pragma unroll
             for (int c = 0; c < CPL; ++c) in[c] = carry[c];
+#pragma unroll 4
             for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
+#pragma unroll 4
             for (int j = rank; j < p.split; ++j) apply_map<CPL>(set + j * 2 * C, carry);
+            if (peers.lost) {
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) in[c] = carry[c] = __int_as_float(0x7fc00000);
+            }
         }
         if (p.states && t0 < p.T && t0 % kSaved == 0)
             write_state<CPL>(p.states + ((long long)b * p.chunks + t0 / kSaved) * p.D + d, in, left);
@@ -257,7 +308,8 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
             if (s < steps) write_out<T, CPL, (ALIGN >= 4)>(to, h[s], left);
         }
     }
-    if (warp == 0 && rank == 0) write_state<CPL>(p.last + at_state, carry, left);
+    if (warp == W - 1 && rank == 0) write_state<CPL>(p.last + at_state, carry, left);
+    if (p.split > 1) cluster_sync();                      // no block ends while a peer may still write to it
 }
 
 template <class T, int CPL, int S, int ALIGN>
@@ -266,9 +318,12 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
     extern __shared__ __align__(128) unsigned char smem[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
     T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x, dy][rows][C]
-    float* maps = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T));   // [H, E][W][C]{A, H or E}
-    float* peers = maps + 4 * W * C;                                          // [2][block][C]{A, E}
+    float* mapH = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T)) + lane * CPL * 2;  // [W][C]{A, H}
+    float* mapE = mapH + 2 * W * C;                                           // [W][C]{A, E}
+    float* next = mapH - lane * CPL * 2 + 4 * W * C + lane * CPL;             // [C]
     const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
+    Peers<CPL> peers{next - lane * CPL + C, nullptr, p.split, rank};
+    peers.bars = reinterpret_cast<unsigned long long*>(peers.sets + 2 * kMaxCluster * C * 2);
     const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
     const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
     const T* x = static_cast<const T*>(p.x) + b * p.x_b;
@@ -282,81 +337,82 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
         if (k < n) {
             T* s = stage + (k & 1) * 3 * rows * C;
             const int t0 = ((n - 1 - k) * p.split + rank) * rows;
-            stage_rows<T, CPL, ALIGN>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
-            stage_rows<T, CPL, ALIGN>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
-            stage_rows<T, CPL, ALIGN>(s + 2 * rows * C, dy, p.dy_t, t0, rows, d0, p.T, p.D, 0.f);
+            stage_rows<T, CPL, ALIGN, S>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
+            stage_rows<T, CPL, ALIGN, S>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
+            stage_rows<T, CPL, ALIGN, S>(s + 2 * rows * C, dy, p.dy_t, t0, rows, d0, p.T, p.D, 0.f);
         }
         cp_commit();
     };
     issue(0);
     float carry[CPL];                                     // a e of the step after the cluster's next piece
     read_state<CPL>(p.dlast ? p.dlast + at_state : nullptr, carry, left);
-    if (p.split > 1) cluster_sync();
+    if (p.split > 1) peers.begin();
     for (int k = 0; k < n; ++k) {
         const int first = ((n - 1 - k) * p.split + rank) * rows, t0 = first + warp * S;
         const T* sg = stage + (k & 1) * 3 * rows * C + warp * S * C + lane * CPL;
         const T* sx = sg + rows * C;
         const T* sd = sx + rows * C;
-        float* mapH = maps + lane * CPL * 2;        // {A, H}, then {A, E}
-        float* mapE = mapH + 2 * W * C;
-        cp_wait<0>();
-        __syncthreads();                                  // the stage is there, and the other one has been read
-        issue(k + 1);
         // a block's piece begins where the forward pass saved a state
         float hb[CPL];
         read_state<CPL>(first < p.T ? p.states + ((long long)b * p.chunks + first / kSaved) * p.D + d : nullptr, hb, left);
+        cp_wait<0>();
+        __syncthreads();                                  // the stage is there, and the other one has been read
+        issue(k + 1);
+        if (p.split == 1 && k > 0) read_row<float, CPL>(next, carry);
+        // E, what e of zero becomes over the steps, is the sum of dy_t times the product of the a up to a_t
         float a[S][CPL], z[S][CPL], A[CPL], H[CPL], E[CPL];
 #pragma unroll
         for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = E[c] = 0.f; }
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            float g[CPL], v[CPL];
+            float g[CPL], v[CPL], u[CPL];
             read_row<T, CPL>(sg + s * C, g);
             read_row<T, CPL>(sx + s * C, v);
+            read_row<T, CPL>(sd + s * C, u);
 #pragma unroll
             for (int c = 0; c < CPL; ++c) {
                 gates(g[c], a[s][c], z[s][c]);
                 H[c] = fmaf(a[s][c], H[c], z[s][c] * v[c]);
                 A[c] *= a[s][c];
+                E[c] = fmaf(A[c], u[c], E[c]);
             }
-        }
-#pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            float v[CPL];
-            read_row<T, CPL>(sd + s * C, v);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) E[c] = (E[c] + v[c]) * a[s][c];
         }
         write_map<CPL>(mapH + warp * 2 * C, A, H);
         write_map<CPL>(mapE + warp * 2 * C, A, E);
         __syncthreads();
+#pragma unroll 4
         for (int w = 0; w < warp; ++w) apply_map<CPL>(mapH + w * 2 * C, hb);
         float e[CPL];
         if (p.split == 1) {
 #pragma unroll
             for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+#pragma unroll 4
             for (int w = W - 1; w > warp; --w) apply_map<CPL>(mapE + w * 2 * C, e);
+            if (warp == 0) {
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) carry[c] = e[c];
-            for (int w = warp; w >= 0; --w) apply_map<CPL>(mapE + w * 2 * C, carry);
+                for (int c = 0; c < CPL; ++c) next[c] = carry[c] = fmaf(A[c], e[c], E[c]);
+            }
         } else {
-            float* set = peers + ((k & 1) * kMaxCluster * C + lane * CPL) * 2;
             if (warp < p.split) {
 #pragma unroll
                 for (int c = 0; c < CPL; ++c) { A[c] = 1.f; E[c] = 0.f; }
+#pragma unroll 4
                 for (int w = W - 1; w >= 0; --w) join_map<CPL>(mapE + w * 2 * C, A, E);
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) {
-                    store_peer(set + rank * 2 * C + 2 * c, warp, A[c]);
-                    store_peer(set + rank * 2 * C + 2 * c + 1, warp, E[c]);
-                }
+                peers.send(k, warp, lane, A, E);
             }
-            cluster_sync();
+            const float* set = peers.receive(k, lane);
+#pragma unroll 4
             for (int j = p.split - 1; j > rank; --j) apply_map<CPL>(set + j * 2 * C, carry);
 #pragma unroll
             for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+#pragma unroll 4
             for (int w = W - 1; w > warp; --w) apply_map<CPL>(mapE + w * 2 * C, e);
+#pragma unroll 4
             for (int j = rank; j >= 0; --j) apply_map<CPL>(set + j * 2 * C, carry);
+            if (peers.lost) {
+#pragma unroll
+                for (int c = 0; c < CPL; ++c) e[c] = carry[c] = __int_as_float(0x7fc00000);
+            }
         }
         // dgate's factor (h_{t-1} - x_t) a z of each step, the states run again
         float f[S][CPL];
@@ -391,6 +447,7 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
         }
     }
     if (warp == 0 && rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
+    if (p.split > 1) cluster_sync();
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
