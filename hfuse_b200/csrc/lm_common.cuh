@@ -92,6 +92,21 @@ __device__ __forceinline__ void store_stream(T* p, const Pack<T, N>& r) {
     }
 }
 
+// two neighbouring elements, one 32-bit word where they are 16-bit
+template <class T>
+__device__ __forceinline__ float2 unpack2(const Pack<T, 2>& p) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        unsigned u;
+        memcpy(&u, &p, 4);
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    } else if constexpr (std::is_same_v<T, __half>) {
+        __half2 h;
+        memcpy(&h, &p, 4);
+        return __half22float2(h);
+    } else {
+        return make_float2(p.v[0], p.v[1]);
+    }
+}
 // N floats rounded to T
 template <class T, int N>
 __device__ __forceinline__ Pack<T, N> pack_f32(const float (&v)[N]) {
@@ -115,6 +130,36 @@ __device__ __forceinline__ Pack<T, N> pack_f32(const float (&v)[N]) {
     }
     return r;
 }
+
+// two floats in one instruction: these kernels are short of issue slots sooner than of arithmetic
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r, x, y, z;
+    memcpy(&x, &a, 8);
+    memcpy(&y, &b, 8);
+    memcpy(&z, &c, 8);
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    memcpy(&a, &r, 8);
+    return a;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r, x, y;
+    memcpy(&x, &a, 8);
+    memcpy(&y, &b, 8);
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    memcpy(&a, &r, 8);
+    return a;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r, x, y;
+    memcpy(&x, &a, 8);
+    memcpy(&y, &b, 8);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    memcpy(&a, &r, 8);
+    return a;
+}
+
+// the warp's index in its block, known to the compiler to be the same in all lanes
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0); }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -38,15 +38,19 @@ struct RecArgs {
 };
 
 // a = sigmoid(g) and z = 1 - a = sigmoid(-g), both to a few units in their last place: with e = exp(-g),
-// a = 1 / (1 + e) and z = e a.  The exponent stops at 126 so that e a cannot be infinity times zero (the
-// subtraction then makes an a of 2^-126 the zero that a gate of -infinity stands for); a NaN stays one.
-__device__ __forceinline__ void gates(float g, float& a, float& z) {
-    float t = g * -1.4426950408889634f, e;
-    asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.f + e));
-    z = e * a;
-    a -= 0x1p-126f;
+// a = 1 / (1 + e) and z = e a.  A gate of -infinity has e = infinity, a = 0 and z = min(infinity * 0, 1) = 1 (the minimum
+// of a NaN and a number is the number); a gate that is a NaN makes a one.
+__device__ __forceinline__ void gates2(float2 g, float2& a, float2& z) {
+    const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    float2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    const float2 d = add2(e, make_float2(1.f, 1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a.x) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a.y) : "f"(d.y));
+    z = mul2(e, a);
+    z.x = fminf(z.x, 1.f);
+    z.y = fminf(z.y, 1.f);
 }
 
 // ---- staging: `rows` steps of 32 * CPL channels into shared memory ----------------------------------------
@@ -97,14 +101,63 @@ __device__ __forceinline__ void read_row(const T* row, float (&v)[CPL]) {
 #pragma unroll
     for (int c = 0; c < CPL; ++c) v[c] = to_f32(p.v[c]);
 }
-template <class T, int CPL, bool WHOLE>
-__device__ __forceinline__ void write_out(T* p, const float (&v)[CPL], int left) {
-    if constexpr (WHOLE) {                 // rows keep the alignment of CPL elements, D is a multiple of CPL
-        if (left > 0) store_stream<T, CPL>(p, pack_f32<T, CPL>(v));
+// Elements are worked on in pairs: the two channels of a lane, or two steps of its only channel.
+template <class T, int CPL>
+__device__ __forceinline__ float2 read_pair(const T* at, int i) {
+    constexpr int C = 32 * CPL;
+    if constexpr (CPL == 2) {
+        return unpack2(*reinterpret_cast<const Pack<T, 2>*>(at + i * C));
     } else {
-#pragma unroll
-        for (int c = 0; c < CPL; ++c)
-            if (c < left) p[c] = from_f32<T>(v[c]);
+        return make_float2(to_f32(at[2 * i * C]), to_f32(at[(2 * i + 1) * C]));
+    }
+}
+// h -> a h + b over a pair; `all` are the results (before: what h was ahead of each)
+template <int CPL>
+__device__ __forceinline__ float2 run_pair(float2 a, float2 b, float (&h)[CPL], float2* before = nullptr) {
+    if constexpr (CPL == 2) {
+        const float2 old = make_float2(h[0], h[1]), r = fma2(a, old, b);
+        h[0] = r.x;
+        h[1] = r.y;
+        if (before) *before = old;
+        return r;
+    } else {
+        const float x = fmaf(a.x, h[0], b.x), y = fmaf(a.y, x, b.y);
+        if (before) *before = make_float2(h[0], x);
+        h[0] = y;
+        return make_float2(x, y);
+    }
+}
+// the same for a product
+template <int CPL>
+__device__ __forceinline__ float2 scale_pair(float2 a, float (&A)[CPL]) {
+    if constexpr (CPL == 2) {
+        const float2 r = mul2(a, make_float2(A[0], A[1]));
+        A[0] = r.x;
+        A[1] = r.y;
+        return r;
+    } else {
+        const float x = a.x * A[0], y = a.y * x;
+        A[0] = y;
+        return make_float2(x, y);
+    }
+}
+template <int CPL>
+__device__ __forceinline__ float2 both(const float (&v)[CPL]) { return make_float2(v[0], v[CPL - 1]); }
+
+// a pair to its place: `steps` steps and `left` channels are there
+template <class T, int CPL, bool WHOLE>
+__device__ __forceinline__ void write_pair(T* at, long long stride, int i, float2 v, int steps, int left) {
+    if constexpr (CPL == 2) {
+        if constexpr (WHOLE) {             // rows keep the alignment of two elements, D is even
+            const float w[2] = {v.x, v.y};
+            if (i < steps && left > 0) store_stream<T, 2>(at + i * stride, pack_f32<T, 2>(w));
+        } else if (i < steps) {
+            if (left > 0) at[i * stride] = from_f32<T>(v.x);
+            if (left > 1) at[i * stride + 1] = from_f32<T>(v.y);
+        }
+    } else if (left > 0) {
+        if (2 * i < steps) store_stream<T, 1>(at + 2 * i * stride, Pack<T, 1>{{from_f32<T>(v.x)}});
+        if (2 * i + 1 < steps) store_stream<T, 1>(at + (2 * i + 1) * stride, Pack<T, 1>{{from_f32<T>(v.y)}});
     }
 }
 template <int CPL>
@@ -207,9 +260,9 @@ size_t rec_smem(int warps, int steps, int tensors, int maps, int split) {
 
 template <class T, int CPL, int S, int ALIGN>
 __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
-    constexpr int C = 32 * CPL;
+    constexpr int C = 32 * CPL, N = S * CPL / 2;
     extern __shared__ __align__(128) unsigned char smem[];
-    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
+    const int W = blockDim.x >> 5, warp = warp_index(), lane = threadIdx.x & 31, rows = W * S;
     T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x][rows][C]
     float* map = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T)) + lane * CPL * 2;   // [W][C]{A, H}
     float* next = map - lane * CPL * 2 + 2 * W * C + lane * CPL;              // [C]
@@ -244,23 +297,16 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
         cp_wait<1>();
         __syncthreads();
         if (p.split == 1 && it > 0) read_row<float, CPL>(next, carry);
-        float h[S][CPL], a[S][CPL], H[CPL], A[CPL];
+        float2 h[N], a[N];                                // results from zero, products of the a so far
+        float H[CPL], A[CPL];
 #pragma unroll
         for (int c = 0; c < CPL; ++c) { H[c] = 0.f; A[c] = 1.f; }
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float g[CPL], v[CPL];
-            read_row<T, CPL>(sg + s * C, g);
-            read_row<T, CPL>(sx + s * C, v);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                float at, zt;
-                gates(g[c], at, zt);
-                H[c] = fmaf(at, H[c], zt * v[c]);
-                A[c] *= at;
-                h[s][c] = H[c];
-                a[s][c] = A[c];
-            }
+        for (int i = 0; i < N; ++i) {
+            float2 at, zt;
+            gates2(read_pair<T, CPL>(sg, i), at, zt);
+            h[i] = run_pair<CPL>(at, mul2(zt, read_pair<T, CPL>(sx, i)), H);
+            a[i] = scale_pair<CPL>(at, A);
         }
         write_map<CPL>(map + warp * 2 * C, A, H);
         __syncthreads();
@@ -300,12 +346,14 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
         if (p.states && t0 < p.T && t0 % kSaved == 0)
             write_state<CPL>(p.states + ((long long)b * p.chunks + t0 / kSaved) * p.D + d, in, left);
         T* to = y + (long long)t0 * p.D;
-        const int steps = p.T - t0;
 #pragma unroll
-        for (int s = 0; s < S; ++s, to += p.D) {
+        for (int i = 0; i < N; ++i) h[i] = fma2(a[i], both<CPL>(in), h[i]);
+        if (p.T - t0 >= S) {
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) h[s][c] = fmaf(a[s][c], in[c], h[s][c]);
-            if (s < steps) write_out<T, CPL, (ALIGN >= 4)>(to, h[s], left);
+            for (int i = 0; i < N; ++i) write_pair<T, CPL, (ALIGN >= 4)>(to, p.D, i, h[i], S, left);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) write_pair<T, CPL, (ALIGN >= 4)>(to, p.D, i, h[i], p.T - t0, left);
         }
     }
     if (warp == W - 1 && rank == 0) write_state<CPL>(p.last + at_state, carry, left);
@@ -314,9 +362,9 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
 
 template <class T, int CPL, int S, int ALIGN>
 __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
-    constexpr int C = 32 * CPL;
+    constexpr int C = 32 * CPL, N = S * CPL / 2;
     extern __shared__ __align__(128) unsigned char smem[];
-    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = W * S;
+    const int W = blockDim.x >> 5, warp = warp_index(), lane = threadIdx.x & 31, rows = W * S;
     T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x, dy][rows][C]
     float* mapH = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T)) + lane * CPL * 2;  // [W][C]{A, H}
     float* mapE = mapH + 2 * W * C;                                           // [W][C]{A, E}
@@ -360,21 +408,21 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
         issue(k + 1);
         if (p.split == 1 && k > 0) read_row<float, CPL>(next, carry);
         // E, what e of zero becomes over the steps, is the sum of dy_t times the product of the a up to a_t
-        float a[S][CPL], z[S][CPL], A[CPL], H[CPL], E[CPL];
+        float2 a[N], z[N];
+        float A[CPL], H[CPL], E[CPL];
 #pragma unroll
         for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = E[c] = 0.f; }
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float g[CPL], v[CPL], u[CPL];
-            read_row<T, CPL>(sg + s * C, g);
-            read_row<T, CPL>(sx + s * C, v);
-            read_row<T, CPL>(sd + s * C, u);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                gates(g[c], a[s][c], z[s][c]);
-                H[c] = fmaf(a[s][c], H[c], z[s][c] * v[c]);
-                A[c] *= a[s][c];
-                E[c] = fmaf(A[c], u[c], E[c]);
+        for (int i = 0; i < N; ++i) {
+            gates2(read_pair<T, CPL>(sg, i), a[i], z[i]);
+            run_pair<CPL>(a[i], mul2(z[i], read_pair<T, CPL>(sx, i)), H);
+            const float2 P = scale_pair<CPL>(a[i], A), u = read_pair<T, CPL>(sd, i);
+            if constexpr (CPL == 2) {
+                const float2 r = fma2(P, u, make_float2(E[0], E[1]));
+                E[0] = r.x;
+                E[1] = r.y;
+            } else {
+                E[0] = fmaf(P.y, u.y, fmaf(P.x, u.x, E[0]));
             }
         }
         write_map<CPL>(mapH + warp * 2 * C, A, H);
@@ -415,36 +463,36 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
             }
         }
         // dgate's factor (h_{t-1} - x_t) a z of each step, the states run again
-        float f[S][CPL];
+        float2 f[N];
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float v[CPL];
-            read_row<T, CPL>(sx + s * C, v);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                f[s][c] = (hb[c] - v[c]) * (a[s][c] * z[s][c]);
-                hb[c] = fmaf(a[s][c], hb[c], z[s][c] * v[c]);
-            }
+        for (int i = 0; i < N; ++i) {
+            const float2 v = read_pair<T, CPL>(sx, i);
+            float2 before;
+            run_pair<CPL>(a[i], mul2(z[i], v), hb, &before);
+            f[i] = mul2(fma2(v, make_float2(-1.f, -1.f), before), mul2(a[i], z[i]));
         }
-        const int steps = p.T - t0;
-        const long long end = (long long)(t0 + S - 1) * p.D;
-        T *to_g = dgate + end, *to_x = dx + end;
+        T *to_g = dgate + (long long)t0 * p.D, *to_x = dx + (long long)t0 * p.D;
+        auto sweep = [&](int steps) {
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s, to_g -= p.D, to_x -= p.D) {
-            float v[CPL], dg[CPL], dv[CPL];
-            read_row<T, CPL>(sd + s * C, v);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-                e[c] += v[c];
-                dg[c] = e[c] * f[s][c];
-                dv[c] = e[c] * z[s][c];
-                e[c] *= a[s][c];
+            for (int i = N - 1; i >= 0; --i) {
+                const float2 u = read_pair<T, CPL>(sd, i);
+                float2 et;                                // e of the pair's steps
+                if constexpr (CPL == 2) {
+                    et = add2(make_float2(e[0], e[1]), u);
+                    const float2 r = mul2(et, a[i]);
+                    e[0] = r.x;
+                    e[1] = r.y;
+                } else {
+                    et.y = e[0] + u.y;
+                    et.x = fmaf(et.y, a[i].y, u.x);
+                    e[0] = et.x * a[i].x;
+                }
+                write_pair<T, CPL, (ALIGN >= 4)>(to_g, p.D, i, mul2(et, f[i]), steps, left);
+                write_pair<T, CPL, (ALIGN >= 4)>(to_x, p.D, i, mul2(et, z[i]), steps, left);
             }
-            if (s < steps) {
-                write_out<T, CPL, (ALIGN >= 4)>(to_g, dg, left);
-                write_out<T, CPL, (ALIGN >= 4)>(to_x, dv, left);
-            }
-        }
+        };
+        if (p.T - t0 >= S) sweep(S);
+        else sweep(p.T - t0);
     }
     if (warp == 0 && rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
     if (p.split > 1) cluster_sync();
