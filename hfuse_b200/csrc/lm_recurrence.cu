@@ -55,11 +55,11 @@ __device__ __forceinline__ void gates2(float2 g, float2& a, float2& z) {
 
 // ---- staging: `rows` steps of 32 * CPL channels into shared memory ----------------------------------------
 // ALIGN: bytes that every row's begin and the number of channels are a multiple of (16, 4, or one 16-bit element)
-__device__ __forceinline__ void cp_async16(void* s, const void* g) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s)), "l"(g) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t s, const void* g) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(__cvta_generic_to_global(g)) : "memory");
 }
-__device__ __forceinline__ void cp_async4(void* s, const void* g) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(s)), "l"(g) : "memory");
+__device__ __forceinline__ void cp_async4(uint32_t s, const void* g) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(__cvta_generic_to_global(g)) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -72,6 +72,7 @@ __device__ __forceinline__ void stage_rows(T* dst, const T* src, long long strid
                                            float beyond) {
     constexpr int C = 32 * CPL, E = ALIGN >= (int)sizeof(T) ? ALIGN / (int)sizeof(T) : 1, PER = C / E;
     constexpr int COLS = PER < 32 ? PER : 32;                // accesses of a row that a warp has in its lanes
+    constexpr int COUNT = S * COLS / 32;                     // accesses of a thread in its column: rows / step
     const int step = blockDim.x / COLS, r0 = threadIdx.x / COLS, in = T_end - t0;
 #pragma unroll
     for (int k0 = 0; k0 < PER; k0 += COLS) {
@@ -79,18 +80,26 @@ __device__ __forceinline__ void stage_rows(T* dst, const T* src, long long strid
         if (d0 + k >= D) continue;
         const T* from = src + (long long)(t0 + r0) * stride + d0 + k;
         T* to = dst + r0 * C + k;
+        const long long ahead = step * stride;
+        const uint32_t s0 = smem_u32(to), sahead = step * C * (int)sizeof(T);
+        if (in >= rows) {                                    // all pieces but a sequence's last one
 #pragma unroll
-        for (int j = 0; j < S * COLS / 32; ++j) {            // rows / step
-            if (r0 + j * step < in) {
-                if constexpr (ALIGN == 16) cp_async16(to, from);
-                else if constexpr (ALIGN == 4) cp_async4(to, from);
-                else *to = *from;
-            } else {
-#pragma unroll
-                for (int q = 0; q < E; ++q) to[q] = from_f32<T>(beyond);
+            for (int j = 0; j < COUNT; ++j) {
+                if constexpr (ALIGN == 16) cp_async16(s0 + j * sahead, from + j * ahead);
+                else if constexpr (ALIGN == 4) cp_async4(s0 + j * sahead, from + j * ahead);
+                else to[j * step * C] = from[j * ahead];
             }
-            from += step * stride;
-            to += step * C;
+        } else {
+            for (int j = 0; j < COUNT; ++j) {
+                if (r0 + j * step < in) {
+                    if constexpr (ALIGN == 16) cp_async16(s0 + j * sahead, from + j * ahead);
+                    else if constexpr (ALIGN == 4) cp_async4(s0 + j * sahead, from + j * ahead);
+                    else to[j * step * C] = from[j * ahead];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < E; ++q) to[j * step * C + q] = from_f32<T>(beyond);
+                }
+            }
         }
     }
 }
@@ -172,29 +181,31 @@ __device__ __forceinline__ void write_state(float* p, const float (&v)[CPL], int
         if (c < left) p[c] = v[c];
 }
 
-// ---- maps h -> A h + H of one stretch of steps in shared memory: {A, H} per channel ------------------------
+// ---- maps h -> A h + H of one stretch of steps in shared memory: a lane's A, then its H ---------------------
 template <int CPL>
 __device__ __forceinline__ void write_map(float* m, const float (&A)[CPL], const float (&H)[CPL]) {
     Pack<float, 2 * CPL> r;
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) { r.v[2 * c] = A[c]; r.v[2 * c + 1] = H[c]; }
+    for (int c = 0; c < CPL; ++c) { r.v[c] = A[c]; r.v[CPL + c] = H[c]; }
     *reinterpret_cast<Pack<float, 2 * CPL>*>(m) = r;
 }
 template <int CPL>
 __device__ __forceinline__ void apply_map(const float* m, float (&h)[CPL]) {
     const Pack<float, 2 * CPL> r = *reinterpret_cast<const Pack<float, 2 * CPL>*>(m);
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) h[c] = fmaf(r.v[2 * c], h[c], r.v[2 * c + 1]);
+    if constexpr (CPL == 2) {
+        const float2 n = fma2(make_float2(r.v[0], r.v[1]), make_float2(h[0], h[1]), make_float2(r.v[2], r.v[3]));
+        h[0] = n.x;
+        h[1] = n.y;
+    } else {
+        h[0] = fmaf(r.v[0], h[0], r.v[1]);
+    }
 }
 // the map of the steps so far, then m's
 template <int CPL>
 __device__ __forceinline__ void join_map(const float* m, float (&A)[CPL], float (&H)[CPL]) {
-    const Pack<float, 2 * CPL> r = *reinterpret_cast<const Pack<float, 2 * CPL>*>(m);
+    apply_map<CPL>(m, H);
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-        H[c] = fmaf(r.v[2 * c], H[c], r.v[2 * c + 1]);
-        A[c] *= r.v[2 * c];
-    }
+    for (int c = 0; c < CPL; ++c) A[c] *= m[c];
 }
 
 // ---- cluster: the blocks that share a group of channels --------------------------------------------------
@@ -206,9 +217,9 @@ __device__ __forceinline__ uint32_t at_peer(const void* p, int rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
     return at;
 }
-// one channel's map into a peer's shared memory; its 8 bytes are counted on the peer's mbarrier, so neither side needs
-// a fence or a barrier of the whole cluster
-__device__ __forceinline__ void send_map(uint32_t to, uint32_t bar, float A, float H) {
+// two floats of a map into a peer's shared memory; their 8 bytes are counted on the peer's mbarrier, so neither side
+// needs a fence or a barrier of the whole cluster
+__device__ __forceinline__ void send_two(uint32_t to, uint32_t bar, float A, float H) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(A), "f"(H),
                  "r"(bar)
                  : "memory");
@@ -240,8 +251,12 @@ struct Peers {
         if (threadIdx.x == 0) mbar_expect_tx(bars + (it & 1), (uint32_t)(split * C * 8));
         const uint32_t bar = at_peer(bars + (it & 1), warp);
         const uint32_t to = at_peer(sets + (((it & 1) * kMaxCluster + rank) * C + lane * CPL) * 2, warp);
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) send_map(to + 8 * c, bar, A[c], H[c]);
+        if constexpr (CPL == 2) {
+            send_two(to, bar, A[0], A[1]);
+            send_two(to + 8, bar, H[0], H[1]);
+        } else {
+            send_two(to, bar, A[0], H[0]);
+        }
     }
     __device__ __forceinline__ const float* receive(int it, int lane) {
         if (!lost) lost = !mbar_wait<true>(bars + (it & 1), (it >> 1) & 1, kPeerWaitNs);
