@@ -70,6 +70,16 @@ __device__ __forceinline__ Pack<T, N> load_cached(const T* p) {
     }
     return r;
 }
+// weights: N elements, in accesses of 16 bytes at most
+template <class T, int N>
+__device__ __forceinline__ void load_weights(const T* p, Pack<T, N>& r) {
+    constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+#pragma unroll
+    for (int k = 0; k < N; k += M) {
+        const Pack<T, M> q = load_cached<T, M>(p + k);
+        memcpy(r.v + k, q.v, sizeof(q));
+    }
+}
 // outputs that this kernel does not read again
 template <class T, int N>
 __device__ __forceinline__ void store_stream(T* p, const Pack<T, N>& r) {
@@ -106,6 +116,14 @@ __device__ __forceinline__ float2 unpack2(const Pack<T, 2>& p) {
     } else {
         return make_float2(p.v[0], p.v[1]);
     }
+}
+// the k-th pair of N elements
+template <class T, int N>
+__device__ __forceinline__ float2 pair_of(const Pack<T, N>& p, int k) {
+    Pack<T, 2> q;
+    q.v[0] = p.v[2 * k];
+    q.v[1] = p.v[2 * k + 1];
+    return unpack2(q);
 }
 // N floats rounded to T
 template <class T, int N>
