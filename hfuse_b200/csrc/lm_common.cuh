@@ -23,128 +23,101 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// N neighbouring elements as one memory access (2 to 16 bytes, aligned to its size)
+// N neighbouring elements as one memory access (2 to 32 bytes, aligned to its size, 16 at most), kept as the words that
+// were loaded: two 16-bit elements to a register
 template <class T, int N>
-struct alignas(N * sizeof(T)) Pack {
-    T v[N];
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
+    static constexpr int BYTES = N * (int)sizeof(T);
+    using Word = std::conditional_t<BYTES >= 4, unsigned, unsigned short>;
+    Word w[BYTES / sizeof(Word)];
 };
 // inputs that are read once bypass L1
 template <class T, int N>
 __device__ __forceinline__ Pack<T, N> load_stream(const T* p) {
     Pack<T, N> r;
-    if constexpr (sizeof(r) == 16) {
-        uint4 u;
-        asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
-        memcpy(&r, &u, 16);
-    } else if constexpr (sizeof(r) == 8) {
-        uint2 u;
-        asm("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
-        memcpy(&r, &u, 8);
-    } else if constexpr (sizeof(r) == 4) {
-        unsigned u;
-        asm("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(u) : "l"(p));
-        memcpy(&r, &u, 4);
-    } else {
-        unsigned short u;
-        asm("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(u) : "l"(p));
-        memcpy(&r, &u, 2);
-    }
+    if constexpr (r.BYTES == 16)
+        asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(p));
+    else if constexpr (r.BYTES == 8)
+        asm("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
+    else if constexpr (r.BYTES == 4)
+        asm("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r.w[0]) : "l"(p));
+    else
+        asm("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(r.w[0]) : "l"(p));
     return r;
 }
-// inputs that several blocks or rows read (weights, ids, states)
+// inputs that several blocks or rows read (weights, tables), in accesses of 16 bytes at most
 template <class T, int N>
 __device__ __forceinline__ Pack<T, N> load_cached(const T* p) {
     Pack<T, N> r;
-    if constexpr (sizeof(r) == 16) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        memcpy(&r, &u, 16);
-    } else if constexpr (sizeof(r) == 8) {
+    if constexpr (r.BYTES >= 16) {
+#pragma unroll
+        for (int k = 0; k < r.BYTES / 16; ++k) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + k);
+            r.w[4 * k] = u.x;
+            r.w[4 * k + 1] = u.y;
+            r.w[4 * k + 2] = u.z;
+            r.w[4 * k + 3] = u.w;
+        }
+    } else if constexpr (r.BYTES == 8) {
         const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-        memcpy(&r, &u, 8);
-    } else if constexpr (sizeof(r) == 4) {
-        const unsigned u = __ldg(reinterpret_cast<const unsigned*>(p));
-        memcpy(&r, &u, 4);
+        r.w[0] = u.x;
+        r.w[1] = u.y;
     } else {
-        const unsigned short u = __ldg(reinterpret_cast<const unsigned short*>(p));
-        memcpy(&r, &u, 2);
+        r.w[0] = __ldg(reinterpret_cast<const typename Pack<T, N>::Word*>(p));
     }
     return r;
-}
-// weights: N elements, in accesses of 16 bytes at most
-template <class T, int N>
-__device__ __forceinline__ void load_weights(const T* p, Pack<T, N>& r) {
-    constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
-#pragma unroll
-    for (int k = 0; k < N; k += M) {
-        const Pack<T, M> q = load_cached<T, M>(p + k);
-        memcpy(r.v + k, q.v, sizeof(q));
-    }
 }
 // outputs that this kernel does not read again
 template <class T, int N>
 __device__ __forceinline__ void store_stream(T* p, const Pack<T, N>& r) {
-    if constexpr (sizeof(r) == 16) {
-        uint4 u;
-        memcpy(&u, &r, 16);
-        asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
-    } else if constexpr (sizeof(r) == 8) {
-        uint2 u;
-        memcpy(&u, &r, 8);
-        asm volatile("st.global.cs.v2.u32 [%0], {%1,%2};" ::"l"(p), "r"(u.x), "r"(u.y) : "memory");
-    } else if constexpr (sizeof(r) == 4) {
-        unsigned u;
-        memcpy(&u, &r, 4);
-        asm volatile("st.global.cs.u32 [%0], %1;" ::"l"(p), "r"(u) : "memory");
-    } else {
-        unsigned short u;
-        memcpy(&u, &r, 2);
-        asm volatile("st.global.cs.u16 [%0], %1;" ::"l"(p), "h"(u) : "memory");
-    }
+    if constexpr (r.BYTES == 16)
+        asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]) : "memory");
+    else if constexpr (r.BYTES == 8)
+        asm volatile("st.global.cs.v2.u32 [%0], {%1,%2};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]) : "memory");
+    else if constexpr (r.BYTES == 4)
+        asm volatile("st.global.cs.u32 [%0], %1;" ::"l"(p), "r"(r.w[0]) : "memory");
+    else
+        asm volatile("st.global.cs.u16 [%0], %1;" ::"l"(p), "h"(r.w[0]) : "memory");
 }
 
-// two neighbouring elements, one 32-bit word where they are 16-bit
-template <class T>
-__device__ __forceinline__ float2 unpack2(const Pack<T, 2>& p) {
-    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-        unsigned u;
-        memcpy(&u, &p, 4);
-        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-    } else if constexpr (std::is_same_v<T, __half>) {
-        __half2 h;
-        memcpy(&h, &p, 4);
-        return __half22float2(h);
-    } else {
-        return make_float2(p.v[0], p.v[1]);
-    }
-}
-// the k-th pair of N elements
+// the k-th pair of N elements; an odd element is a pair with a second value of zero
 template <class T, int N>
 __device__ __forceinline__ float2 pair_of(const Pack<T, N>& p, int k) {
-    Pack<T, 2> q;
-    q.v[0] = p.v[2 * k];
-    q.v[1] = p.v[2 * k + 1];
-    return unpack2(q);
+    if constexpr (N == 1) {
+        T v;
+        memcpy(&v, p.w, sizeof(T));
+        return make_float2(to_f32(v), 0.f);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        return make_float2(__uint_as_float(p.w[k] << 16), __uint_as_float(p.w[k] & 0xffff0000u));
+    } else if constexpr (std::is_same_v<T, __half>) {
+        __half2 h;
+        memcpy(&h, &p.w[k], 4);
+        return __half22float2(h);
+    } else {
+        return make_float2(__uint_as_float(p.w[2 * k]), __uint_as_float(p.w[2 * k + 1]));
+    }
 }
-// N floats rounded to T
+// pairs of floats rounded to N elements of type T (N = 1: the pair's first value)
 template <class T, int N>
-__device__ __forceinline__ Pack<T, N> pack_f32(const float (&v)[N]) {
+__device__ __forceinline__ Pack<T, N> pack_pairs(const float2 (&v)[(N + 1) / 2]) {
     Pack<T, N> r;
-    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
-#pragma unroll
-        for (int k = 0; k < N; k += 2) {
-            if constexpr (std::is_same_v<T, __half>) {
-                const __half2 h = __floats2half2_rn(v[k], v[k + 1]);
-                r.v[k] = h.x;
-                r.v[k + 1] = h.y;
-            } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[k], v[k + 1]);
-                r.v[k] = h.x;
-                r.v[k + 1] = h.y;
-            }
-        }
+    if constexpr (N == 1) {
+        const T t = from_f32<T>(v[0].x);
+        memcpy(r.w, &t, sizeof(T));
     } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) r.v[k] = from_f32<T>(v[k]);
+        for (int k = 0; k < N / 2; ++k) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 h = __floats2half2_rn(v[k].x, v[k].y);
+                memcpy(&r.w[k], &h, 4);
+            } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[k].x, v[k].y);
+                memcpy(&r.w[k], &h, 4);
+            } else {
+                r.w[2 * k] = __float_as_uint(v[k].x);
+                r.w[2 * k + 1] = __float_as_uint(v[k].y);
+            }
+        }
     }
     return r;
 }

@@ -41,12 +41,13 @@ __global__ void __launch_bounds__(256) emb_fwd(const EmbFwdArgs a) {
         const long long v = static_cast<const I*>(a.ids)[i];
         Pack<T, EV> r;
         if (v >= 0 && v < a.rows) {
-            r = load_cached<T, EV>(table + v * a.D + p * EV);
+            const Pack<T, EV> q = load_cached<T, EV>(table + v * a.D + p * EV);
+            float2 f[(EV + 1) / 2];
 #pragma unroll
-            for (int k = 0; k < EV; ++k) r.v[k] = from_f32<T>(to_f32(r.v[k]) * a.scale);
+            for (int k = 0; k < (EV + 1) / 2; ++k) f[k] = mul2(pair_of(q, k), make_float2(a.scale, a.scale));
+            r = pack_pairs<T, EV>(f);
         } else {
-#pragma unroll
-            for (int k = 0; k < EV; ++k) r.v[k] = from_f32<T>(0.f);
+            r = {};
         }
         store_stream<T, EV>(out + i * a.D + p * EV, r);
     }
@@ -175,11 +176,11 @@ struct EmbSumArgs {
 };
 
 template <class T, int EV>
-__device__ __forceinline__ void write_row(const EmbSumArgs& a, unsigned v, int p, const float (&acc)[EV]) {
-    Pack<T, EV> r;
+__device__ __forceinline__ void write_row(const EmbSumArgs& a, unsigned v, int p, const float2 (&acc)[(EV + 1) / 2]) {
+    float2 r[(EV + 1) / 2];
 #pragma unroll
-    for (int k = 0; k < EV; ++k) r.v[k] = from_f32<T>(acc[k] * a.scale);
-    store_stream<T, EV>(static_cast<T*>(a.grad) + (long long)v * a.D + p * EV, r);
+    for (int k = 0; k < (EV + 1) / 2; ++k) r[k] = mul2(acc[k], make_float2(a.scale, a.scale));
+    store_stream<T, EV>(static_cast<T*>(a.grad) + (long long)v * a.D + p * EV, pack_pairs<T, EV>(r));
 }
 
 template <class T, int EV>
@@ -190,37 +191,35 @@ __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
         unsigned cur = a.key[s];
         if (cur >= a.rows) continue;
         bool begun = s > 0 && a.key[s - 1] == cur;          // the run began in an earlier chunk
-        float acc[EV];
+        float2 acc[(EV + 1) / 2];
+        auto clear = [&] {
 #pragma unroll
-        for (int k = 0; k < EV; ++k) acc[k] = 0.f;
+            for (int k = 0; k < (EV + 1) / 2; ++k) acc[k] = make_float2(0.f, 0.f);
+        };
+        auto keep = [&](float* to) {
+#pragma unroll
+            for (int k = 0; k < EV; ++k) to[k] = k & 1 ? acc[k / 2].y : acc[k / 2].x;
+        };
+        clear();
         float* part = a.part + 2LL * c * a.D + p * EV;
         for (int i = s; i < e; ++i) {
             const unsigned v = a.key[i];
             if (v != cur) {
-                if (begun) {
-#pragma unroll
-                    for (int k = 0; k < EV; ++k) part[k] = acc[k];
-                } else {
-                    write_row<T, EV>(a, cur, p, acc);
-                }
+                if (begun) keep(part);
+                else write_row<T, EV>(a, cur, p, acc);
                 cur = v;
                 begun = false;
                 if (v >= a.rows) break;
-#pragma unroll
-                for (int k = 0; k < EV; ++k) acc[k] = 0.f;
+                clear();
             }
             const Pack<T, EV> g = load_stream<T, EV>(static_cast<const T*>(a.dy) + (long long)a.pos[i] * a.D + p * EV);
 #pragma unroll
-            for (int k = 0; k < EV; ++k) acc[k] += to_f32(g.v[k]);
+            for (int k = 0; k < (EV + 1) / 2; ++k) acc[k] = add2(acc[k], pair_of(g, k));
         }
         if (cur >= a.rows) continue;
-        if (begun || (e < a.n && a.key[e] == cur)) {
-            if (!begun) part += a.D;
-#pragma unroll
-            for (int k = 0; k < EV; ++k) part[k] = acc[k];
-        } else {
-            write_row<T, EV>(a, cur, p, acc);
-        }
+        if (begun) keep(part);
+        else if (e < a.n && a.key[e] == cur) keep(part + a.D);
+        else write_row<T, EV>(a, cur, p, acc);
     }
 }
 
@@ -234,8 +233,8 @@ __global__ void __launch_bounds__(256) emb_join(const EmbSumArgs a) {
         const unsigned v = a.key[e];
         if (v >= a.rows || a.key[e - 1] != v) continue;                          // nothing crosses this chunk's end
         if (s > 0 && a.key[s] == v && a.key[s - 1] == v) continue;               // the run began earlier
-        float acc[1] = {a.part[(2LL * c + 1) * a.D + p]};
-        for (int k = c + 1; k < a.chunks && a.key[k * kChunk] == v; ++k) acc[0] += a.part[2LL * k * a.D + p];
+        float2 acc[1] = {make_float2(a.part[(2LL * c + 1) * a.D + p], 0.f)};
+        for (int k = c + 1; k < a.chunks && a.key[k * kChunk] == v; ++k) acc[0].x += a.part[2LL * k * a.D + p];
         write_row<T, 1>(a, v, p, acc);
     }
 }

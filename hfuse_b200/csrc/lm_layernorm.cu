@@ -2,6 +2,16 @@
 //
 //   forward   mu = sum x / D,  var = sum (x - mu)^2 / D,  r = 1 / sqrt(var + eps),  y = (x - mu) r w + b
 //   backward  xh = (x - mu) r,  g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
+//
+// Memory-bound: a row is read once, its mean and the sum of squares around it are formed on chip, and the result is written.
+// Three layouts, by the length of a row:
+//   short rows   2^k <= 32 lanes share a row and a block has many; no barrier at all, the next row is on its way into
+//                registers while one is reduced;
+//   rows         one-dimensional bulk (TMA) copies bring whole rows into shared memory ahead of their use, so
+//                that the bytes in flight cost neither registers nor threads; forward, one warp (or a few that share a named
+//                barrier) takes a row; backward, a block takes a few rows at a time and each thread keeps its columns, for
+//                which it adds up dw and db in registers over all of the block's rows;
+//   long rows    a block per row that reads it again from L2 for each step.
 #include <type_traits>
 
 #include "launch.cuh"
@@ -17,8 +27,10 @@ struct LnFwdArgs {
     float *mean, *invstd;
     long long rows, ldx;
     int D;
-    int lanes;               // threads that share a row
     float inv_d, eps;
+    int lanes;               // short rows: threads that share a row
+    int team, stages;        // rows: warps that share a row, buffers of each team
+    int buf, wbytes;         // bytes of a row buffer and of the weights in shared memory
 };
 
 struct LnBwdArgs {
@@ -27,15 +39,13 @@ struct LnBwdArgs {
     void *dx, *dw, *db;
     float* part;             // [slices][2][D]
     long long rows, ldx, lddy, slice_rows;
-    int D, slices, lanes;
+    int D, slices;
     float inv_d;
+    int lanes, stages, buf;
 };
 
-// A row lives in the registers of the threads that share it, NV accesses of EV elements each: it is read once, the mean
-// and the sum of squares around it are formed there, and y is written.  MANY: 2^k <= 32 lanes share a row and a
-// block has many, without any barrier; otherwise the whole block shares one, its warps' moments meet in shared memory behind one
-// barrier.  Each thread keeps its columns from row to row, so their weights stay in registers too (KEEP), and
-// the next row is loaded (AHEAD) before this one is reduced.
+// ---- short rows: NV accesses of EV elements in the registers of each of the 2^k <= 32 lanes that share a row ---------
+// Each thread keeps its columns from row to row, so their weights stay in registers too.
 template <int NV, int EV, class T>
 struct Row {
     Pack<T, EV> v[NV];
@@ -46,153 +56,115 @@ __device__ __forceinline__ void load_row(Row<NV, EV, T>& r, const T* p, int at, 
     for (int k = 0; k < NV; ++k)
         if (at + k * lanes < packs) r.v[k] = load_stream<T, EV>(p + (at + k * lanes) * EV);
 }
-// f(pair index, value) over a pack; an odd element is a pair with a second value of zero
-template <class T, int EV>
-__device__ __forceinline__ float2 elements(const Pack<T, EV>& p, int k) {
-    if constexpr (EV == 1) return make_float2(to_f32(p.v[0]), 0.f);
-    else return pair_of(p, k);
-}
 template <int EV>
 constexpr int kPairs = (EV + 1) / 2;
 
-template <bool MANY>
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-    if constexpr (MANY) {
-        for (int o = lanes >> 1; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
-    } else {
-        return warp_sum(v);
-    }
+// sum over the first n lanes, the others being zero; the same in all lanes up to the next power of two
+__device__ __forceinline__ float few_sum(float v, int n) {
+    if (n > 16) v += __shfl_xor_sync(0xffffffffu, v, 16);
+    if (n > 8) v += __shfl_xor_sync(0xffffffffu, v, 8);
+    if (n > 4) v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 2);
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return __shfl_sync(0xffffffffu, v, 0);
 }
 
-template <class T, class W, int EV, int NV, bool MANY, int MAXT>
-__global__ void __launch_bounds__(MAXT) ln_fwd(const LnFwdArgs a) {
-    constexpr bool KEEP = NV * EV * (int)sizeof(W) <= 64 && MAXT <= 512, AHEAD = MAXT <= 512;
-    __shared__ float2 moments[2][32];
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = lanes >> 1; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// 1 / sqrt(var + eps): rsqrt is off by 2 units in the last place at most
+__device__ __forceinline__ float inv_std(float q, float inv_d, float eps) {
+    return rsqrtf(fmaf(q, inv_d, eps));
+}
+
+template <class W, int EV>
+__device__ __forceinline__ void weights_of(const W* from, int p, float2 (&to)[kPairs<EV>], float none) {
+    Pack<W, EV> q = {};
+    if (from) q = load_cached<W, EV>(from + p * EV);
+#pragma unroll
+    for (int j = 0; j < kPairs<EV>; ++j) to[j] = from ? pair_of<W, EV>(q, j) : make_float2(none, none);
+}
+
+template <class T, class W, int EV, int NV>
+__global__ void __launch_bounds__(256) ln_fwd_short(const LnFwdArgs a) {
     const T* x = static_cast<const T*>(a.x);
-    const W* w = static_cast<const W*>(a.w);
-    const W* b = static_cast<const W*>(a.b);
-    const int lanes = MANY ? a.lanes : blockDim.x, packs = a.D / EV;
-    const int at = MANY ? threadIdx.x & (lanes - 1) : threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = MANY ? blockDim.x / lanes : 1;
+    const int lanes = a.lanes, packs = a.D / EV, per = 256 / lanes, at = threadIdx.x & (lanes - 1);
     const long long step = (long long)gridDim.x * per;
-    long long r = (long long)blockIdx.x * per + (MANY ? threadIdx.x / lanes : 0);
-    long long head = MANY ? (long long)blockIdx.x * per + warp * (32 / lanes) : r;      // the warp's first row
-    // elements that warp number `lane` of the block holds
-    float count = 0.f, inv_count = 0.f;
-    if constexpr (!MANY) {
-        int n = 0;
+    long long r = (long long)blockIdx.x * per + threadIdx.x / lanes;
+    long long head = (long long)blockIdx.x * per + (threadIdx.x >> 5) * (32 / lanes);      // the warp's first row
+    float2 kw[NV][kPairs<EV>], kb[NV][kPairs<EV>];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) n += min(max(packs - k * lanes - 32 * lane, 0), min(32, max(lanes - 32 * lane, 0)));
-        count = (float)(n * EV);
-        inv_count = n ? 1.f / count : 0.f;
-    }
-    const float mine = MANY ? 0.f : __shfl_sync(0xffffffffu, inv_count, warp);
-    Pack<W, EV> kw[NV], kb[NV];
-    if constexpr (KEEP) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (at + k * lanes < packs) {
-                if (w) load_weights<W, EV>(w + (at + k * lanes) * EV, kw[k]);
-                if (b) load_weights<W, EV>(b + (at + k * lanes) * EV, kb[k]);
-            }
-    }
+    for (int k = 0; k < NV; ++k)
+        if (at + k * lanes < packs) {
+            weights_of<W, EV>(static_cast<const W*>(a.w), at + k * lanes, kw[k], 1.f);
+            weights_of<W, EV>(static_cast<const W*>(a.b), at + k * lanes, kb[k], 0.f);
+        }
     Row<NV, EV, T> row, ahead;
     if (r < a.rows) load_row<T, EV, NV>(row, x + r * a.ldx, at, lanes, packs);
-    for (int turn = 0; head < a.rows; head += step, r += step, turn ^= 1) {
-        const bool in = !MANY || r < a.rows;
-        if constexpr (AHEAD) {
-            if (r + step < a.rows) load_row<T, EV, NV>(ahead, x + (r + step) * a.ldx, at, lanes, packs);
-        } else if (r >= step && in) {
-            load_row<T, EV, NV>(row, x + r * a.ldx, at, lanes, packs);
-        }
-        float2 s2 = make_float2(0.f, 0.f);
+    for (; head < a.rows; head += step, r += step) {
+        const bool in = r < a.rows;
+        if (r + step < a.rows) load_row<T, EV, NV>(ahead, x + (r + step) * a.ldx, at, lanes, packs);
+        float2 f[NV][kPairs<EV>], s2 = make_float2(0.f, 0.f), q2 = s2;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
             if (in && at + k * lanes < packs) {
 #pragma unroll
-                for (int q = 0; q < kPairs<EV>; ++q) s2 = add2(s2, elements<T, EV>(row.v[k], q));
-            }
-        float s = lanes_sum<MANY>(s2.x + s2.y, lanes);
-        const float mid = MANY ? s * a.inv_d : s * mine;              // of the row, or of the warp's part of it
-        float2 q2 = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (in && at + k * lanes < packs) {
-#pragma unroll
-                for (int q = 0; q < kPairs<EV>; ++q) {
-                    float2 d = add2(elements<T, EV>(row.v[k], q), make_float2(-mid, -mid));
-                    if (EV == 1) d.y = 0.f;
-                    q2 = fma2(d, d, q2);
+                for (int j = 0; j < kPairs<EV>; ++j) {
+                    f[k][j] = pair_of<T, EV>(row.v[k], j);
+                    s2 = add2(s2, f[k][j]);
                 }
             }
-        float q = lanes_sum<MANY>(q2.x + q2.y, lanes), mu = mid;
-        if constexpr (!MANY) {
-            if (lane == 0) moments[turn][warp] = make_float2(s, q);
-            __syncthreads();
-            // lane l takes warp l's part: sums of squares around the parts' means, moved to the row's mean
-            const float2 m = lane < (lanes >> 5) ? moments[turn][lane] : make_float2(0.f, 0.f);
-            mu = warp_sum(m.x) * a.inv_d;
-            const float d = m.x * inv_count - mu;
-            q = warp_sum(fmaf(count * d, d, m.y));
-        }
-        const float is = 1.f / sqrtf(fmaf(q, a.inv_d, a.eps));
+        const float mu = lanes_sum(s2.x + s2.y, lanes) * a.inv_d;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (in && at + k * lanes < packs) {
+#pragma unroll
+                for (int j = 0; j < kPairs<EV>; ++j) {
+                    f[k][j] = add2(f[k][j], make_float2(-mu, -mu));
+                    if (EV == 1) f[k][j].y = 0.f;
+                    q2 = fma2(f[k][j], f[k][j], q2);
+                }
+            }
+        const float is = inv_std(lanes_sum(q2.x + q2.y, lanes), a.inv_d, a.eps);
         if (in) {
             T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int p = at + k * lanes;
-                if (p >= packs) continue;
-                if constexpr (!KEEP) {
-                    if (w) load_weights<W, EV>(w + p * EV, kw[k]);
-                    if (b) load_weights<W, EV>(b + p * EV, kb[k]);
-                }
-                float o[2 * kPairs<EV>];
+                if (at + k * lanes >= packs) continue;
+                float2 o[kPairs<EV>];
 #pragma unroll
-                for (int j = 0; j < kPairs<EV>; ++j) {
-                    float2 d = mul2(add2(elements<T, EV>(row.v[k], j), make_float2(-mu, -mu)), make_float2(is, is));
-                    if (w) d = mul2(d, elements<W, EV>(kw[k], j));
-                    if (b) d = add2(d, elements<W, EV>(kb[k], j));
-                    o[2 * j] = d.x;
-                    o[2 * j + 1] = d.y;
-                }
-                if constexpr (EV == 1) store_stream<T, 1>(y + p, Pack<T, 1>{{from_f32<T>(o[0])}});
-                else store_stream<T, EV>(y + p * EV, pack_f32<T, EV>(o));
+                for (int j = 0; j < kPairs<EV>; ++j) o[j] = fma2(f[k][j], mul2(kw[k][j], make_float2(is, is)), kb[k][j]);
+                store_stream<T, EV>(y + (at + k * lanes) * EV, pack_pairs<T, EV>(o));
             }
             if (at == 0) {
                 a.mean[r] = mu;
                 a.invstd[r] = is;
             }
         }
-        if constexpr (AHEAD) row = ahead;
+        row = ahead;
     }
 }
 
 // The same layout backwards: x and dy of a row are in registers, the two row sums are reduced together, and each
-// thread adds up dy xh and dy of its columns over all rows of its block.  The blocks' sums go to the workspace, [block][2][D].
-template <class T, class W, int EV, int NV, bool MANY, int MAXT>
-__global__ void __launch_bounds__(MAXT) ln_bwd(const LnBwdArgs a) {
-    constexpr bool AHEAD = MAXT <= 512;
-    extern __shared__ float shared_sums[];                  // MANY: 2 EV NV floats of every thread
-    __shared__ float2 sums[2][32];
+// thread adds up dy xh and dy of its columns over all its rows.  The blocks' sums go to the workspace, [block][2][D].
+template <class T, class W, int EV, int NV>
+__global__ void __launch_bounds__(256) ln_bwd_short(const LnBwdArgs a) {
+    extern __shared__ float shared_sums[];                  // 2 EV NV floats of every thread, [value][thread]
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.dy);
-    const W* w = static_cast<const W*>(a.w);
-    const int lanes = MANY ? a.lanes : blockDim.x, packs = a.D / EV;
-    const int at = MANY ? threadIdx.x & (lanes - 1) : threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = MANY ? blockDim.x / lanes : 1;
+    const int lanes = a.lanes, packs = a.D / EV, per = 256 / lanes, at = threadIdx.x & (lanes - 1);
     const long long step = (long long)gridDim.x * per;
-    long long r = (long long)blockIdx.x * per + (MANY ? threadIdx.x / lanes : 0);
-    long long head = MANY ? (long long)blockIdx.x * per + warp * (32 / lanes) : r;
-    Pack<W, EV> kw[NV];
+    long long r = (long long)blockIdx.x * per + threadIdx.x / lanes;
+    long long head = (long long)blockIdx.x * per + (threadIdx.x >> 5) * (32 / lanes);
+    float2 kw[NV][kPairs<EV>], dw[NV][kPairs<EV>], db[NV][kPairs<EV>];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if (w && at + k * lanes < packs) load_weights<W, EV>(w + (at + k * lanes) * EV, kw[k]);
-    float2 dw[NV][kPairs<EV>], db[NV][kPairs<EV>];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+        if (at + k * lanes < packs) weights_of<W, EV>(static_cast<const W*>(a.w), at + k * lanes, kw[k], 1.f);
 #pragma unroll
         for (int j = 0; j < kPairs<EV>; ++j) dw[k][j] = db[k][j] = make_float2(0.f, 0.f);
+    }
     Row<NV, EV, T> rx, rd, nx, nd;
     float mu = 0.f, is = 0.f, nmu = 0.f, nis = 0.f;
     if (r < a.rows) {
@@ -201,103 +173,445 @@ __global__ void __launch_bounds__(MAXT) ln_bwd(const LnBwdArgs a) {
         mu = __ldg(a.mean + r);
         is = __ldg(a.invstd + r);
     }
-    for (int turn = 0; head < a.rows; head += step, r += step, turn ^= 1) {
-        const bool in = !MANY || r < a.rows;
-        if (!AHEAD && r >= step && in) {
-            load_row<T, EV, NV>(rx, x + r * a.ldx, at, lanes, packs);
-            load_row<T, EV, NV>(rd, dy + r * a.lddy, at, lanes, packs);
-            mu = __ldg(a.mean + r);
-            is = __ldg(a.invstd + r);
-        }
-        if (AHEAD && r + step < a.rows) {
+    for (; head < a.rows; head += step, r += step) {
+        const bool in = r < a.rows;
+        if (r + step < a.rows) {
             load_row<T, EV, NV>(nx, x + (r + step) * a.ldx, at, lanes, packs);
             load_row<T, EV, NV>(nd, dy + (r + step) * a.lddy, at, lanes, packs);
             nmu = __ldg(a.mean + r + step);
             nis = __ldg(a.invstd + r + step);
         }
         const float2 mu2 = make_float2(-mu, -mu), is2 = make_float2(is, is);
-        float2 s = make_float2(0.f, 0.f), d = make_float2(0.f, 0.f);
+        float2 s = make_float2(0.f, 0.f), d = s, xh[NV][kPairs<EV>], g[NV][kPairs<EV>];
 #pragma unroll
         for (int k = 0; k < NV; ++k)
             if (in && at + k * lanes < packs) {
 #pragma unroll
                 for (int j = 0; j < kPairs<EV>; ++j) {
-                    const float2 xh = mul2(add2(elements<T, EV>(rx.v[k], j), mu2), is2), g0 = elements<T, EV>(rd.v[k], j);
-                    const float2 g = w ? mul2(g0, elements<W, EV>(kw[k], j)) : g0;
-                    dw[k][j] = fma2(g0, xh, dw[k][j]);
+                    const float2 g0 = pair_of<T, EV>(rd.v[k], j);
+                    xh[k][j] = mul2(add2(pair_of<T, EV>(rx.v[k], j), mu2), is2);
+                    g[k][j] = mul2(g0, kw[k][j]);
+                    dw[k][j] = fma2(g0, xh[k][j], dw[k][j]);
                     db[k][j] = add2(db[k][j], g0);
-                    s = add2(s, g);
-                    d = fma2(g, xh, d);
+                    s = add2(s, g[k][j]);
+                    d = fma2(g[k][j], xh[k][j], d);
                 }
             }
-        float2 both = make_float2(lanes_sum<MANY>(s.x + s.y, lanes), lanes_sum<MANY>(d.x + d.y, lanes));
-        if constexpr (!MANY) {
-            if (lane == 0) sums[turn][warp] = both;
-            __syncthreads();
-            both = make_float2(0.f, 0.f);
-            for (int k = 0; k < (lanes >> 5); ++k) both = add2(both, sums[turn][k]);
-        }
+        const float ms = -lanes_sum(s.x + s.y, lanes) * a.inv_d, md = -lanes_sum(d.x + d.y, lanes) * a.inv_d;
         if (in && a.dx) {
-            const float2 ms = make_float2(-both.x * a.inv_d, -both.x * a.inv_d), md = make_float2(-both.y * a.inv_d, -both.y * a.inv_d);
             T* dx = static_cast<T*>(a.dx) + r * a.D;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int p = at + k * lanes;
-                if (p >= packs) continue;
-                float o[2 * kPairs<EV>];
+                if (at + k * lanes >= packs) continue;
+                float2 o[kPairs<EV>];
 #pragma unroll
-                for (int j = 0; j < kPairs<EV>; ++j) {
-                    const float2 xh = mul2(add2(elements<T, EV>(rx.v[k], j), mu2), is2), g0 = elements<T, EV>(rd.v[k], j);
-                    const float2 g = w ? mul2(g0, elements<W, EV>(kw[k], j)) : g0;
-                    const float2 v = mul2(is2, fma2(xh, md, add2(g, ms)));
-                    o[2 * j] = v.x;
-                    o[2 * j + 1] = v.y;
-                }
-                if constexpr (EV == 1) store_stream<T, 1>(dx + p, Pack<T, 1>{{from_f32<T>(o[0])}});
-                else store_stream<T, EV>(dx + p * EV, pack_f32<T, EV>(o));
+                for (int j = 0; j < kPairs<EV>; ++j)
+                    o[j] = mul2(is2, fma2(xh[k][j], make_float2(md, md), add2(g[k][j], make_float2(ms, ms))));
+                store_stream<T, EV>(dx + (at + k * lanes) * EV, pack_pairs<T, EV>(o));
             }
         }
-        if constexpr (AHEAD) {
-            rx = nx;
-            rd = nd;
-            mu = nmu;
-            is = nis;
-        }
+        rx = nx;
+        rd = nd;
+        mu = nmu;
+        is = nis;
     }
     if (!a.part) return;
     float* part = a.part + 2LL * blockIdx.x * a.D;
-    if constexpr (MANY) {
-        // the block's groups of lanes, added in their order; [value][thread]
+    // the block's groups of lanes, added in their order
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int j = 0; j < EV; ++j) {
-                shared_sums[(2 * (k * EV + j)) * 256 + threadIdx.x] = j & 1 ? dw[k][j / 2].y : dw[k][j / 2].x;
-                shared_sums[(2 * (k * EV + j) + 1) * 256 + threadIdx.x] = j & 1 ? db[k][j / 2].y : db[k][j / 2].x;
-            }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2 * NV * EV * lanes; i += 256) {
-            const int l = i & (lanes - 1), v = i / lanes, c = ((v >> 1) / EV * lanes + l) * EV + (v >> 1) % EV;
-            if (c >= a.D) continue;
-            float t = 0.f;
-            for (int g = 0; g < per; ++g) t += shared_sums[v * 256 + g * lanes + l];
-            part[(v & 1) * (long long)a.D + c] = t;
+        for (int j = 0; j < EV; ++j) {
+            shared_sums[(2 * (k * EV + j)) * 256 + threadIdx.x] = j & 1 ? dw[k][j / 2].y : dw[k][j / 2].x;
+            shared_sums[(2 * (k * EV + j) + 1) * 256 + threadIdx.x] = j & 1 ? db[k][j / 2].y : db[k][j / 2].x;
         }
-    } else {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (at + k * lanes < packs) {
-#pragma unroll
-                for (int j = 0; j < EV; ++j) {
-                    const int c = (at + k * lanes) * EV + j;
-                    part[c] = j & 1 ? dw[k][j / 2].y : dw[k][j / 2].x;
-                    part[a.D + c] = j & 1 ? db[k][j / 2].y : db[k][j / 2].x;
-                }
-            }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * NV * EV * lanes; i += 256) {
+        const int l = i & (lanes - 1), v = i / lanes, c = ((v >> 1) / EV * lanes + l) * EV + (v >> 1) % EV;
+        if (c >= a.D) continue;
+        float t = 0.f;
+        for (int g = 0; g < per; ++g) t += shared_sums[v * 256 + g * lanes + l];
+        part[(v & 1) * (long long)a.D + c] = t;
     }
 }
 
-// ---- any width: one block per row, the row read again from L2 for each step ---------------------
+// ---- rows in shared memory ---------------------------------------------------------------------------------
+// A bulk copy begins on a 16-byte boundary and has a multiple of 16 bytes, so a row that does not is copied with what
+// shares its first and last 16 bytes, as far as that belongs to the tensor; the first and the last row may lack some
+// elements at the tensor's very ends, which are fetched one by one (patch).  Element 0 is `shift` bytes into the buffer.
+struct Span {
+    const unsigned char *lo, *hi;      // what is copied
+    int shift;
+};
+template <class T>
+__device__ __forceinline__ Span row_span(const T* base, long long ld, long long rows, int D, long long r) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(base), end = reinterpret_cast<uintptr_t>(base + (rows - 1) * ld + D);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(base + r * ld), q = p + (size_t)D * sizeof(T);
+    Span s;
+    s.shift = (int)(p & 15);
+    uintptr_t lo = p & ~(uintptr_t)15, hi = (q + 15) & ~(uintptr_t)15;
+    if (lo < begin) lo += 16;
+    if (hi > end) hi -= 16;
+    s.lo = reinterpret_cast<const unsigned char*>(lo);
+    s.hi = reinterpret_cast<const unsigned char*>(hi);
+    return s;
+}
+// announces and starts the copy of a row (one thread)
+template <class T>
+__device__ __forceinline__ void fetch_row(unsigned char* buf, unsigned long long* bar, const T* base, long long ld, long long rows, int D,
+                                          long long r) {
+    const Span s = row_span(base, ld, rows, D, r);
+    const long long bytes = s.hi - s.lo;
+    if (bytes > 0) {
+        mbar_expect_tx(bar, (uint32_t)bytes);
+        const uintptr_t row = reinterpret_cast<uintptr_t>(base + r * ld) & ~(uintptr_t)15;
+        bulk_load(buf + (reinterpret_cast<uintptr_t>(s.lo) - row), s.lo, (uint32_t)bytes, bar);
+    } else {
+        mbar_arrive(bar);
+    }
+}
+// whether patch_row has something to do; every thread of the team, then a barrier of the team
+template <class T>
+__device__ __forceinline__ bool row_lacks(const T* base, long long ld, long long rows, int D, long long r) {
+    if (r != 0 && r != rows - 1) return false;
+    const Span s = row_span(base, ld, rows, D, r);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(base + r * ld);
+    return reinterpret_cast<uintptr_t>(s.lo) > p || reinterpret_cast<uintptr_t>(s.hi) < p + (size_t)D * sizeof(T);
+}
+template <class T>
+__device__ __forceinline__ void patch_row(unsigned char* buf, const T* base, long long ld, long long rows, int D, long long r, int at,
+                                          int lanes) {
+    const Span s = row_span(base, ld, rows, D, r);
+    const T* p = base + r * ld;
+    T* to = reinterpret_cast<T*>(buf + s.shift);
+    for (int i = at; i < D; i += lanes) {
+        const unsigned char* q = reinterpret_cast<const unsigned char*>(p + i);
+        if (q < s.lo || q >= s.hi) to[i] = p[i];
+    }
+    fence_proxy_async_shared();        // a later copy may write there
+}
+constexpr unsigned long long kRowWaitNs = 2000000000ull;
+
+// the warps of a team meet at their own named barrier
+__device__ __forceinline__ void team_sync(int team, int warps) {
+    if (warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(warps * 32) : "memory");
+}
+
+// A row's elements in the registers of a team: accesses of EV elements, or (EV = 1) single elements in pairs of
+// accesses.  VALUES pairs; element(s) of pair i that are beyond the row have a place, but no value.
+template <class T, int EV, int NV>
+struct Team {
+    static constexpr int VALUES = NV * EV / 2;
+    Pack<T, EV> v[NV];
+    __device__ __forceinline__ void read(const unsigned char* row, int at, int lanes, int packs) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (at + k * lanes < packs) v[k] = *(reinterpret_cast<const Pack<T, EV>*>(row) + at + k * lanes);
+            else v[k] = {};
+        }
+    }
+    __device__ __forceinline__ float2 get(int i) const {
+        if constexpr (EV == 1) return make_float2(pair_of<T, 1>(v[2 * i], 0).x, pair_of<T, 1>(v[2 * i + 1], 0).x);
+        else return pair_of<T, EV>(v[i / (EV / 2)], i % (EV / 2));
+    }
+};
+// which of a pair's elements exist
+template <int EV>
+__device__ __forceinline__ void exists(int i, int at, int lanes, int packs, bool& x, bool& y) {
+    if constexpr (EV == 1) {
+        x = at + 2 * i * lanes < packs;
+        y = at + (2 * i + 1) * lanes < packs;
+    } else {
+        x = y = at + i / (EV / 2) * lanes < packs;
+    }
+}
+
+template <class T, class W, int EV, int NV>
+__global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int VALUES = NV * EV / 2;
+    const T* x = static_cast<const T*>(a.x);
+    const int M = a.team, lane = threadIdx.x & 31, warp = warp_index(), warps = blockDim.x >> 5, teams = warps / M;
+    const int team = warp / M, part = warp - team * M, lanes = 32 * M, at = part * 32 + lane, packs = a.D / EV;
+    W* sw = reinterpret_cast<W*>(smem);
+    W* sb = reinterpret_cast<W*>(smem + a.wbytes);
+    unsigned char* ring = smem + 2 * a.wbytes + (size_t)team * a.stages * a.buf;
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + 2 * a.wbytes + (size_t)teams * a.stages * a.buf) + team * a.stages;
+    float2* moments = reinterpret_cast<float2*>(smem + 2 * a.wbytes + (size_t)teams * a.stages * (a.buf + 8));    // [2][warps]
+    const long long step = (long long)gridDim.x * teams;
+    long long r = (long long)blockIdx.x * teams + team;
+    const bool lead = part == 0 && lane == 0;
+    if (lead) {
+        for (int s = 0; s < a.stages; ++s) mbar_init(bars + s, 1);
+        fence_mbar_init();
+        for (int s = 0; s < a.stages; ++s)
+            if (r + s * step < a.rows) fetch_row(ring + (size_t)s * a.buf, bars + s, x, a.ldx, a.rows, a.D, r + s * step);
+    }
+    for (int i = threadIdx.x; i < a.D; i += blockDim.x) {
+        sw[i] = a.w ? static_cast<const W*>(a.w)[i] : from_f32<W>(1.f);
+        sb[i] = a.b ? static_cast<const W*>(a.b)[i] : from_f32<W>(0.f);
+    }
+    // elements that the team's warp number `lane` holds
+    float count = 0.f, inv_count = 0.f;
+    if (M > 1 && lane < M) {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) n += min(max(packs - k * lanes - 32 * lane, 0), 32);
+        count = (float)(n * EV);
+        inv_count = n ? 1.f / count : 0.f;
+    }
+    const float mine = M > 1 ? __shfl_sync(0xffffffffu, inv_count, part) : a.inv_d;
+    __syncthreads();
+    int stage = 0, parity = 0;
+    for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
+        unsigned char* buf = ring + (size_t)stage * a.buf;
+        const bool there = mbar_wait(bars + stage, parity, kRowWaitNs);
+        int shift = 0;
+        if constexpr (EV == 1) {
+            shift = (int)(reinterpret_cast<uintptr_t>(x + r * a.ldx) & 15);
+            if (row_lacks(x, a.ldx, a.rows, a.D, r)) {
+                patch_row(buf, x, a.ldx, a.rows, a.D, r, at, lanes);
+                team_sync(team, M);
+            }
+        }
+        Team<T, EV, NV> row;
+        row.read(buf + shift, at, lanes, packs);
+        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) s2 = add2(s2, row.get(i));              // zeros beyond the row
+        const float s = warp_sum(s2.x + s2.y), mid = s * mine;                   // the mean of the warp's part
+        float2 q2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) {
+            float2 d = add2(row.get(i), make_float2(-mid, -mid));
+            bool ex, ey;
+            exists<EV>(i, at, lanes, packs, ex, ey);
+            if (!ex) d.x = 0.f;
+            if (!ey) d.y = 0.f;
+            q2 = fma2(d, d, q2);
+        }
+        float q = warp_sum(q2.x + q2.y), mu = mid;
+        if (M == 1) {
+            __syncwarp();
+        } else {
+            float2* mine2 = moments + turn * warps + team * M;
+            if (lane == 0) mine2[part] = make_float2(s, q);
+            team_sync(team, M);
+            // lane l takes warp l's part: sums of squares around the parts' means, moved to the row's mean
+            const float2 m = lane < M ? mine2[lane] : make_float2(0.f, 0.f);
+            mu = few_sum(m.x, M) * a.inv_d;
+            const float d = m.x * inv_count - mu;
+            q = few_sum(fmaf(count * d, d, m.y), M);
+        }
+        // the whole team has read the buffer
+        if (lead && r + a.stages * step < a.rows) fetch_row(buf, bars + stage, x, a.ldx, a.rows, a.D, r + a.stages * step);
+        if (++stage == a.stages) {
+            stage = 0;
+            parity ^= 1;
+        }
+        float is = inv_std(q, a.inv_d, a.eps);
+        if (!there) mu = is = __int_as_float(0x7fc00000);
+        T* y = static_cast<T*>(a.y) + r * a.D;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int p = at + k * lanes;
+            if (p >= packs) continue;
+            const Pack<W, EV> w = *(reinterpret_cast<const Pack<W, EV>*>(sw) + p), b = *(reinterpret_cast<const Pack<W, EV>*>(sb) + p);
+            float2 o[kPairs<EV>];
+#pragma unroll
+            for (int j = 0; j < kPairs<EV>; ++j)
+                o[j] = fma2(add2(pair_of<T, EV>(row.v[k], j), make_float2(-mu, -mu)), mul2(pair_of<W, EV>(w, j), make_float2(is, is)),
+                            pair_of<W, EV>(b, j));
+            store_stream<T, EV>(y + p * EV, pack_pairs<T, EV>(o));
+        }
+        if (lead) {
+            a.mean[r] = mu;
+            a.invstd[r] = is;
+        }
+    }
+}
+
+// The sums over a warp of 4 values of each lane, in 6 shuffles instead of 20: halves of the lanes take over halves of the
+// values.  Lane l gets value l / 8's sum (the same in its 8 lanes).
+__device__ __forceinline__ float warp_sum4(float a, float b, float c, float d, int lane) {
+    const bool up = lane & 16;
+    const float u = (up ? c : a) + __shfl_xor_sync(0xffffffffu, up ? a : c, 16);
+    const float v = (up ? d : b) + __shfl_xor_sync(0xffffffffu, up ? b : d, 16);
+    const bool odd = lane & 8;
+    float t = (odd ? v : u) + __shfl_xor_sync(0xffffffffu, odd ? u : v, 8);
+    t += __shfl_xor_sync(0xffffffffu, t, 4);
+    t += __shfl_xor_sync(0xffffffffu, t, 2);
+    t += __shfl_xor_sync(0xffffffffu, t, 1);
+    return t;
+}
+
+// A block takes two rows at a time: [stage][x, dy][row] buffers.
+template <class T, class W, int EV, int NV>
+__global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int VALUES = NV * EV / 2;
+    const T* x = static_cast<const T*>(a.x);
+    const T* dy = static_cast<const T*>(a.dy);
+    const W* w = static_cast<const W*>(a.w);
+    const int lanes = blockDim.x, at = threadIdx.x, lane = threadIdx.x & 31, warp = warp_index(), warps = lanes >> 5, packs = a.D / EV;
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)a.stages * 4 * a.buf);
+    float* sums = reinterpret_cast<float*>(bars + a.stages + (a.stages & 1));            // [2][warps][4]
+    float2 kw[VALUES], dw[VALUES], db[VALUES];
+    {
+        Team<W, EV, NV> t;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            t.v[k] = {};
+            if (w && at + k * lanes < packs) t.v[k] = load_cached<W, EV>(w + (at + k * lanes) * EV);
+        }
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) {
+            kw[i] = w ? t.get(i) : make_float2(1.f, 1.f);
+            dw[i] = db[i] = make_float2(0.f, 0.f);
+        }
+    }
+    // the block's k-th pair of rows; lanes 0 to 3 of the first warp fetch one row each
+    const long long step = 2LL * gridDim.x;
+    auto fetch = [&](long long r, int s) {
+        if (warp == 0 && lane < 4) {
+            const long long row = r + (lane & 1);
+            if (row >= a.rows) mbar_arrive(bars + s);
+            else if (lane < 2) fetch_row(smem + (size_t)(4 * s + lane) * a.buf, bars + s, x, a.ldx, a.rows, a.D, row);
+            else fetch_row(smem + (size_t)(4 * s + lane) * a.buf, bars + s, dy, a.lddy, a.rows, a.D, row);
+        }
+    };
+    // mean and invstd of a pair of rows in lanes 0 to 3
+    auto stats = [&](long long r) {
+        const long long row = r + (lane & 1);
+        return lane < 4 && row < a.rows ? __ldg((lane < 2 ? a.mean : a.invstd) + row) : 0.f;
+    };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; ++s) mbar_init(bars + s, 4);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    long long r = 2LL * blockIdx.x;
+    for (int s = 0; s < a.stages; ++s)
+        if (r + s * step < a.rows) fetch(r + s * step, s);
+    float now = stats(r), next = 0.f;
+    int stage = 0, parity = 0;
+    for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
+        next = stats(r + step);
+        unsigned char* buf = smem + (size_t)4 * stage * a.buf;
+        const bool there = mbar_wait(bars + stage, parity, kRowWaitNs);
+        const unsigned char *px[2], *pd[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            int sx = 0, sd = 0;
+            if (EV == 1 && r + g < a.rows) {
+                sx = (int)(reinterpret_cast<uintptr_t>(x + (r + g) * a.ldx) & 15);
+                sd = (int)(reinterpret_cast<uintptr_t>(dy + (r + g) * a.lddy) & 15);
+            }
+            px[g] = buf + (size_t)g * a.buf + sx;
+            pd[g] = buf + (size_t)(2 + g) * a.buf + sd;
+        }
+        if constexpr (EV == 1) {
+            bool lacks = false;
+            for (int g = 0; g < 2; ++g) {
+                if (r + g >= a.rows) continue;
+                if (row_lacks(x, a.ldx, a.rows, a.D, r + g)) {
+                    patch_row(buf + (size_t)g * a.buf, x, a.ldx, a.rows, a.D, r + g, at, lanes);
+                    lacks = true;
+                }
+                if (row_lacks(dy, a.lddy, a.rows, a.D, r + g)) {
+                    patch_row(buf + (size_t)(2 + g) * a.buf, dy, a.lddy, a.rows, a.D, r + g, at, lanes);
+                    lacks = true;
+                }
+            }
+            if (lacks) __syncthreads();
+        }
+        float2 s[2], d[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            s[g] = d[g] = make_float2(0.f, 0.f);
+            if (r + g >= a.rows) continue;
+            const float mu = __shfl_sync(0xffffffffu, now, g), is = __shfl_sync(0xffffffffu, now, 2 + g);
+            Team<T, EV, NV> vx, vd;                        // dy of zero beyond the row: nothing is added
+            vx.read(px[g], at, lanes, packs);
+            vd.read(pd[g], at, lanes, packs);
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) {
+                const float2 xh = mul2(add2(vx.get(i), make_float2(-mu, -mu)), make_float2(is, is)), g0 = vd.get(i), gw = mul2(g0, kw[i]);
+                dw[i] = fma2(g0, xh, dw[i]);
+                db[i] = add2(db[i], g0);
+                s[g] = add2(s[g], gw);
+                d[g] = fma2(gw, xh, d[g]);
+            }
+        }
+        const float t4 = warp_sum4(s[0].x + s[0].y, d[0].x + d[0].y, s[1].x + s[1].y, d[1].x + d[1].y, lane);
+        float* set = sums + turn * warps * 4;
+        if ((lane & 7) == 0) set[warp * 4 + (lane >> 3)] = t4;
+        __syncthreads();
+        // lane l adds value l % 4 of warps l / 4, l / 4 + 8, ..
+        float total = 0.f;
+        for (int k = lane >> 2; k < warps; k += 8) total += set[k * 4 + (lane & 3)];
+        total += __shfl_xor_sync(0xffffffffu, total, 4);
+        total += __shfl_xor_sync(0xffffffffu, total, 8);
+        total += __shfl_xor_sync(0xffffffffu, total, 16);
+        total *= -a.inv_d;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            if (r + g >= a.rows) continue;
+            const float mu = __shfl_sync(0xffffffffu, now, g), is = __shfl_sync(0xffffffffu, now, 2 + g);
+            float ms = __shfl_sync(0xffffffffu, total, 2 * g), md = __shfl_sync(0xffffffffu, total, 2 * g + 1);
+            if (!a.dx) continue;
+            if (!there) ms = __int_as_float(0x7fc00000);
+            Team<T, EV, NV> vx, vd;
+            vx.read(px[g], at, lanes, packs);
+            vd.read(pd[g], at, lanes, packs);
+            T* dx = static_cast<T*>(a.dx) + (r + g) * a.D;
+            float2 o[VALUES];
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) {
+                const float2 xh = mul2(add2(vx.get(i), make_float2(-mu, -mu)), make_float2(is, is));
+                o[i] = mul2(make_float2(is, is), fma2(xh, make_float2(md, md), fma2(vd.get(i), kw[i], make_float2(ms, ms))));
+            }
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (at + k * lanes >= packs) continue;
+                if constexpr (EV == 1) {
+                    dx[at + k * lanes] = from_f32<T>(k & 1 ? o[k / 2].y : o[k / 2].x);
+                } else {
+                    float2 part[EV / 2];
+#pragma unroll
+                    for (int j = 0; j < EV / 2; ++j) part[j] = o[k * (EV / 2) + j];
+                    store_stream<T, EV>(dx + (at + k * lanes) * EV, pack_pairs<T, EV>(part));
+                }
+            }
+        }
+        if (!there) {
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) dw[i] = db[i] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+        }
+        __syncthreads();                                   // every thread has read the stage
+        if (r + a.stages * step < a.rows) fetch(r + a.stages * step, stage);
+        if (++stage == a.stages) {
+            stage = 0;
+            parity ^= 1;
+        }
+        now = next;
+    }
+    if (!a.part) return;
+    float* part = a.part + 2LL * blockIdx.x * a.D;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+        if (at + k * lanes < packs) {
+#pragma unroll
+            for (int j = 0; j < EV; ++j) {
+                const int c = (at + k * lanes) * EV + j, i = (k * EV + j) / 2;
+                part[c] = (k * EV + j) & 1 ? dw[i].y : dw[i].x;
+                part[a.D + c] = (k * EV + j) & 1 ? db[i].y : db[i].x;
+            }
+        }
+}
+
+// ---- long rows: one block per row, the row read again from L2 for each step ---------------------
 template <class T, class W>
 __global__ void __launch_bounds__(512) ln_fwd_wide(const LnFwdArgs a) {
     __shared__ float sh[16];
@@ -325,7 +639,7 @@ __global__ void __launch_bounds__(512) ln_fwd_wide(const LnFwdArgs a) {
 }
 
 template <class T, class W>
-__global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
+__global__ void __launch_bounds__(512) ln_bwd_wide(const LnBwdArgs a) {
     __shared__ float sh[16];
     const W* w = static_cast<const W*>(a.w);
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -374,86 +688,99 @@ __global__ void __launch_bounds__(256) ln_bwd_cols(const LnBwdArgs a) {
     }
 }
 
-// The slices' (or blocks') sums: 32 columns and 8 runs of slices to a block, the runs added in their order.  Launched
+// The slices' (or blocks') sums: 32 columns and 32 runs of slices to a block, the runs added in a fixed order.  Launched
 // as the programmatic dependent of the kernel that makes the sums.
 template <class W>
-__global__ void __launch_bounds__(256) ln_bwd_fold(const LnBwdArgs a) {
-    __shared__ float sh[8][32];
+__global__ void __launch_bounds__(1024) ln_bwd_fold(const LnBwdArgs a) {
+    __shared__ float sh[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const long long i = blockIdx.x * 32LL + tx;                   // of 2 D values
     asm volatile("griddepcontrol.wait;" ::: "memory");
     float t = 0.f;
     if (i < 2LL * a.D) {
-        const int per = (a.slices + 7) / 8, s0 = ty * per, s1 = min(a.slices, s0 + per);
-#pragma unroll 8
+        const int per = (a.slices + 31) / 32, s0 = ty * per, s1 = min(a.slices, s0 + per);
+#pragma unroll 16
         for (int s = s0; s < s1; ++s) t += a.part[2LL * s * a.D + i];
     }
     sh[ty][tx] = t;
     __syncthreads();
-    if (ty == 0 && i < 2LL * a.D) {
-        for (int k = 1; k < 8; ++k) t += sh[k][tx];
-        W* out = static_cast<W*>(i < a.D ? a.dw : a.db);
-        if (out) out[i < a.D ? i : i - a.D] = from_f32<W>(t);
+    t = warp_sum(sh[tx][ty]);                                     // warp k adds column k
+    const long long o = blockIdx.x * 32LL + ty;
+    if (tx == 0 && o < 2LL * a.D) {
+        W* out = static_cast<W*>(o < a.D ? a.dw : a.db);
+        if (out) out[o < a.D ? o : o - a.D] = from_f32<W>(t);
     }
 }
 
-constexpr int kMaxParts = 592;        // blocks whose sums the workspace holds: 4 on each of 148 SMs
+constexpr int kMaxParts = 1184;       // blocks whose sums the workspace holds: 8 on each of 148 SMs
 
-// rows of the column sums of rows too wide for registers
+// slices of the column sums of long rows
 int ln_slices(int64_t rows) {
     const int64_t s = (rows + 31) / 32;
     return (int)(s < 1 ? 1 : s > 296 ? 296 : s);
 }
 
-using Yes = std::bool_constant<true>;
-using No = std::bool_constant<false>;
 template <int N>
 using Num = std::integral_constant<int, N>;
 
-// How a row of `packs` accesses is shared: by `lanes` threads with `nv` accesses each (nv = 0: too wide).  Up to 32
-// threads: `many` rows to a block.  Above: blocks of about 256 threads while two accesses of each do, then up to 512, then
-// (`big`) up to 1024 with half the registers.
-struct LnShape {
-    int nv, lanes;
-    bool many, big;
-};
-LnShape ln_shape(long long packs, int max_nv_many, int max_nv) {
-    LnShape s{};
-    for (int nv = 1; nv <= max_nv_many; nv *= 2)
-        if (packs <= 32LL * nv) {
-            s.nv = nv;
-            s.many = true;
-            s.lanes = 32;
-            while (s.lanes > 1 && (long long)(s.lanes / 2) * nv >= packs) s.lanes /= 2;
-            return s;
-        }
-    for (int nv = 1; nv <= max_nv; nv *= 2)
-        if (packs <= (nv == max_nv ? 1024LL : 256LL) * nv) {
-            s.nv = nv;
-            s.lanes = (int)((packs + 32LL * nv - 1) / (32LL * nv) * 32);
-            s.big = s.lanes > 512;
-            return s;
-        }
-    return s;
+// lanes that share a short row of `packs` accesses, nv each: the fewest, a power of two
+int short_lanes(long long packs, int nv) {
+    int lanes = 32;
+    while (lanes > 1 && (long long)(lanes / 2) * nv >= packs) lanes /= 2;
+    return lanes;
 }
 
-template <class T, class W, int EV, int NV, bool MANY, int MAXT>
-int ln_fwd_launch(LnFwdArgs a, LnShape h, int sms, cudaStream_t s) {
-    auto kern = ln_fwd<T, W, EV, NV, MANY, MAXT>;
-    const int block = MANY ? 256 : h.lanes, per = MANY ? 256 / h.lanes : 1;
-    const long long want = (a.rows + per - 1) / per, most = (long long)sms * resident_blocks((const void*)kern, block, 0);
-    a.lanes = h.lanes;
-    return launch_kernel(kern, (int)(want < most ? want : most), block, 0, s, false, a);
+constexpr size_t kRowSmem = 200 * 1024;      // of the 227 KB that a block may have
+
+template <class T, class W, int EV, int NV>
+int ln_fwd_short_launch(LnFwdArgs a, int sms, cudaStream_t s) {
+    auto kern = ln_fwd_short<T, W, EV, NV>;
+    a.lanes = short_lanes(a.D / EV, NV);
+    const int per = 256 / a.lanes;
+    const long long want = (a.rows + per - 1) / per, most = (long long)sms * resident_blocks((const void*)kern, 256, 0);
+    return launch_kernel(kern, (int)(want < most ? want : most), 256, 0, s, false, a);
 }
-template <class T, class W, int EV, int NV, bool MANY, int MAXT>
-int ln_bwd_launch(LnBwdArgs& a, LnShape h, int sms, cudaStream_t s) {
-    auto kern = ln_bwd<T, W, EV, NV, MANY, MAXT>;
-    const int block = MANY ? 256 : h.lanes, per = MANY ? 256 / h.lanes : 1;
-    const size_t smem = MANY ? (size_t)2 * NV * EV * 256 * 4 : 0;
+
+// One block of up to 16 warps to an SM; as many teams as there are rows for, as many buffers as fit (up to 4).
+template <class T, class W, int EV, int NV>
+int ln_fwd_rows_launch(LnFwdArgs a, int team, int sms, cudaStream_t s) {
+    const long long per_sm = (a.rows + sms - 1) / sms;
+    int teams = 16 / team;
+    if (per_sm < teams) teams = (int)per_sm;
+    a.team = team;
+    a.buf = (int)((a.D * sizeof(T) + 15) / 16 * 16 + (EV == 1 ? 16 : 0));
+    a.wbytes = (int)((a.D * sizeof(W) + 15) / 16 * 16);
+    while (teams > 1 && 2 * (size_t)a.wbytes + (size_t)teams * a.buf > kRowSmem) --teams;
+    const size_t room = (kRowSmem - 2 * (size_t)a.wbytes) / ((size_t)teams * a.buf);
+    a.stages = (int)(room > 4 ? 4 : room);
+    const size_t smem = 2 * (size_t)a.wbytes + (size_t)teams * a.stages * (a.buf + 8) + 2 * (size_t)teams * team * sizeof(float2);
+    const long long want = (a.rows + teams - 1) / teams;
+    return launch_kernel(ln_fwd_rows<T, W, EV, NV>, (int)(want < sms ? want : sms), teams * team * 32, smem, s, false, a);
+}
+
+template <class T, class W, int EV, int NV>
+int ln_bwd_short_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
+    auto kern = ln_bwd_short<T, W, EV, NV>;
+    a.lanes = short_lanes(a.D / EV, NV);
+    const int per = 256 / a.lanes;
+    const size_t smem = (size_t)2 * NV * EV * 256 * 4;
     const long long want = (a.rows + per - 1) / per;
+    long long most = (long long)sms * resident_blocks((const void*)kern, 256, smem);
+    most = most < kMaxParts ? most : kMaxParts;
+    a.slices = (int)(want < most ? want : most);
+    return launch_kernel(kern, a.slices, 256, smem, s, false, a);
+}
+
+template <class T, class W, int EV, int NV>
+int ln_bwd_rows_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
+    auto kern = ln_bwd_rows2<T, W, EV, NV>;
+    const int block = (int)((a.D / EV + 32 * NV - 1) / (32 * NV) * 32);
+    a.buf = (int)((a.D * sizeof(T) + 15) / 16 * 16 + (EV == 1 ? 16 : 0));
+    a.stages = 8 * (size_t)a.buf <= kRowSmem ? 2 : 1;
+    const size_t smem = (size_t)a.stages * 4 * a.buf + (a.stages + 1) * 8 + 2 * (size_t)(block / 32) * 16;
+    const long long want = (a.rows + 1) / 2;
     long long most = (long long)sms * resident_blocks((const void*)kern, block, smem);
     most = most < kMaxParts ? most : kMaxParts;
-    a.lanes = h.lanes;
     a.slices = (int)(want < most ? want : most);
     return launch_kernel(kern, a.slices, block, smem, s, false, a);
 }
@@ -476,7 +803,9 @@ int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype,
         return HFUSE_ERR_ALIGNMENT;
     DeviceFacts f;
     if (int rc = device_facts(f)) return rc;
-    LnFwdArgs a{x, weight, bias, y, mean, invstd, rows, ld_x, D, 0, 1.f / (float)D, eps};
+    LnFwdArgs a{};
+    a.x = x; a.w = weight; a.b = bias; a.y = y; a.mean = mean; a.invstd = invstd;
+    a.rows = rows; a.ldx = ld_x; a.D = D; a.inv_d = 1.f / (float)D; a.eps = eps;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = aligned_to(x, 16) && aligned_to(y, 16) && aligned_to(weight, 16) && aligned_to(bias, 16) &&
                       D * es % 16 == 0 && ld_x * es % 16 == 0;
@@ -484,20 +813,24 @@ int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype,
         using T = typename decltype(t)::type;
         using W = typename decltype(w)::type;
         constexpr int EV = 16 / sizeof(T);
-        const LnShape h = ln_shape(wide ? D / EV : D, 4, 4);
-        if (h.nv == 0) {
-            const int grid = (int)(rows < f.sms * 4LL ? rows : f.sms * 4LL);
-            return launch_kernel(ln_fwd_wide<T, W>, grid, 512, 0, s, false, a);
+        const long long packs = wide ? D / EV : D;
+        // short rows: up to 4 accesses of 32 lanes (unaligned: 2)
+        if (wide && packs <= 32) return ln_fwd_short_launch<T, W, EV, 1>(a, f.sms, s);
+        if (wide && packs <= 64) return ln_fwd_short_launch<T, W, EV, 2>(a, f.sms, s);
+        if (!wide && packs <= 32) return ln_fwd_short_launch<T, W, 1, 1>(a, f.sms, s);
+        if (!wide && packs <= 64) return ln_fwd_short_launch<T, W, 1, 2>(a, f.sms, s);
+        // rows that fit shared memory beside their weights.  Few rows are spread over more warps each.
+        const bool few = rows < 4LL * f.sms;
+        auto team = [&](int nv) { return (int)((packs + 32LL * nv - 1) / (32LL * nv)); };
+        if (2 * D * ws + D * es + 64 <= kRowSmem) {
+            if (wide && packs <= 32 * 4 * 16 && (few || packs <= 32 * 4)) return ln_fwd_rows_launch<T, W, EV, 4>(a, team(4), f.sms, s);
+            if (wide && packs <= 32 * 8) return ln_fwd_rows_launch<T, W, EV, 8>(a, team(8), f.sms, s);
+            if (wide && packs <= 32 * 16 * 16) return ln_fwd_rows_launch<T, W, EV, 16>(a, team(16), f.sms, s);
+            if (!wide && packs <= 32 * 8 * 16 && (few || packs <= 32 * 8)) return ln_fwd_rows_launch<T, W, 1, 8>(a, team(8), f.sms, s);
+            if (!wide && packs <= 32 * 32 * 16) return ln_fwd_rows_launch<T, W, 1, 32>(a, team(32), f.sms, s);
         }
-        auto go = [&](auto many, auto nv, auto maxt) {
-            constexpr bool MANY = decltype(many)::value;
-            constexpr int NV = decltype(nv)::value, MAXT = decltype(maxt)::value;
-            return wide ? ln_fwd_launch<T, W, EV, NV, MANY, MAXT>(a, h, f.sms, s) : ln_fwd_launch<T, W, 1, NV, MANY, MAXT>(a, h, f.sms, s);
-        };
-        if (h.many)
-            return h.nv == 1 ? go(Yes{}, Num<1>{}, Num<256>{}) : h.nv == 2 ? go(Yes{}, Num<2>{}, Num<256>{}) : go(Yes{}, Num<4>{}, Num<256>{});
-        if (h.big) return go(No{}, Num<4>{}, Num<1024>{});
-        return h.nv == 1 ? go(No{}, Num<1>{}, Num<512>{}) : h.nv == 2 ? go(No{}, Num<2>{}, Num<512>{}) : go(No{}, Num<4>{}, Num<512>{});
+        const int grid = (int)(rows < f.sms * 4LL ? rows : f.sms * 4LL);
+        return launch_kernel(ln_fwd_wide<T, W>, grid, 512, 0, s, false, a);
     });
 }
 
@@ -524,43 +857,36 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
     if (int rc = device_facts(f)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int slices = ln_slices(rows);
-    LnBwdArgs a{x, grad_out, weight, mean, invstd, grad_in, grad_weight, grad_bias, want_w ? static_cast<float*>(workspace) : nullptr,
-                rows, ld_x, ld_grad_out, (rows + slices - 1) / slices, D, slices, 0, 1.f / (float)D};
+    LnBwdArgs a{};
+    a.x = x; a.dy = grad_out; a.w = weight; a.mean = mean; a.invstd = invstd;
+    a.dx = grad_in; a.dw = grad_weight; a.db = grad_bias; a.part = want_w ? static_cast<float*>(workspace) : nullptr;
+    a.rows = rows; a.ldx = ld_x; a.lddy = ld_grad_out; a.D = D; a.inv_d = 1.f / (float)D;
+    a.slices = slices; a.slice_rows = (rows + slices - 1) / slices;
     const bool wide = aligned_to(x, 16) && aligned_to(grad_out, 16) && aligned_to(grad_in, 16) && aligned_to(weight, 16) &&
                       D * es % 16 == 0 && ld_x * es % 16 == 0 && ld_grad_out * es % 16 == 0;
     return by_types(dtype, weight_dtype, [&](auto t, auto w) {
         using T = typename decltype(t)::type;
         using W = typename decltype(w)::type;
-        constexpr int EV = 16 / sizeof(T);
-        const LnShape h = rows > 0 ? ln_shape(wide ? D / EV : D, 2, wide ? EV == 8 ? 2 : 4 : 8) : LnShape{};
+        constexpr int EV = 16 / sizeof(T), NV = 16 / EV;               // 16 columns to a thread
+        const long long packs = wide ? D / EV : D;
         int rc;
-        if (h.nv == 0) {
+        if (rows > 0 && packs <= 64) {
+            rc = wide ? packs <= 32 ? ln_bwd_short_launch<T, W, EV, 1>(a, f.sms, s) : ln_bwd_short_launch<T, W, EV, 2>(a, f.sms, s)
+                      : packs <= 32 ? ln_bwd_short_launch<T, W, 1, 1>(a, f.sms, s) : ln_bwd_short_launch<T, W, 1, 2>(a, f.sms, s);
+        } else if (rows > 0 && D <= 16 * 512) {
+            rc = wide ? ln_bwd_rows_launch<T, W, EV, NV>(a, f.sms, s)
+                 : D <= 8 * 256 ? ln_bwd_rows_launch<T, W, 1, 8>(a, f.sms, s) : ln_bwd_rows_launch<T, W, 1, 16>(a, f.sms, s);
+        } else {
             if (grad_in && rows > 0) {
                 const int grid = (int)(rows < f.sms * 4LL ? rows : f.sms * 4LL);
-                if ((rc = launch_kernel(ln_bwd_rows<T, W>, grid, 512, 0, s, false, a))) return rc;
+                if ((rc = launch_kernel(ln_bwd_wide<T, W>, grid, 512, 0, s, false, a))) return rc;
             }
             if (!want_w) return (int)HFUSE_OK;
             ln_bwd_cols<T><<<dim3((unsigned)((D + 31) / 32), (unsigned)slices), 256, 0, s>>>(a);
             rc = check_launch();
-        } else {
-            auto go = [&](auto many, auto nv, auto maxt) {
-                constexpr bool MANY = decltype(many)::value;
-                constexpr int NV = decltype(nv)::value, MAXT = decltype(maxt)::value;
-                if (!wide) return ln_bwd_launch<T, W, 1, NV, MANY, MAXT>(a, h, f.sms, s);
-                if constexpr (NV * EV <= 16) return ln_bwd_launch<T, W, EV, NV, MANY, MAXT>(a, h, f.sms, s);
-                else return (int)HFUSE_ERR_BAD_ARG;                    // ln_shape gives no such shape
-            };
-            if (h.many) rc = h.nv == 1 ? go(Yes{}, Num<1>{}, Num<256>{}) : go(Yes{}, Num<2>{}, Num<256>{});
-            else if (h.big)
-                rc = h.nv == 2 ? go(No{}, Num<2>{}, Num<1024>{}) : h.nv == 4 ? go(No{}, Num<4>{}, Num<1024>{}) : go(No{}, Num<8>{}, Num<1024>{});
-            else
-                rc = h.nv == 1   ? go(No{}, Num<1>{}, Num<512>{})
-                     : h.nv == 2 ? go(No{}, Num<2>{}, Num<512>{})
-                     : h.nv == 4 ? go(No{}, Num<4>{}, Num<512>{})
-                                 : go(No{}, Num<8>{}, Num<512>{});
         }
         if (rc || !want_w) return rc;
-        return launch_kernel(ln_bwd_fold<W>, (int)((2LL * D + 31) / 32), 256, 0, s, true, a);
+        return launch_kernel(ln_bwd_fold<W>, (int)((2LL * D + 31) / 32), 1024, 0, s, true, a);
     });
 }
 

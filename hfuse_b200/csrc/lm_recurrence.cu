@@ -104,18 +104,12 @@ __device__ __forceinline__ void stage_rows(T* dst, const T* src, long long strid
     }
 }
 
-template <class T, int CPL>
-__device__ __forceinline__ void read_row(const T* row, float (&v)[CPL]) {
-    const Pack<T, CPL> p = *reinterpret_cast<const Pack<T, CPL>*>(row);
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) v[c] = to_f32(p.v[c]);
-}
 // Elements are worked on in pairs: the two channels of a lane, or two steps of its only channel.
 template <class T, int CPL>
 __device__ __forceinline__ float2 read_pair(const T* at, int i) {
     constexpr int C = 32 * CPL;
     if constexpr (CPL == 2) {
-        return unpack2(*reinterpret_cast<const Pack<T, 2>*>(at + i * C));
+        return pair_of(*reinterpret_cast<const Pack<T, 2>*>(at + i * C), 0);
     } else {
         return make_float2(to_f32(at[2 * i * C]), to_f32(at[(2 * i + 1) * C]));
     }
@@ -158,15 +152,15 @@ template <class T, int CPL, bool WHOLE>
 __device__ __forceinline__ void write_pair(T* at, long long stride, int i, float2 v, int steps, int left) {
     if constexpr (CPL == 2) {
         if constexpr (WHOLE) {             // rows keep the alignment of two elements, D is even
-            const float w[2] = {v.x, v.y};
-            if (i < steps && left > 0) store_stream<T, 2>(at + i * stride, pack_f32<T, 2>(w));
+            const float2 w[1] = {v};
+            if (i < steps && left > 0) store_stream<T, 2>(at + i * stride, pack_pairs<T, 2>(w));
         } else if (i < steps) {
             if (left > 0) at[i * stride] = from_f32<T>(v.x);
             if (left > 1) at[i * stride + 1] = from_f32<T>(v.y);
         }
     } else if (left > 0) {
-        if (2 * i < steps) store_stream<T, 1>(at + 2 * i * stride, Pack<T, 1>{{from_f32<T>(v.x)}});
-        if (2 * i + 1 < steps) store_stream<T, 1>(at + (2 * i + 1) * stride, Pack<T, 1>{{from_f32<T>(v.y)}});
+        if (2 * i < steps) at[2 * i * stride] = from_f32<T>(v.x);
+        if (2 * i + 1 < steps) at[(2 * i + 1) * stride] = from_f32<T>(v.y);
     }
 }
 template <int CPL>
@@ -184,20 +178,19 @@ __device__ __forceinline__ void write_state(float* p, const float (&v)[CPL], int
 // ---- maps h -> A h + H of one stretch of steps in shared memory: a lane's A, then its H ---------------------
 template <int CPL>
 __device__ __forceinline__ void write_map(float* m, const float (&A)[CPL], const float (&H)[CPL]) {
-    Pack<float, 2 * CPL> r;
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) { r.v[c] = A[c]; r.v[CPL + c] = H[c]; }
-    *reinterpret_cast<Pack<float, 2 * CPL>*>(m) = r;
+    if constexpr (CPL == 2) *reinterpret_cast<float4*>(m) = make_float4(A[0], A[1], H[0], H[1]);
+    else *reinterpret_cast<float2*>(m) = make_float2(A[0], H[0]);
 }
 template <int CPL>
 __device__ __forceinline__ void apply_map(const float* m, float (&h)[CPL]) {
-    const Pack<float, 2 * CPL> r = *reinterpret_cast<const Pack<float, 2 * CPL>*>(m);
     if constexpr (CPL == 2) {
-        const float2 n = fma2(make_float2(r.v[0], r.v[1]), make_float2(h[0], h[1]), make_float2(r.v[2], r.v[3]));
+        const float4 r = *reinterpret_cast<const float4*>(m);
+        const float2 n = fma2(make_float2(r.x, r.y), make_float2(h[0], h[1]), make_float2(r.z, r.w));
         h[0] = n.x;
         h[1] = n.y;
     } else {
-        h[0] = fmaf(r.v[0], h[0], r.v[1]);
+        const float2 r = *reinterpret_cast<const float2*>(m);
+        h[0] = fmaf(r.x, h[0], r.y);
     }
 }
 // the map of the steps so far, then m's
@@ -311,7 +304,7 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
         const T* sx = sg + rows * C;
         cp_wait<1>();
         __syncthreads();
-        if (p.split == 1 && it > 0) read_row<float, CPL>(next, carry);
+        if (p.split == 1 && it > 0) read_state<CPL>(next, carry, CPL);
         float2 h[N], a[N];                                // results from zero, products of the a so far
         float H[CPL], A[CPL];
 #pragma unroll
@@ -421,7 +414,7 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
         cp_wait<0>();
         __syncthreads();                                  // the stage is there, and the other one has been read
         issue(k + 1);
-        if (p.split == 1 && k > 0) read_row<float, CPL>(next, carry);
+        if (p.split == 1 && k > 0) read_state<CPL>(next, carry, CPL);
         // E, what e of zero becomes over the steps, is the sum of dy_t times the product of the a up to a_t
         float2 a[N], z[N];
         float A[CPL], H[CPL], E[CPL];
