@@ -67,6 +67,20 @@ __device__ __forceinline__ Pack<T, N> load_cached(const T* p) {
     }
     return r;
 }
+// the same from shared memory (32-bit address)
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> load_shared(uint32_t p) {
+    Pack<T, N> r;
+    if constexpr (r.BYTES == 16)
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "r"(p) : "memory");
+    else if constexpr (r.BYTES == 8)
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "r"(p) : "memory");
+    else if constexpr (r.BYTES == 4)
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r.w[0]) : "r"(p) : "memory");
+    else
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r.w[0]) : "r"(p) : "memory");
+    return r;
+}
 // outputs that this kernel does not read again
 template <class T, int N>
 __device__ __forceinline__ void store_stream(T* p, const Pack<T, N>& r) {

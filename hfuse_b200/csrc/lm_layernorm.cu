@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(256) ln_bwd_short(const LnBwdArgs a) {
     }
     Row<NV, EV, T> rx, rd, nx, nd;
     float mu = 0.f, is = 0.f, nmu = 0.f, nis = 0.f;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the sums' last step waits for this grid's end
     if (r < a.rows) {
         load_row<T, EV, NV>(rx, x + r * a.ldx, at, lanes, packs);
         load_row<T, EV, NV>(rd, dy + r * a.lddy, at, lanes, packs);
@@ -299,23 +300,31 @@ __device__ __forceinline__ void team_sync(int team, int warps) {
 }
 
 // A row's elements in the registers of a team: accesses of EV elements, or (EV = 1) single elements in pairs of
-// accesses.  VALUES pairs; element(s) of pair i that are beyond the row have a place, but no value.
+// accesses.  VALUES pairs.  A place beyond the row holds the row's last access again: who adds up has to leave it out.
 template <class T, int EV, int NV>
 struct Team {
     static constexpr int VALUES = NV * EV / 2;
     Pack<T, EV> v[NV];
-    __device__ __forceinline__ void read(const unsigned char* row, int at, int lanes, int packs) {
+    __device__ __forceinline__ void read(uint32_t row, const int (&place)[NV]) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (at + k * lanes < packs) v[k] = *(reinterpret_cast<const Pack<T, EV>*>(row) + at + k * lanes);
-            else v[k] = {};
-        }
+        for (int k = 0; k < NV; ++k) v[k] = load_shared<T, EV>(row + place[k]);
     }
     __device__ __forceinline__ float2 get(int i) const {
         if constexpr (EV == 1) return make_float2(pair_of<T, 1>(v[2 * i], 0).x, pair_of<T, 1>(v[2 * i + 1], 0).x);
         else return pair_of<T, EV>(v[i / (EV / 2)], i % (EV / 2));
     }
 };
+// where in a row's buffer a thread's accesses are
+template <class T, int EV, int NV>
+__device__ __forceinline__ void places(int (&place)[NV], int at, int lanes, int packs) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) place[k] = min(at + k * lanes, packs - 1) * EV * (int)sizeof(T);
+}
+// the 16-byte boundary's distance from row r, in bytes; the low bits of a product need no wide multiplication
+template <class T>
+__device__ __forceinline__ int shift_of(const T* base, long long ld, long long r) {
+    return (int)(((unsigned)reinterpret_cast<uintptr_t>(base) + (unsigned)r * ((unsigned)ld * (unsigned)sizeof(T))) & 15u);
+}
 // which of a pair's elements exist
 template <int EV>
 __device__ __forceinline__ void exists(int i, int at, int lanes, int packs, bool& x, bool& y) {
@@ -327,6 +336,27 @@ __device__ __forceinline__ void exists(int i, int at, int lanes, int packs, bool
     }
 }
 
+// The weights are in shared memory as floats, the halves of eight-element accesses in planes of their own, so that
+// neighbouring lanes read neighbouring 16 bytes.
+template <int EV>
+__device__ __forceinline__ int weight_at(int c, int packs) {
+    if constexpr (EV == 8) return ((c & 4) ? packs * 4 : 0) + (c >> 3) * 4 + (c & 3);
+    else return c;
+}
+template <int EV>
+__device__ __forceinline__ void weight_pairs(const float* w, int p, int packs, float2 (&to)[kPairs<EV>]) {
+    if constexpr (EV == 1) {
+        to[0] = make_float2(w[p], 0.f);
+    } else {
+#pragma unroll
+        for (int h = 0; h < EV / 4; ++h) {
+            const float4 v = *reinterpret_cast<const float4*>(w + h * packs * 4 + p * 4);
+            to[2 * h] = make_float2(v.x, v.y);
+            to[2 * h + 1] = make_float2(v.z, v.w);
+        }
+    }
+}
+
 template <class T, class W, int EV, int NV>
 __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -334,8 +364,8 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
     const T* x = static_cast<const T*>(a.x);
     const int M = a.team, lane = threadIdx.x & 31, warp = warp_index(), warps = blockDim.x >> 5, teams = warps / M;
     const int team = warp / M, part = warp - team * M, lanes = 32 * M, at = part * 32 + lane, packs = a.D / EV;
-    W* sw = reinterpret_cast<W*>(smem);
-    W* sb = reinterpret_cast<W*>(smem + a.wbytes);
+    float* sw = reinterpret_cast<float*>(smem);
+    float* sb = reinterpret_cast<float*>(smem + a.wbytes);
     unsigned char* ring = smem + 2 * a.wbytes + (size_t)team * a.stages * a.buf;
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + 2 * a.wbytes + (size_t)teams * a.stages * a.buf) + team * a.stages;
     float2* moments = reinterpret_cast<float2*>(smem + 2 * a.wbytes + (size_t)teams * a.stages * (a.buf + 8));    // [2][warps]
@@ -348,9 +378,15 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
         for (int s = 0; s < a.stages; ++s)
             if (r + s * step < a.rows) fetch_row(ring + (size_t)s * a.buf, bars + s, x, a.ldx, a.rows, a.D, r + s * step);
     }
-    for (int i = threadIdx.x; i < a.D; i += blockDim.x) {
-        sw[i] = a.w ? static_cast<const W*>(a.w)[i] : from_f32<W>(1.f);
-        sb[i] = a.b ? static_cast<const W*>(a.b)[i] : from_f32<W>(0.f);
+    for (int p = threadIdx.x; p < packs; p += blockDim.x) {
+        float2 w[kPairs<EV>], b[kPairs<EV>];
+        weights_of<W, EV>(static_cast<const W*>(a.w), p, w, 1.f);
+        weights_of<W, EV>(static_cast<const W*>(a.b), p, b, 0.f);
+#pragma unroll
+        for (int j = 0; j < EV; ++j) {
+            sw[weight_at<EV>(p * EV + j, packs)] = j & 1 ? w[j / 2].y : w[j / 2].x;
+            sb[weight_at<EV>(p * EV + j, packs)] = j & 1 ? b[j / 2].y : b[j / 2].x;
+        }
     }
     // elements that the team's warp number `lane` holds
     float count = 0.f, inv_count = 0.f;
@@ -362,6 +398,9 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
         inv_count = n ? 1.f / count : 0.f;
     }
     const float mine = M > 1 ? __shfl_sync(0xffffffffu, inv_count, part) : a.inv_d;
+    const bool whole = packs == NV * lanes;                // no place beyond the row
+    int place[NV];
+    places<T, EV, NV>(place, at, lanes, packs);
     __syncthreads();
     int stage = 0, parity = 0;
     for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
@@ -369,27 +408,40 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
         const bool there = mbar_wait(bars + stage, parity, kRowWaitNs);
         int shift = 0;
         if constexpr (EV == 1) {
-            shift = (int)(reinterpret_cast<uintptr_t>(x + r * a.ldx) & 15);
+            shift = shift_of(x, a.ldx, r);
             if (row_lacks(x, a.ldx, a.rows, a.D, r)) {
                 patch_row(buf, x, a.ldx, a.rows, a.D, r, at, lanes);
                 team_sync(team, M);
             }
         }
-        Team<T, EV, NV> row;
-        row.read(buf + shift, at, lanes, packs);
-        float2 s2 = make_float2(0.f, 0.f);
+        float2 f[VALUES], s2 = make_float2(0.f, 0.f), q2 = s2;
+        {
+            Team<T, EV, NV> row;
+            row.read(smem_u32(buf) + shift, place);
 #pragma unroll
-        for (int i = 0; i < VALUES; ++i) s2 = add2(s2, row.get(i));              // zeros beyond the row
+            for (int i = 0; i < VALUES; ++i) {
+                f[i] = row.get(i);
+                if (whole) {
+                    s2 = add2(s2, f[i]);
+                } else {
+                    bool ex, ey;
+                    exists<EV>(i, at, lanes, packs, ex, ey);
+                    s2 = add2(s2, make_float2(ex ? f[i].x : 0.f, ey ? f[i].y : 0.f));
+                }
+            }
+        }
         const float s = warp_sum(s2.x + s2.y), mid = s * mine;                   // the mean of the warp's part
-        float2 q2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
-            float2 d = add2(row.get(i), make_float2(-mid, -mid));
-            bool ex, ey;
-            exists<EV>(i, at, lanes, packs, ex, ey);
-            if (!ex) d.x = 0.f;
-            if (!ey) d.y = 0.f;
-            q2 = fma2(d, d, q2);
+            f[i] = add2(f[i], make_float2(-mid, -mid));
+            if (whole) {
+                q2 = fma2(f[i], f[i], q2);
+            } else {
+                bool ex, ey;
+                exists<EV>(i, at, lanes, packs, ex, ey);
+                const float2 d = make_float2(ex ? f[i].x : 0.f, ey ? f[i].y : 0.f);
+                q2 = fma2(d, d, q2);
+            }
         }
         float q = warp_sum(q2.x + q2.y), mu = mid;
         if (M == 1) {
@@ -412,17 +464,23 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
         }
         float is = inv_std(q, a.inv_d, a.eps);
         if (!there) mu = is = __int_as_float(0x7fc00000);
+        // f is relative to the mean of the warp's part: y = (f + (mid - mu)) is w + b
+        const float2 is2 = make_float2(is, is), move = make_float2((mid - mu) * is, (mid - mu) * is);
         T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int p = at + k * lanes;
             if (p >= packs) continue;
-            const Pack<W, EV> w = *(reinterpret_cast<const Pack<W, EV>*>(sw) + p), b = *(reinterpret_cast<const Pack<W, EV>*>(sb) + p);
-            float2 o[kPairs<EV>];
+            float2 w[kPairs<EV>], b[kPairs<EV>], o[kPairs<EV>];
+            weight_pairs<EV>(sw, p, packs, w);
+            weight_pairs<EV>(sb, p, packs, b);
 #pragma unroll
-            for (int j = 0; j < kPairs<EV>; ++j)
-                o[j] = fma2(add2(pair_of<T, EV>(row.v[k], j), make_float2(-mu, -mu)), mul2(pair_of<W, EV>(w, j), make_float2(is, is)),
-                            pair_of<W, EV>(b, j));
+            for (int j = 0; j < kPairs<EV>; ++j) {
+                float2 v;
+                if constexpr (EV == 1) v = make_float2(k & 1 ? f[k / 2].y : f[k / 2].x, 0.f);
+                else v = f[k * (EV / 2) + j];
+                o[j] = fma2(fma2(v, is2, move), w[j], b[j]);
+            }
             store_stream<T, EV>(y + p * EV, pack_pairs<T, EV>(o));
         }
         if (lead) {
@@ -446,17 +504,21 @@ __device__ __forceinline__ float warp_sum4(float a, float b, float c, float d, i
     return t;
 }
 
-// A block takes two rows at a time: [stage][x, dy][row] buffers.
+// Teams of warps take two rows at a time, [team][stage][x, dy][row] buffers; the block's teams add up their dw and db in
+// the same memory at the end.
 template <class T, class W, int EV, int NV>
-__global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
+__global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int VALUES = NV * EV / 2;
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.dy);
     const W* w = static_cast<const W*>(a.w);
-    const int lanes = blockDim.x, at = threadIdx.x, lane = threadIdx.x & 31, warp = warp_index(), warps = lanes >> 5, packs = a.D / EV;
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)a.stages * 4 * a.buf);
-    float* sums = reinterpret_cast<float*>(bars + a.stages + (a.stages & 1));            // [2][warps][4]
+    const int lanes = a.lanes, warps = lanes >> 5, lane = threadIdx.x & 31, team = warp_index() / warps, warp = warp_index() - team * warps;
+    const int teams = blockDim.x / lanes, at = warp * 32 + lane, packs = a.D / EV;
+    unsigned char* ring = smem + (size_t)team * a.stages * 4 * a.buf;
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)teams * a.stages * 4 * a.buf) + team * 2;
+    float* sums = reinterpret_cast<float*>(smem + (size_t)teams * (a.stages * 4 * (size_t)a.buf + 16)) + team * 8 * warps;   // [2][warps][4]
+    // a weight of zero keeps places beyond the row out of the row sums; nothing is stored for them
     float2 kw[VALUES], dw[VALUES], db[VALUES];
     {
         Team<W, EV, NV> t;
@@ -467,18 +529,23 @@ __global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
-            kw[i] = w ? t.get(i) : make_float2(1.f, 1.f);
+            bool ex, ey;
+            exists<EV>(i, at, lanes, packs, ex, ey);
+            kw[i] = w ? t.get(i) : make_float2(ex ? 1.f : 0.f, ey ? 1.f : 0.f);
             dw[i] = db[i] = make_float2(0.f, 0.f);
         }
     }
-    // the block's k-th pair of rows; lanes 0 to 3 of the first warp fetch one row each
-    const long long step = 2LL * gridDim.x;
+    int place[NV];
+    places<T, EV, NV>(place, at, lanes, packs);
+    // a pair of rows; lanes 0 to 3 of the team's first warp fetch one row each
+    const long long step = 2LL * gridDim.x * teams;
     auto fetch = [&](long long r, int s) {
         if (warp == 0 && lane < 4) {
             const long long row = r + (lane & 1);
+            unsigned char* buf = ring + (size_t)(4 * s + lane) * a.buf;
             if (row >= a.rows) mbar_arrive(bars + s);
-            else if (lane < 2) fetch_row(smem + (size_t)(4 * s + lane) * a.buf, bars + s, x, a.ldx, a.rows, a.D, row);
-            else fetch_row(smem + (size_t)(4 * s + lane) * a.buf, bars + s, dy, a.lddy, a.rows, a.D, row);
+            else if (lane < 2) fetch_row(buf, bars + s, x, a.ldx, a.rows, a.D, row);
+            else fetch_row(buf, bars + s, dy, a.lddy, a.rows, a.D, row);
         }
     };
     // mean and invstd of a pair of rows in lanes 0 to 3
@@ -486,35 +553,30 @@ __global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
         const long long row = r + (lane & 1);
         return lane < 4 && row < a.rows ? __ldg((lane < 2 ? a.mean : a.invstd) + row) : 0.f;
     };
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < a.stages; ++s) mbar_init(bars + s, 4);
+    if (at == 0) {
+        mbar_init(bars, 4);
+        mbar_init(bars + 1, 4);
         fence_mbar_init();
     }
-    __syncthreads();
-    long long r = 2LL * blockIdx.x;
+    team_sync(team, warps);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the sums' last step waits for this grid's end
+    long long r = 2LL * ((long long)blockIdx.x * teams + team);
     for (int s = 0; s < a.stages; ++s)
         if (r + s * step < a.rows) fetch(r + s * step, s);
     float now = stats(r), next = 0.f;
     int stage = 0, parity = 0;
     for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
         next = stats(r + step);
-        unsigned char* buf = smem + (size_t)4 * stage * a.buf;
+        unsigned char* buf = ring + (size_t)4 * stage * a.buf;
         const bool there = mbar_wait(bars + stage, parity, kRowWaitNs);
-        const unsigned char *px[2], *pd[2];
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            int sx = 0, sd = 0;
-            if (EV == 1 && r + g < a.rows) {
-                sx = (int)(reinterpret_cast<uintptr_t>(x + (r + g) * a.ldx) & 15);
-                sd = (int)(reinterpret_cast<uintptr_t>(dy + (r + g) * a.lddy) & 15);
-            }
-            px[g] = buf + (size_t)g * a.buf + sx;
-            pd[g] = buf + (size_t)(2 + g) * a.buf + sd;
-        }
+        const uint32_t at_buf = smem_u32(buf);
+        const int two = r + 1 < a.rows ? 2 : 1;
+        int shift[4] = {0, 0, 0, 0};
         if constexpr (EV == 1) {
             bool lacks = false;
-            for (int g = 0; g < 2; ++g) {
-                if (r + g >= a.rows) continue;
+            for (int g = 0; g < two; ++g) {
+                shift[g] = shift_of(x, a.ldx, r + g);
+                shift[2 + g] = shift_of(dy, a.lddy, r + g);
                 if (row_lacks(x, a.ldx, a.rows, a.D, r + g)) {
                     patch_row(buf + (size_t)g * a.buf, x, a.ldx, a.rows, a.D, r + g, at, lanes);
                     lacks = true;
@@ -524,20 +586,21 @@ __global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
                     lacks = true;
                 }
             }
-            if (lacks) __syncthreads();
+            if (lacks) team_sync(team, warps);
         }
         float2 s[2], d[2];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             s[g] = d[g] = make_float2(0.f, 0.f);
-            if (r + g >= a.rows) continue;
+            if (g >= two) continue;
             const float mu = __shfl_sync(0xffffffffu, now, g), is = __shfl_sync(0xffffffffu, now, 2 + g);
-            Team<T, EV, NV> vx, vd;                        // dy of zero beyond the row: nothing is added
-            vx.read(px[g], at, lanes, packs);
-            vd.read(pd[g], at, lanes, packs);
+            const float2 is2 = make_float2(is, is), off = make_float2(-mu, -mu);
+            Team<T, EV, NV> vx, vd;
+            vx.read(at_buf + g * a.buf + shift[g], place);
+            vd.read(at_buf + (2 + g) * a.buf + shift[2 + g], place);
 #pragma unroll
             for (int i = 0; i < VALUES; ++i) {
-                const float2 xh = mul2(add2(vx.get(i), make_float2(-mu, -mu)), make_float2(is, is)), g0 = vd.get(i), gw = mul2(g0, kw[i]);
+                const float2 xh = mul2(add2(vx.get(i), off), is2), g0 = vd.get(i), gw = mul2(g0, kw[i]);
                 dw[i] = fma2(g0, xh, dw[i]);
                 db[i] = add2(db[i], g0);
                 s[g] = add2(s[g], gw);
@@ -547,7 +610,7 @@ __global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
         const float t4 = warp_sum4(s[0].x + s[0].y, d[0].x + d[0].y, s[1].x + s[1].y, d[1].x + d[1].y, lane);
         float* set = sums + turn * warps * 4;
         if ((lane & 7) == 0) set[warp * 4 + (lane >> 3)] = t4;
-        __syncthreads();
+        team_sync(team, warps);
         // lane l adds value l % 4 of warps l / 4, l / 4 + 8, ..
         float total = 0.f;
         for (int k = lane >> 2; k < warps; k += 8) total += set[k * 4 + (lane & 3)];
@@ -555,22 +618,26 @@ __global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
         total += __shfl_xor_sync(0xffffffffu, total, 8);
         total += __shfl_xor_sync(0xffffffffu, total, 16);
         total *= -a.inv_d;
+        if (!there) {                                      // a copy that never came: no number comes out
+            total = __int_as_float(0x7fc00000);
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) dw[i] = db[i] = make_float2(total, total);
+        }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            if (r + g >= a.rows) continue;
             const float mu = __shfl_sync(0xffffffffu, now, g), is = __shfl_sync(0xffffffffu, now, 2 + g);
-            float ms = __shfl_sync(0xffffffffu, total, 2 * g), md = __shfl_sync(0xffffffffu, total, 2 * g + 1);
-            if (!a.dx) continue;
-            if (!there) ms = __int_as_float(0x7fc00000);
+            const float ms = __shfl_sync(0xffffffffu, total, 2 * g), md = __shfl_sync(0xffffffffu, total, 2 * g + 1);
+            if (g >= two || !a.dx) continue;
+            const float2 is2 = make_float2(is, is), off = make_float2(-mu, -mu), ms2 = make_float2(ms, ms), md2 = make_float2(md, md);
             Team<T, EV, NV> vx, vd;
-            vx.read(px[g], at, lanes, packs);
-            vd.read(pd[g], at, lanes, packs);
+            vx.read(at_buf + g * a.buf + shift[g], place);
+            vd.read(at_buf + (2 + g) * a.buf + shift[2 + g], place);
             T* dx = static_cast<T*>(a.dx) + (r + g) * a.D;
             float2 o[VALUES];
 #pragma unroll
             for (int i = 0; i < VALUES; ++i) {
-                const float2 xh = mul2(add2(vx.get(i), make_float2(-mu, -mu)), make_float2(is, is));
-                o[i] = mul2(make_float2(is, is), fma2(xh, make_float2(md, md), fma2(vd.get(i), kw[i], make_float2(ms, ms))));
+                const float2 xh = mul2(add2(vx.get(i), off), is2);
+                o[i] = mul2(is2, fma2(xh, md2, fma2(vd.get(i), kw[i], ms2)));
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -585,11 +652,7 @@ __global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
                 }
             }
         }
-        if (!there) {
-#pragma unroll
-            for (int i = 0; i < VALUES; ++i) dw[i] = db[i] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
-        }
-        __syncthreads();                                   // every thread has read the stage
+        team_sync(team, warps);                            // the whole team has read the stage
         if (r + a.stages * step < a.rows) fetch(r + a.stages * step, stage);
         if (++stage == a.stages) {
             stage = 0;
@@ -598,17 +661,33 @@ __global__ void __launch_bounds__(512) ln_bwd_rows2(const LnBwdArgs a) {
         now = next;
     }
     if (!a.part) return;
-    float* part = a.part + 2LL * blockIdx.x * a.D;
+    // every copy has been waited for, so the buffers are free: [team][2][D]
+    __syncthreads();
+    float* all = reinterpret_cast<float*>(smem);
+    auto put = [&](float* to) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if (at + k * lanes < packs) {
+        for (int k = 0; k < NV; ++k)
+            if (at + k * lanes < packs) {
 #pragma unroll
-            for (int j = 0; j < EV; ++j) {
-                const int c = (at + k * lanes) * EV + j, i = (k * EV + j) / 2;
-                part[c] = (k * EV + j) & 1 ? dw[i].y : dw[i].x;
-                part[a.D + c] = (k * EV + j) & 1 ? db[i].y : db[i].x;
+                for (int j = 0; j < EV; ++j) {
+                    const int c = (at + k * lanes) * EV + j, i = (k * EV + j) / 2;
+                    to[c] = (k * EV + j) & 1 ? dw[i].y : dw[i].x;
+                    to[a.D + c] = (k * EV + j) & 1 ? db[i].y : db[i].x;
+                }
             }
-        }
+    };
+    float* part = a.part + 2LL * blockIdx.x * a.D;
+    if (teams == 1) {
+        put(part);
+        return;
+    }
+    put(all + 2LL * team * a.D);
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * a.D; c += blockDim.x) {
+        float t = all[c];
+        for (int k = 1; k < teams; ++k) t += all[2LL * k * a.D + c];
+        part[c] = t;
+    }
 }
 
 // ---- long rows: one block per row, the row read again from L2 for each step ---------------------
@@ -749,7 +828,7 @@ int ln_fwd_rows_launch(LnFwdArgs a, int team, int sms, cudaStream_t s) {
     if (per_sm < teams) teams = (int)per_sm;
     a.team = team;
     a.buf = (int)((a.D * sizeof(T) + 15) / 16 * 16 + (EV == 1 ? 16 : 0));
-    a.wbytes = (int)((a.D * sizeof(W) + 15) / 16 * 16);
+    a.wbytes = (a.D * 4 + 15) / 16 * 16;
     while (teams > 1 && 2 * (size_t)a.wbytes + (size_t)teams * a.buf > kRowSmem) --teams;
     const size_t room = (kRowSmem - 2 * (size_t)a.wbytes) / ((size_t)teams * a.buf);
     a.stages = (int)(room > 4 ? 4 : room);
@@ -771,18 +850,24 @@ int ln_bwd_short_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
     return launch_kernel(kern, a.slices, 256, smem, s, false, a);
 }
 
+// Teams of as many warps as the row's columns need, 16 columns to a thread: up to 16 warps and as many teams to a block as
+// fit with two stages each (one team with one stage for the longest rows).
 template <class T, class W, int EV, int NV>
 int ln_bwd_rows_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
-    auto kern = ln_bwd_rows2<T, W, EV, NV>;
-    const int block = (int)((a.D / EV + 32 * NV - 1) / (32 * NV) * 32);
+    auto kern = ln_bwd_rows<T, W, EV, NV>;
+    a.lanes = (int)((a.D / EV + 32 * NV - 1) / (32 * NV) * 32);
     a.buf = (int)((a.D * sizeof(T) + 15) / 16 * 16 + (EV == 1 ? 16 : 0));
     a.stages = 8 * (size_t)a.buf <= kRowSmem ? 2 : 1;
-    const size_t smem = (size_t)a.stages * 4 * a.buf + (a.stages + 1) * 8 + 2 * (size_t)(block / 32) * 16;
-    const long long want = (a.rows + 1) / 2;
-    long long most = (long long)sms * resident_blocks((const void*)kern, block, smem);
+    const long long pairs = (a.rows + 1) / 2;
+    int teams = 512 / a.lanes;
+    while (teams > 1 && ((size_t)teams * a.stages * 4 * a.buf > kRowSmem || (long long)(teams - 1) * sms >= pairs)) --teams;
+    // a team's dw and db, 8 D bytes, fit its buffers: 16 D with two stages of 16-bit rows
+    const size_t smem = (size_t)teams * (a.stages * 4 * (size_t)a.buf + 16 + (size_t)(a.lanes / 32) * 32);
+    const long long want = (pairs + teams - 1) / teams;
+    long long most = (long long)sms * resident_blocks((const void*)kern, teams * a.lanes, smem);
     most = most < kMaxParts ? most : kMaxParts;
     a.slices = (int)(want < most ? want : most);
-    return launch_kernel(kern, a.slices, block, smem, s, false, a);
+    return launch_kernel(kern, a.slices, teams * a.lanes, smem, s, false, a);
 }
 
 bool ln_shape_ok(int64_t rows, int D, int64_t ld) { return rows >= 0 && D > 0 && (rows <= 1 || ld >= D); }
@@ -822,10 +907,9 @@ int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype,
         // rows that fit shared memory beside their weights.  Few rows are spread over more warps each.
         const bool few = rows < 4LL * f.sms;
         auto team = [&](int nv) { return (int)((packs + 32LL * nv - 1) / (32LL * nv)); };
-        if (2 * D * ws + D * es + 64 <= kRowSmem) {
+        if (8 * (size_t)D + D * es + 64 <= kRowSmem) {
             if (wide && packs <= 32 * 4 * 16 && (few || packs <= 32 * 4)) return ln_fwd_rows_launch<T, W, EV, 4>(a, team(4), f.sms, s);
-            if (wide && packs <= 32 * 8) return ln_fwd_rows_launch<T, W, EV, 8>(a, team(8), f.sms, s);
-            if (wide && packs <= 32 * 16 * 16) return ln_fwd_rows_launch<T, W, EV, 16>(a, team(16), f.sms, s);
+            if (wide && packs <= 32 * 8 * 16) return ln_fwd_rows_launch<T, W, EV, 8>(a, team(8), f.sms, s);
             if (!wide && packs <= 32 * 8 * 16 && (few || packs <= 32 * 8)) return ln_fwd_rows_launch<T, W, 1, 8>(a, team(8), f.sms, s);
             if (!wide && packs <= 32 * 32 * 16) return ln_fwd_rows_launch<T, W, 1, 32>(a, team(32), f.sms, s);
         }
@@ -875,7 +959,7 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
                       : packs <= 32 ? ln_bwd_short_launch<T, W, 1, 1>(a, f.sms, s) : ln_bwd_short_launch<T, W, 1, 2>(a, f.sms, s);
         } else if (rows > 0 && D <= 16 * 512) {
             rc = wide ? ln_bwd_rows_launch<T, W, EV, NV>(a, f.sms, s)
-                 : D <= 8 * 256 ? ln_bwd_rows_launch<T, W, 1, 8>(a, f.sms, s) : ln_bwd_rows_launch<T, W, 1, 16>(a, f.sms, s);
+                 : D <= 8 * 512 ? ln_bwd_rows_launch<T, W, 1, 8>(a, f.sms, s) : ln_bwd_rows_launch<T, W, 1, 16>(a, f.sms, s);
         } else {
             if (grad_in && rows > 0) {
                 const int grid = (int)(rows < f.sms * 4LL ? rows : f.sms * 4LL);
