@@ -5,11 +5,23 @@
 //
 // An id outside [0, rows) gives a row of zeros and no gradient; a padding id gives no gradient.
 //
-// The tokens are sorted by id with a stable radix sort (digits of up to 9 bits, at most 4 passes), so that the order
-// of every sum, and with it every bit of the result, is fixed.  The sorted list is cut into chunks of kChunk tokens;
-// each chunk is summed by one thread per group of columns, whatever ids it holds, so a frequent token costs no more than
-// rare ones.  A token's run inside one chunk goes straight to the table; the parts of a run that crosses
-// chunks go to the workspace and are added in order.
+// Memory-bound: the forward pass reads each row it needs and writes it; the backward pass reads grad_out once and
+// writes every row of grad_table once.  The tokens are sorted by id with a stable radix sort (digits of up to 9 bits, at
+// most 4 passes), so that the order of every sum, and with it every bit of the result, is fixed.  The sorted list is cut
+// into chunks of kChunk tokens; each chunk is summed by one thread per group of columns, whatever ids it holds, so a frequent
+// token costs no more than rare ones.  A token's run inside one chunk goes straight to the table; the parts of a run that
+// crosses chunks go to the workspace, and a last kernel adds them in order.
+//
+// The kernels of a call, each the programmatic dependent of the one before (its launch overlaps the other's end):
+//   up to 8192 tokens and 262144 rows
+//     sort_small  one block: all passes in shared memory, and the bitmap of the rows that are met
+//   otherwise
+//     clear       the bitmap and the counters
+//     count       digit counts of each tile of tokens for the first pass; marks the rows that are met
+//     scatter     one per pass: places the tile's tokens and counts the next pass's digits.  A few blocks sort; the others
+//                 meanwhile write the table's rows that are not met, batch by batch until the sorting is done
+//   sum           chunks, and the other rows that are not met
+//   join          runs that cross chunks
 #include "launch.cuh"
 #include "lm_common.cuh"
 
@@ -21,52 +33,116 @@ constexpr int kChunk = 32;
 constexpr int kTile = 2048;          // tokens a block ranks at a time
 constexpr int kMaxTiles = 128;
 constexpr int kMaxBins = 512;
+constexpr int kMaxPasses = 4;
+constexpr int kSortThreads = 512;
+constexpr int kSmallTokens = 8192;   // one block's
+constexpr long long kSmallRows = 262144;
+constexpr int kLongRun = 33;         // parts from which a block, not a warp, adds them up
+
+// counters in the workspace, zero before the first use
+struct Counters {
+    unsigned short_runs, long_runs;      // runs that cross chunks
+    unsigned zero_next;                  // batches of rows that sorting kernels have taken to write zeros into
+    unsigned sorted[kMaxPasses];         // tiles that are done
+};
+
+__device__ __forceinline__ void after_predecessor() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 struct EmbFwdArgs {
     const void *table, *ids;
     void* out;
-    long long n, rows, items;
-    int D, packs;
+    long long n, rows;
+    int D, packs, lanes;
     float scale;
-    FastDiv div;
 };
 
+// `lanes` threads to a token, kAhead accesses each, the block's second index over longer rows: all loads of a thread are
+// under way together
+constexpr int kAhead = 4;
 template <class T, int EV, class I>
 __global__ void __launch_bounds__(256) emb_fwd(const EmbFwdArgs a) {
-    const T* table = static_cast<const T*>(a.table);
-    T* out = static_cast<T*>(a.out);
-    for (long long it = (long long)blockIdx.x * blockDim.x + threadIdx.x; it < a.items; it += (long long)gridDim.x * blockDim.x) {
-        const long long i = it / a.packs;
-        const int p = (int)(it - i * a.packs);
-        const long long v = static_cast<const I*>(a.ids)[i];
-        Pack<T, EV> r;
-        if (v >= 0 && v < a.rows) {
-            const Pack<T, EV> q = load_cached<T, EV>(table + v * a.D + p * EV);
+    const int lanes = a.lanes, at = threadIdx.x & (lanes - 1);
+    const long long i = (long long)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    if (i >= a.n) return;
+    const long long v = __ldg(static_cast<const I*>(a.ids) + i);
+    const bool in = v >= 0 && v < a.rows;
+    const T* row = static_cast<const T*>(a.table) + (in ? v : 0) * a.D;
+    T* out = static_cast<T*>(a.out) + i * a.D;
+    for (int p0 = blockIdx.y * lanes * kAhead + at; p0 < a.packs; p0 += gridDim.y * lanes * kAhead) {
+        Pack<T, EV> q[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            q[k] = {};
+            if (in && p0 + k * lanes < a.packs) q[k] = load_cached<T, EV>(row + (p0 + k * lanes) * (long long)EV);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (p0 + k * lanes >= a.packs) continue;
             float2 f[(EV + 1) / 2];
 #pragma unroll
-            for (int k = 0; k < (EV + 1) / 2; ++k) f[k] = mul2(pair_of(q, k), make_float2(a.scale, a.scale));
-            r = pack_pairs<T, EV>(f);
-        } else {
-            r = {};
+            for (int j = 0; j < (EV + 1) / 2; ++j) f[j] = in ? mul2(pair_of(q[k], j), make_float2(a.scale, a.scale)) : make_float2(0.f, 0.f);
+            store_stream<T, EV>(out + (p0 + k * lanes) * (long long)EV, pack_pairs<T, EV>(f));
         }
-        store_stream<T, EV>(out + i * a.D + p * EV, r);
+    }
+}
+
+// ---- rows of the table that no token meets ---------------------------------------------------------------
+struct ZeroArgs {
+    unsigned char* grad;
+    const unsigned* met;         // a bit for each row
+    long long row_bytes, rows, batches;
+    int per_warp;                // rows of a warp, a power of two up to 32
+};
+// the batch's rows, 8 * per_warp of them (or 16 warps' in a block of 512 threads)
+__device__ __forceinline__ void zero_batch(const ZeroArgs& z, long long batch) {
+    const int lane = threadIdx.x & 31;
+    const long long r0 = (batch * 8 + (threadIdx.x >> 5)) * z.per_warp;
+    if (r0 >= z.rows) return;
+    unsigned todo = ~(z.met[r0 >> 5] >> (r0 & 31));
+    const int here = (int)min((long long)z.per_warp, z.rows - r0);
+    if (here < 32) todo &= (1u << here) - 1;
+    while (todo) {
+        // neighbouring rows are written as one stretch
+        const int k = __ffs(todo) - 1, run = __ffs(~(todo >> k)) - 1;
+        const int count = run < 0 ? 32 - k : run;
+        todo = k + count >= 32 ? 0 : todo & (~0u << (k + count));
+        unsigned char* p = z.grad + (r0 + k) * z.row_bytes;
+        unsigned char* const end = p + count * z.row_bytes;
+        unsigned char* const a0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p) + 15) & ~(uintptr_t)15);
+        unsigned char* const a1 = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(end) & ~(uintptr_t)15);
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (a0 >= a1) {
+            for (unsigned char* q = p + 2 * lane; q < end; q += 64) *reinterpret_cast<unsigned short*>(q) = 0;
+        } else {
+            if (p + 2 * lane < a0) *reinterpret_cast<unsigned short*>(p + 2 * lane) = 0;
+            for (unsigned char* q = a0 + 16 * lane; q < a1; q += 512) stg_stream4(reinterpret_cast<float*>(q), zero);
+            if (a1 + 2 * lane < end) *reinterpret_cast<unsigned short*>(a1 + 2 * lane) = 0;
+        }
     }
 }
 
 // ---- sort ------------------------------------------------------------------------------------------
 struct SortArgs {
-    const void* ids;            // first pass only
+    const void* ids;            // first pass and small sort
     const unsigned *key, *pos;  // later passes
     unsigned *key_out, *pos_out;
-    unsigned* count;            // [tiles][bins] of this pass
+    unsigned *count, *next;     // [tiles][bins] of this pass and of the next one (or null)
+    unsigned* met;
+    Counters* counters;
+    unsigned* clear;            // clear kernel: 4-byte words
+    long long clear_words;
     long long rows, padding;
-    int n, tile, tiles, shift, bits;
+    int n, tile, tiles, shift, bits, pass, passes;
+    ZeroArgs zero;
 };
 
 // ids that get no gradient become the key `rows`, which sorts behind all others
 template <class I>
 __device__ __forceinline__ unsigned token_key(const SortArgs& a, int i) {
-    const long long v = static_cast<const I*>(a.ids)[i];
+    const long long v = __ldg(static_cast<const I*>(a.ids) + i);
     return v < 0 || v >= a.rows || v == a.padding ? (unsigned)a.rows : (unsigned)v;
 }
 struct NoIds {};
@@ -76,53 +152,101 @@ __device__ __forceinline__ unsigned sort_key(const SortArgs& a, int i) {
     else return a.key[i];
 }
 
-template <class I>
-__global__ void __launch_bounds__(256) emb_sort_count(const SortArgs a) {
-    __shared__ unsigned bin[kMaxBins];
-    const int bins = 1 << a.bits;
-    for (int d = threadIdx.x; d < bins; d += 256) bin[d] = 0;
-    __syncthreads();
-    const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile);
-    for (int i = i0 + threadIdx.x; i < i1; i += 256) atomicAdd(&bin[(sort_key<I>(a, i) >> a.shift) & (bins - 1)], 1u);
-    __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += 256) a.count[(size_t)blockIdx.x * bins + d] = bin[d];
+__global__ void __launch_bounds__(256) emb_clear(const SortArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.clear_words; i += (long long)gridDim.x * 256) a.clear[i] = 0;
 }
 
 template <class I>
-__global__ void __launch_bounds__(256) emb_sort_scatter(const SortArgs a) {
-    constexpr int WARPS = 8, ROUNDS = kTile / 256;
-    __shared__ unsigned base[kMaxBins];               // where the tile's next key with this digit goes
-    __shared__ unsigned cnt[WARPS][kMaxBins];         // a warp's keys with this digit
-    __shared__ unsigned wsum[WARPS];
-    const int bins = 1 << a.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // keys with a smaller digit, and those with the same digit in earlier tiles: two neighbouring digits per thread
-    unsigned total[2] = {0, 0}, before[2] = {0, 0};
-    for (int k = 0; k < 2; ++k) {
-        const int d = 2 * threadIdx.x + k;
-        if (d < bins)
-            for (int t = 0; t < a.tiles; ++t) {
-                const unsigned c = a.count[(size_t)t * bins + d];
-                total[k] += c;
-                before[k] += t < (int)blockIdx.x ? c : 0;
-            }
+__global__ void __launch_bounds__(kSortThreads) emb_sort_count(const SortArgs a) {
+    __shared__ unsigned bin[kMaxBins];
+    const int bins = 1 << a.bits;
+    for (int d = threadIdx.x; d < bins; d += kSortThreads) bin[d] = 0;
+    __syncthreads();
+    after_predecessor();
+    const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile);
+#pragma unroll 4
+    for (int i = i0 + threadIdx.x; i < i1; i += kSortThreads) {
+        const unsigned k = token_key<I>(a, i);
+        atomicAdd(&bin[k & (bins - 1)], 1u);
+        if (k < (unsigned)a.rows && !(a.met[k >> 5] >> (k & 31) & 1u)) atomicOr(a.met + (k >> 5), 1u << (k & 31));
     }
-    unsigned s = total[0] + total[1], incl = s;
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kSortThreads) a.count[(size_t)blockIdx.x * bins + d] = bin[d];
+}
+
+// ranks of a warp's keys among those with the same digit, 32 keys at a time in their order; cnt: the warp's counts so far
+template <class C>
+__device__ __forceinline__ unsigned rank_digit(C* cnt, unsigned d, bool in, int lane) {
+    const unsigned same = __match_any_sync(0xffffffffu, in ? d : 0xffffffffu);
+    const unsigned rank = in ? cnt[d] + __popc(same & ((1u << lane) - 1)) : 0u;
+    __syncwarp();
+    if (in && (same >> lane) == 1u) cnt[d] += (C)__popc(same);         // the highest lane of each digit
+    __syncwarp();
+    return rank;
+}
+
+template <class I>
+__global__ void __launch_bounds__(kSortThreads) emb_sort_scatter(const SortArgs a) {
+    constexpr int WARPS = kSortThreads / 32, ROUNDS = kTile / kSortThreads;
+    __shared__ unsigned base[kMaxBins];               // where the tile's next key with this digit goes
+    __shared__ unsigned sums[2][2][kMaxBins];         // two halves of the tiles: all keys with a digit, and those before this tile
+    __shared__ unsigned short cnt[WARPS][kMaxBins];   // a warp's keys with this digit
+    __shared__ unsigned wsum[WARPS];
+    __shared__ unsigned batch;
+    after_predecessor();
+    if ((int)blockIdx.x >= a.tiles) {
+        // nothing waits here: batches are taken until there are none, or the tiles are done
+        for (;;) {
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const unsigned done = *reinterpret_cast<volatile unsigned*>(&a.counters->sorted[a.pass]);
+                batch = done == (unsigned)a.tiles ? 0xffffffffu : atomicAdd(&a.counters->zero_next, 2u);
+            }
+            __syncthreads();
+            if (batch >= a.zero.batches) return;
+            zero_batch(a.zero, batch);
+        }
+    }
+    const int bins = 1 << a.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // keys with a smaller digit, and those with the same digit in earlier tiles: two neighbouring digits and every
+    // second tile to a thread
+    {
+        const int pair = threadIdx.x & 255, half = threadIdx.x >> 8;
+        unsigned total[2] = {0, 0}, before[2] = {0, 0};
+        if (2 * pair < bins) {
+#pragma unroll 16
+            for (int t = half; t < a.tiles; t += 2) {
+                const uint2 c = *reinterpret_cast<const uint2*>(a.count + (size_t)t * bins + 2 * pair);
+                total[0] += c.x;
+                total[1] += c.y;
+                before[0] += t < (int)blockIdx.x ? c.x : 0;
+                before[1] += t < (int)blockIdx.x ? c.y : 0;
+            }
+        }
+        sums[half][0][2 * pair] = total[0];
+        sums[half][0][2 * pair + 1] = total[1];
+        sums[half][1][2 * pair] = before[0];
+        sums[half][1][2 * pair + 1] = before[1];
+    }
+    __syncthreads();
+    const int d0 = threadIdx.x;                       // one digit to a thread
+    const unsigned mine = sums[0][0][d0] + sums[1][0][d0];
+    unsigned incl = mine;
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned u = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += u;
     }
     if (lane == 31) wsum[warp] = incl;
     __syncthreads();
-    unsigned off = incl - s;
+    unsigned off = incl - mine;
     for (int w = 0; w < warp; ++w) off += wsum[w];
-    if (2 * threadIdx.x < bins) base[2 * threadIdx.x] = off + before[0];
-    if (2 * threadIdx.x + 1 < bins) base[2 * threadIdx.x + 1] = off + total[0] + before[1];
+    base[d0] = off + sums[0][1][d0] + sums[1][1][d0];
 
     const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile);
     for (int at = i0; at < i1; at += kTile) {
         for (int d = lane; d < bins; d += 32) cnt[warp][d] = 0;
-        __syncwarp();
-        // each warp ranks its own stretch, 32 keys at a time
+        // each warp ranks its own stretch
         unsigned key[ROUNDS], rank[ROUNDS];
         int pos[ROUNDS];
 #pragma unroll
@@ -132,35 +256,123 @@ __global__ void __launch_bounds__(256) emb_sort_scatter(const SortArgs a) {
             key[r] = in ? sort_key<I>(a, i) : 0u;
             if constexpr (sizeof(I) >= 4) pos[r] = i;
             else pos[r] = in ? (int)a.pos[i] : 0;
-            const unsigned d = (key[r] >> a.shift) & (bins - 1);
-            const unsigned same = __match_any_sync(0xffffffffu, in ? d : 0xffffffffu);
-            rank[r] = in ? cnt[warp][d] + __popc(same & ((1u << lane) - 1)) : 0u;
-            __syncwarp();
-            if (in && (same >> lane) == 1u) cnt[warp][d] += __popc(same);      // the highest lane of each digit
-            __syncwarp();
         }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            rank[r] = rank_digit(cnt[warp], (key[r] >> a.shift) & (bins - 1), at + warp * (32 * ROUNDS) + r * 32 + lane < i1, lane);
         __syncthreads();
-        for (int d = threadIdx.x; d < bins; d += 256) {     // each warp's first place for each digit
-            unsigned b = base[d];
+        if (d0 < bins) {                               // each warp's first place for each digit, relative to the tile's
+            unsigned b = 0;
+#pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const unsigned c = cnt[w][d];
-                cnt[w][d] = b;
+                const unsigned c = cnt[w][d0];
+                cnt[w][d0] = (unsigned short)b;
                 b += c;
             }
-            base[d] = b;
+            sums[0][0][d0] = base[d0];
+            base[d0] += b;
         }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
             const int i = at + warp * (32 * ROUNDS) + r * 32 + lane;
             if (i < i1) {
-                const unsigned to = cnt[warp][(key[r] >> a.shift) & (bins - 1)] + rank[r];
+                const unsigned d = (key[r] >> a.shift) & (bins - 1), to = sums[0][0][d] + cnt[warp][d] + rank[r];
                 a.key_out[to] = key[r];
                 a.pos_out[to] = (unsigned)pos[r];
+                if (a.next) atomicAdd(&a.next[(size_t)(to / (unsigned)a.tile) * bins + ((key[r] >> (a.shift + a.bits)) & (bins - 1))], 1u);
             }
         }
         __syncthreads();
     }
+    if (threadIdx.x == 0) atomicAdd(&a.counters->sorted[a.pass], 1u);
+}
+
+// All passes of up to 8192 tokens in one block: [bitmap of the rows][keys][positions][warps' counts], the keys in registers
+// while they are ranked.
+template <class I>
+__global__ void __launch_bounds__(1024) emb_sort_small(const SortArgs a) {
+    constexpr int WARPS = 32, ROUNDS = kSmallTokens / 1024;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ unsigned wsum[WARPS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int words = (int)((a.rows + 31) / 32), bins = 1 << a.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned* met = reinterpret_cast<unsigned*>(smem);
+    unsigned* keys = met + words;
+    unsigned* base = keys + kSmallTokens;
+    unsigned short* poss = reinterpret_cast<unsigned short*>(base + kMaxBins);
+    unsigned short* cnt = poss + kSmallTokens;                 // [WARPS][kMaxBins]
+    const int rounds = (a.n + 1023) / 1024;                    // of 32 keys of each warp
+    for (int i = threadIdx.x; i < words; i += 1024) met[i] = 0;
+    unsigned key[ROUNDS], rank[ROUNDS];
+    unsigned short pos[ROUNDS];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int i = (warp * rounds + r) * 32 + lane;
+        key[r] = 0;
+        pos[r] = (unsigned short)i;
+        if (r < rounds && i < a.n) {
+            key[r] = token_key<I>(a, i);
+            if (key[r] < (unsigned)a.rows) atomicOr(met + (key[r] >> 5), 1u << (key[r] & 31));
+        }
+    }
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const int shift = pass * a.bits;
+        for (int d = threadIdx.x; d < WARPS * kMaxBins / 2; d += 1024) reinterpret_cast<unsigned*>(cnt)[d] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (r < rounds) rank[r] = rank_digit(cnt + warp * kMaxBins, (key[r] >> shift) & (bins - 1), (warp * rounds + r) * 32 + lane < a.n, lane);
+        __syncthreads();
+        unsigned total = 0;
+        if ((int)threadIdx.x < bins) {
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const unsigned c = cnt[w * kMaxBins + threadIdx.x];
+                cnt[w * kMaxBins + threadIdx.x] = (unsigned short)total;
+                total += c;
+            }
+        }
+        unsigned incl = total;
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        if (lane == 31) wsum[warp] = incl;
+        __syncthreads();
+        unsigned off = incl - total;
+        for (int w = 0; w < warp; ++w) off += wsum[w];
+        if ((int)threadIdx.x < bins) base[threadIdx.x] = off;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (r < rounds && (warp * rounds + r) * 32 + lane < a.n) {
+                const unsigned d = (key[r] >> shift) & (bins - 1), to = base[d] + cnt[warp * kMaxBins + d] + rank[r];
+                keys[to] = key[r];
+                poss[to] = pos[r];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const int i = (warp * rounds + r) * 32 + lane;
+            if (r < rounds && i < a.n) {
+                key[r] = keys[i];
+                pos[r] = poss[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int i = (warp * rounds + r) * 32 + lane;
+        if (r < rounds && i < a.n) {
+            a.key_out[i] = key[r];
+            a.pos_out[i] = pos[r];
+        }
+    }
+    for (int i = threadIdx.x; i < words; i += 1024) a.met[i] = met[i];
+    if (threadIdx.x == 0) a.counters->short_runs = a.counters->long_runs = a.counters->zero_next = 0;
 }
 
 // ---- sums ----------------------------------------------------------------------------------------------
@@ -169,85 +381,175 @@ struct EmbSumArgs {
     const unsigned *key, *pos;
     void* grad;
     float* part;                 // [chunks][2][D]: end of a run begun in an earlier chunk, begin of a run that goes on
+    unsigned* crossing;          // chunks in which a run begins that goes on, in any order: short runs from the front, long
+    Counters* counters;          // ones from the back
     long long items;
     unsigned rows;
     int n, D, packs, chunks;
     float scale;
+    ZeroArgs zero;
+    long long blocks;
 };
 
 template <class T, int EV>
-__device__ __forceinline__ void write_row(const EmbSumArgs& a, unsigned v, int p, const float2 (&acc)[(EV + 1) / 2]) {
+__device__ __forceinline__ void write_row(const EmbSumArgs& a, unsigned v, long long c, const float2 (&acc)[(EV + 1) / 2]) {
     float2 r[(EV + 1) / 2];
 #pragma unroll
     for (int k = 0; k < (EV + 1) / 2; ++k) r[k] = mul2(acc[k], make_float2(a.scale, a.scale));
-    store_stream<T, EV>(static_cast<T*>(a.grad) + (long long)v * a.D + p * EV, pack_pairs<T, EV>(r));
+    store_stream<T, EV>(static_cast<T*>(a.grad) + (long long)v * a.D + c, pack_pairs<T, EV>(r));
 }
 
 template <class T, int EV>
 __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
-    for (long long it = (long long)blockIdx.x * 256 + threadIdx.x; it < a.items; it += (long long)gridDim.x * 256) {
-        const int c = (int)(it / a.packs), p = (int)(it - (long long)c * a.packs);
-        const int s = c * kChunk, e = min(a.n, s + kChunk);
-        unsigned cur = a.key[s];
-        if (cur >= a.rows) continue;
-        bool begun = s > 0 && a.key[s - 1] == cur;          // the run began in an earlier chunk
-        float2 acc[(EV + 1) / 2];
-        auto clear = [&] {
+    constexpr int P = (EV + 1) / 2, U = 8;                // U rows of grad_out are under way together
+    after_predecessor();
+    // blocks that sum and blocks that write zeros take turns, so that reads and writes share the memory all the time
+    const long long total = a.blocks + a.zero.batches, z0 = blockIdx.x * a.zero.batches / total, z1 = (blockIdx.x + 1) * a.zero.batches / total;
+    if (z1 > z0) {
+        zero_batch(a.zero, z0 + a.counters->zero_next);         // the batches before were written beside the sort
+        return;
+    }
+    const long long it = (blockIdx.x - z0) * 256 + threadIdx.x;
+    if (it >= a.items) return;
+    const int c = (int)(it / a.packs), p = (int)(it - (long long)c * a.packs) * EV;
+    const int s = c * kChunk, e = min(a.n, s + kChunk);
+    unsigned cur = a.key[s];
+    if (cur >= a.rows) return;
+    bool begun = s > 0 && a.key[s - 1] == cur;            // the run began in an earlier chunk
+    const unsigned after = e < a.n ? a.key[e] : a.rows;
+    float2 acc[P];
 #pragma unroll
-            for (int k = 0; k < (EV + 1) / 2; ++k) acc[k] = make_float2(0.f, 0.f);
-        };
-        auto keep = [&](float* to) {
+    for (int k = 0; k < P; ++k) acc[k] = make_float2(0.f, 0.f);
+    auto keep = [&](float* to) {
 #pragma unroll
-            for (int k = 0; k < EV; ++k) to[k] = k & 1 ? acc[k / 2].y : acc[k / 2].x;
-        };
-        clear();
-        float* part = a.part + 2LL * c * a.D + p * EV;
-        for (int i = s; i < e; ++i) {
-            const unsigned v = a.key[i];
-            if (v != cur) {
+        for (int k = 0; k < EV; ++k) to[k] = k & 1 ? acc[k / 2].y : acc[k / 2].x;
+    };
+    float* part = a.part + 2LL * c * a.D + p;
+    for (int i = s; i < e; i += U) {
+        unsigned key[U], pos[U];
+#pragma unroll
+        for (int j = 0; j < U; j += 4) {                  // the lists are padded to whole chunks
+            const uint4 k4 = *reinterpret_cast<const uint4*>(a.key + i + j), p4 = *reinterpret_cast<const uint4*>(a.pos + i + j);
+            key[j] = k4.x; key[j + 1] = k4.y; key[j + 2] = k4.z; key[j + 3] = k4.w;
+            pos[j] = p4.x; pos[j + 1] = p4.y; pos[j + 2] = p4.z; pos[j + 3] = p4.w;
+        }
+        Pack<T, EV> g[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (i + j >= e) key[j] = a.rows;
+            if (key[j] < a.rows) g[j] = load_stream<T, EV>(static_cast<const T*>(a.dy) + (long long)pos[j] * a.D + p);
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (i + j >= e) break;
+            if (key[j] != cur) {
                 if (begun) keep(part);
                 else write_row<T, EV>(a, cur, p, acc);
-                cur = v;
                 begun = false;
-                if (v >= a.rows) break;
-                clear();
-            }
-            const Pack<T, EV> g = load_stream<T, EV>(static_cast<const T*>(a.dy) + (long long)a.pos[i] * a.D + p * EV);
+                cur = key[j];
+                if (cur >= a.rows) return;                // only such keys follow
 #pragma unroll
-            for (int k = 0; k < (EV + 1) / 2; ++k) acc[k] = add2(acc[k], pair_of(g, k));
+                for (int k = 0; k < P; ++k) acc[k] = make_float2(0.f, 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < P; ++k) acc[k] = add2(acc[k], pair_of(g[j], k));
         }
-        if (cur >= a.rows) continue;
-        if (begun) keep(part);
-        else if (e < a.n && a.key[e] == cur) keep(part + a.D);
-        else write_row<T, EV>(a, cur, p, acc);
+    }
+    if (begun) {
+        keep(part);
+    } else if (after == cur) {
+        keep(part + a.D);
+        if (p == 0) {
+            const bool is_long = c + kLongRun < a.chunks && a.key[(long long)(c + kLongRun) * kChunk] == cur;
+            const unsigned k = atomicAdd(is_long ? &a.counters->long_runs : &a.counters->short_runs, 1u);
+            a.crossing[is_long ? a.chunks - 1 - k : k] = (unsigned)c;
+        }
+    } else {
+        write_row<T, EV>(a, cur, p, acc);
     }
 }
 
-// runs that cross chunks: the thread of the chunk in which the run begins adds its parts in order
-template <class T>
-__global__ void __launch_bounds__(256) emb_join(const EmbSumArgs a) {
-    for (long long it = (long long)blockIdx.x * 256 + threadIdx.x; it < (long long)a.chunks * a.D; it += (long long)gridDim.x * 256) {
-        const int c = (int)(it / a.D), p = (int)(it - (long long)c * a.D);
-        const int s = c * kChunk, e = s + kChunk;
-        if (e >= a.n) continue;
-        const unsigned v = a.key[e];
-        if (v >= a.rows || a.key[e - 1] != v) continue;                          // nothing crosses this chunk's end
-        if (s > 0 && a.key[s] == v && a.key[s - 1] == v) continue;               // the run began earlier
-        float2 acc[1] = {make_float2(a.part[(2LL * c + 1) * a.D + p], 0.f)};
-        for (int k = c + 1; k < a.chunks && a.key[k * kChunk] == v; ++k) acc[0].x += a.part[2LL * k * a.D + p];
-        write_row<T, 1>(a, v, p, acc);
+// Runs that cross chunks.  Up to kLongRun parts: a warp adds them for 32 accesses of COLS columns.  Longer ones: a block, 32
+// columns, kRuns stretches of the run's parts, the stretches' sums added in order.
+constexpr int kRuns = 16;
+template <class T, int COLS>
+__global__ void __launch_bounds__(32 * kRuns) emb_join(const EmbSumArgs a) {
+    __shared__ float sh[kRuns][32];
+    __shared__ int other;
+    after_predecessor();
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int wide_tiles = (a.D + 32 * COLS - 1) / (32 * COLS);
+    const long long work = (long long)a.counters->short_runs * wide_tiles;
+    for (long long i = (long long)blockIdx.x * kRuns + ty; i < work; i += (long long)gridDim.x * kRuns) {
+        const int c = (int)a.crossing[i / wide_tiles], col = ((int)(i % wide_tiles) * 32 + tx) * COLS;
+        const unsigned v = a.key[(long long)(c + 1) * kChunk - 1];
+        // the chunks that begin with the run's id follow each other
+        const bool same = c + 1 + tx < a.chunks && a.key[(long long)(c + 1 + tx) * kChunk] == v;
+        const unsigned more = __ballot_sync(0xffffffffu, same);
+        const int parts = 1 + (more == 0xffffffffu ? 32 : __ffs(~more) - 1);
+        if (col >= a.D) continue;
+        float2 acc[(COLS + 1) / 2];
+#pragma unroll
+        for (int j = 0; j < (COLS + 1) / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < parts; ++k) {
+            // written by the kernel before, which this one overlaps: no read-only load
+            const float* q = a.part + (2LL * (c + k) + (k == 0 ? 1 : 0)) * a.D + col;
+            if constexpr (COLS == 4) {
+                const float4 v4 = __ldcg(reinterpret_cast<const float4*>(q));
+                acc[0] = add2(acc[0], make_float2(v4.x, v4.y));
+                acc[1] = add2(acc[1], make_float2(v4.z, v4.w));
+            } else {
+                acc[0].x += __ldcg(q);
+            }
+        }
+        write_row<T, COLS>(a, v, col, acc);
+    }
+    const int tiles = (a.D + 31) / 32;
+    const long long long_work = (long long)a.counters->long_runs * tiles;
+    for (long long i = blockIdx.x; i < long_work; i += gridDim.x) {
+        const int c = (int)a.crossing[a.chunks - 1 - i / tiles], col = (int)(i % tiles) * 32 + tx;
+        const unsigned v = a.key[(long long)(c + 1) * kChunk - 1];
+        int end = c + kLongRun;                            // the first chunk that begins with another id, or none
+        for (bool found = false; !found; end += found ? 0 : 32 * kRuns) {
+            if (threadIdx.x == 0) other = 0x7fffffff;
+            __syncthreads();
+            const int k = end + (int)threadIdx.x;
+            if (k >= a.chunks || a.key[(long long)k * kChunk] != v) atomicMin(&other, min(k, a.chunks));
+            __syncthreads();
+            found = other != 0x7fffffff;
+            if (found) end = other;
+            __syncthreads();
+        }
+        const int parts = end - c, per = (parts + kRuns - 1) / kRuns, k0 = ty * per, k1 = min(parts, k0 + per);
+        float t = 0.f;
+        if (col < a.D) {
+#pragma unroll 8
+            for (int k = k0; k < k1; ++k) t += a.part[(2LL * (c + k) + (k == 0 ? 1 : 0)) * a.D + col];
+        }
+        sh[ty][tx] = t;
+        __syncthreads();
+        if (ty == 0 && col < a.D) {
+            const int runs = (parts + per - 1) / per;
+            for (int k = 1; k < runs; ++k) t += sh[k][tx];
+            const float2 acc[1] = {make_float2(t, 0.f)};
+            write_row<T, 1>(a, v, col, acc);
+        }
+        __syncthreads();
     }
 }
 
 struct EmbPlan {
     int tile, tiles, passes, bits, chunks;
-    size_t key[2], pos[2], count, part, bytes;
+    bool small;
+    size_t key[2], pos[2], count[kMaxPasses], crossing, counters, met, clear, clear_end, part, bytes;
 };
 EmbPlan emb_plan(long long n, long long rows, int D) {
     EmbPlan p{};
     const long long per = (n + (long long)kMaxTiles * kTile - 1) / ((long long)kMaxTiles * kTile);
     p.tile = (int)(kTile * (per < 1 ? 1 : per));
     p.tiles = (int)((n + p.tile - 1) / p.tile);
+    p.small = n <= kSmallTokens && rows <= kSmallRows;
     int bits = 0;
     while (bits < 32 && (rows >> bits) != 0) ++bits;          // keys are 0 .. rows
     p.passes = (bits + 8) / 9;
@@ -260,10 +562,16 @@ EmbPlan emb_plan(long long n, long long rows, int D) {
         return r;
     };
     for (int k = 0; k < 2; ++k) {
-        p.key[k] = take((size_t)n * 4);
-        p.pos[k] = take((size_t)n * 4);
+        p.key[k] = take((size_t)p.chunks * kChunk * 4);
+        p.pos[k] = take((size_t)p.chunks * kChunk * 4);
     }
-    p.count = take((size_t)p.tiles * kMaxBins * 4);
+    p.crossing = take((size_t)p.chunks * 4);
+    p.count[0] = take((size_t)p.tiles * kMaxBins * 4);
+    p.clear = at;                                              // what is cleared first: from here ..
+    for (int k = 1; k < p.passes; ++k) p.count[k] = take((size_t)p.tiles * kMaxBins * 4);
+    p.counters = take(sizeof(Counters));
+    p.met = take((size_t)((rows + 31) / 32) * 4);
+    p.clear_end = at;                                          // .. to here
     p.part = take((size_t)p.chunks * 2 * (size_t)D * 4);
     p.bytes = at;
     return p;
@@ -271,6 +579,12 @@ EmbPlan emb_plan(long long n, long long rows, int D) {
 
 constexpr long long kMaxTokens = (1LL << 31) - 1 - (long long)kMaxTiles * kTile;
 constexpr long long kMaxRows = (1LL << 31) - 1;
+
+// elements of an access: 16 bytes, or two 16-bit elements, or one
+int emb_access(int es, int D, const void* a, const void* b) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (uintptr_t)D * es;
+    return (all & 15) == 0 ? 16 / es : (all & 3) == 0 ? 4 / es : 1;
+}
 
 }  // namespace
 
@@ -289,20 +603,25 @@ int hfuse_embedding(const void* table, int64_t rows, int D, int dtype, const voi
     EmbFwdArgs a{};
     a.table = table; a.ids = ids; a.out = out;
     a.n = n; a.rows = rows; a.D = D; a.scale = scale;
-    const bool wide = aligned_to(table, 16) && aligned_to(out, 16) && D * es % 16 == 0;
+    const int ev = emb_access((int)es, D, table, out);
+    a.packs = D / ev;
+    a.lanes = 32;
+    while (a.lanes > 1 && a.lanes / 2 * kAhead >= a.packs) a.lanes /= 2;
+    const int per = 256 / a.lanes;
+    const long long stretches = ((long long)a.packs + a.lanes * kAhead - 1) / (a.lanes * kAhead);
+    const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)(stretches < 65535 ? stretches : 65535));
     return by_type(dtype, [&](auto t) {
         using T = typename decltype(t)::type;
-        constexpr int EV = 16 / sizeof(T);
-        a.packs = wide ? D / EV : D;
-        a.items = (long long)n * a.packs;
-        const long long want = (a.items + 255) / 256, most = f.sms * 8LL;
-        const int grid = (int)(want < most ? want : most);
+        constexpr int EV = 16 / sizeof(T), EV4 = 4 / sizeof(T);
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (wide)
-            return id_bytes == 8 ? launch_kernel(emb_fwd<T, EV, long long>, grid, 256, 0, s, false, a)
-                                 : launch_kernel(emb_fwd<T, EV, int>, grid, 256, 0, s, false, a);
-        return id_bytes == 8 ? launch_kernel(emb_fwd<T, 1, long long>, grid, 256, 0, s, false, a)
-                             : launch_kernel(emb_fwd<T, 1, int>, grid, 256, 0, s, false, a);
+        auto go = [&](auto id) {
+            using I = decltype(id);
+            if (ev == EV) emb_fwd<T, EV, I><<<grid, 256, 0, s>>>(a);
+            else if (ev == EV4) emb_fwd<T, EV4, I><<<grid, 256, 0, s>>>(a);
+            else emb_fwd<T, 1, I><<<grid, 256, 0, s>>>(a);
+            return check_launch();
+        };
+        return id_bytes == 8 ? go((long long)0) : go((int)0);
     });
 }
 
@@ -325,50 +644,74 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
     DeviceFacts f;
     if (int rc = device_facts(f)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cudaMemsetAsync(grad_table, 0, (size_t)rows * D * es, s) != cudaSuccess) {
+    if (n == 0) {
+        if (cudaMemsetAsync(grad_table, 0, (size_t)rows * D * es, s) == cudaSuccess) return HFUSE_OK;
         (void)cudaGetLastError();
         return HFUSE_ERR_LAUNCH;
     }
-    if (n == 0) return HFUSE_OK;
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     auto at = [&](size_t off) { return reinterpret_cast<unsigned*>(ws + off); };
+    ZeroArgs z{};
+    z.grad = static_cast<unsigned char*>(grad_table); z.met = at(p.met); z.row_bytes = (long long)D * es; z.rows = rows;
+    const long long wanted = (16 << 10) / z.row_bytes;          // about 16 KB to a warp
+    z.per_warp = 1;
+    while (z.per_warp < 32 && 2 * z.per_warp <= wanted) z.per_warp *= 2;
+    z.batches = (rows + 8LL * z.per_warp - 1) / (8LL * z.per_warp);
     SortArgs a{};
     a.ids = ids; a.rows = rows; a.padding = padding_id;
-    a.n = (int)n; a.tile = p.tile; a.tiles = p.tiles; a.bits = p.bits; a.count = at(p.count);
-    for (int k = 0; k < p.passes; ++k) {
-        a.shift = k * p.bits;
-        a.key = at(p.key[(k + 1) & 1]); a.pos = at(p.pos[(k + 1) & 1]);
-        a.key_out = at(p.key[k & 1]); a.pos_out = at(p.pos[k & 1]);
-        int rc;
-        if (k > 0) {
-            rc = launch_kernel(emb_sort_count<NoIds>, p.tiles, 256, 0, s, false, a);
-            if (!rc) rc = launch_kernel(emb_sort_scatter<NoIds>, p.tiles, 256, 0, s, false, a);
-        } else if (id_bytes == 8) {
-            rc = launch_kernel(emb_sort_count<long long>, p.tiles, 256, 0, s, false, a);
-            if (!rc) rc = launch_kernel(emb_sort_scatter<long long>, p.tiles, 256, 0, s, false, a);
-        } else {
-            rc = launch_kernel(emb_sort_count<int>, p.tiles, 256, 0, s, false, a);
-            if (!rc) rc = launch_kernel(emb_sort_scatter<int>, p.tiles, 256, 0, s, false, a);
-        }
+    a.n = (int)n; a.tile = p.tile; a.tiles = p.tiles; a.bits = p.bits; a.passes = p.passes; a.met = at(p.met);
+    a.counters = reinterpret_cast<Counters*>(ws + p.counters);
+    a.clear = at(p.clear); a.clear_words = (long long)((p.clear_end - p.clear) / 4);
+    a.zero = z;
+    int rc = HFUSE_OK;
+    const int last = p.small ? 0 : (p.passes - 1) & 1;
+    if (p.small) {
+        a.key_out = at(p.key[0]); a.pos_out = at(p.pos[0]);
+        const size_t smem = (size_t)(rows + 31) / 32 * 4 + kSmallTokens * 6 + kMaxBins * 4 + 32 * kMaxBins * 2;
+        rc = id_bytes == 8 ? launch_kernel(emb_sort_small<long long>, 1, 1024, smem, s, false, a)
+                           : launch_kernel(emb_sort_small<int>, 1, 1024, smem, s, false, a);
         if (rc) return rc;
+    } else {
+        if ((rc = launch_kernel(emb_clear, f.sms, 256, 0, s, false, a))) return rc;
+        for (int k = 0; k < p.passes; ++k) {
+            a.pass = k;
+            a.shift = k * p.bits;
+            a.key = at(p.key[(k + 1) & 1]); a.pos = at(p.pos[(k + 1) & 1]);
+            a.key_out = at(p.key[k & 1]); a.pos_out = at(p.pos[k & 1]);
+            a.count = at(p.count[k]); a.next = k + 1 < p.passes ? at(p.count[k + 1]) : nullptr;
+            const int blocks = p.tiles + 2 * f.sms;
+            if (k > 0) {
+                rc = launch_kernel(emb_sort_scatter<NoIds>, blocks, kSortThreads, 0, s, true, a);
+            } else if (id_bytes == 8) {
+                rc = launch_kernel(emb_sort_count<long long>, p.tiles, kSortThreads, 0, s, true, a);
+                if (!rc) rc = launch_kernel(emb_sort_scatter<long long>, blocks, kSortThreads, 0, s, true, a);
+            } else {
+                rc = launch_kernel(emb_sort_count<int>, p.tiles, kSortThreads, 0, s, true, a);
+                if (!rc) rc = launch_kernel(emb_sort_scatter<int>, blocks, kSortThreads, 0, s, true, a);
+            }
+            if (rc) return rc;
+        }
     }
-    const int last = (p.passes - 1) & 1;
+    const int ev = emb_access((int)es, D, grad_out, grad_table);
     EmbSumArgs b{};
     b.dy = grad_out; b.key = at(p.key[last]); b.pos = at(p.pos[last]); b.grad = grad_table;
-    b.part = reinterpret_cast<float*>(ws + p.part);
+    b.part = reinterpret_cast<float*>(ws + p.part); b.crossing = at(p.crossing); b.counters = a.counters;
     b.rows = (unsigned)rows; b.n = (int)n; b.D = D; b.chunks = p.chunks; b.scale = scale;
-    const bool wide = aligned_to(grad_out, 16) && aligned_to(grad_table, 16) && D * es % 16 == 0;
+    b.zero = z;
+    b.packs = D / ev;
+    b.items = (long long)p.chunks * b.packs;
+    b.blocks = (b.items + 255) / 256;
+    const long long grid = b.blocks + z.batches;
+    if (grid > kMaxRows) return HFUSE_ERR_TOO_LARGE;
     return by_type(dtype, [&](auto t) {
         using T = typename decltype(t)::type;
-        constexpr int EV = 16 / sizeof(T);
-        b.packs = wide ? D / EV : D;
-        b.items = (long long)p.chunks * b.packs;
-        const long long want = (b.items + 255) / 256, most = f.sms * 8LL;
-        const int grid = (int)(want < most ? want : most);
-        if (int rc = wide ? launch_kernel(emb_sum<T, EV>, grid, 256, 0, s, false, b) : launch_kernel(emb_sum<T, 1>, grid, 256, 0, s, false, b))
-            return rc;
-        const long long wantj = ((long long)p.chunks * D + 255) / 256;
-        return launch_kernel(emb_join<T>, (int)(wantj < most ? wantj : most), 256, 0, s, false, b);
+        constexpr int EV = 16 / sizeof(T), EV4 = 4 / sizeof(T);
+        rc = ev == EV    ? launch_kernel(emb_sum<T, EV>, (int)grid, 256, 0, s, true, b)
+             : ev == EV4 ? launch_kernel(emb_sum<T, EV4>, (int)grid, 256, 0, s, true, b)
+                         : launch_kernel(emb_sum<T, 1>, (int)grid, 256, 0, s, true, b);
+        if (rc) return rc;
+        return ev == EV ? launch_kernel(emb_join<T, 4>, 2 * f.sms, 32 * kRuns, 0, s, true, b)
+                        : launch_kernel(emb_join<T, 1>, 2 * f.sms, 32 * kRuns, 0, s, true, b);
     });
 }
 
