@@ -8,20 +8,22 @@
 // Memory-bound: the forward pass reads each row it needs and writes it; the backward pass reads grad_out once and
 // writes every row of grad_table once.  The tokens are sorted by id with a stable radix sort (digits of up to 9 bits, at
 // most 4 passes), so that the order of every sum, and with it every bit of the result, is fixed.  The sorted list is cut
-// into chunks of kChunk tokens; each chunk is summed by one thread per group of columns, whatever ids it holds, so a frequent
+// into chunks of 16 or 32 tokens; each chunk is summed by one thread per group of columns, whatever ids it holds, so a frequent
 // token costs no more than rare ones.  A token's run inside one chunk goes straight to the table; the parts of a run that
 // crosses chunks go to the workspace, and a last kernel adds them in order.
 //
 // The kernels of a call, each the programmatic dependent of the one before (its launch overlaps the other's end):
 //   up to 8192 tokens and 262144 rows
-//     sort_small  one block: all passes in shared memory, and the bitmap of the rows that are met
+//     sort_small  every block counts, for a few tokens, how many come before them; marks the rows that are met
 //   otherwise
-//     clear       the bitmap and the counters
+//     clear       the bitmap of the rows that are met and the counters
 //     count       digit counts of each tile of tokens for the first pass; marks the rows that are met
-//     scatter     one per pass: places the tile's tokens and counts the next pass's digits.  A few blocks sort; the others
-//                 meanwhile write the table's rows that are not met, batch by batch until the sorting is done
-//   sum           chunks, and the other rows that are not met
+//     scatter     one per pass: places the tile's tokens and counts the next pass's digits
+//   sum           chunks
 //   join          runs that cross chunks
+// Every row that no token meets is written with zeros, often the larger part of all bytes.  Sorting and joining leave the
+// memory idle most of the time, so every kernel that knows the bitmap writes such rows besides: sort_small a fixed part, the
+// scatters until their tiles are done, join a fixed part, and sum the rest.
 #include "launch.cuh"
 #include "lm_common.cuh"
 
@@ -29,14 +31,16 @@ using namespace hfuse;
 
 namespace {
 
-constexpr int kChunk = 32;
+constexpr int kChunk = 32, kSmallChunk = 16;      // tokens that a thread sums; few tokens: shorter, for twice the threads
 constexpr int kTile = 2048;          // tokens a block ranks at a time
 constexpr int kMaxTiles = 128;
 constexpr int kMaxBins = 512;
 constexpr int kMaxPasses = 4;
 constexpr int kSortThreads = 512;
-constexpr int kSmallTokens = 8192;   // one block's
+constexpr int kSmallTokens = 8192;   // 13 bits beside the 19 of a key
 constexpr long long kSmallRows = 262144;
+constexpr long long kEarlyBytes = 24 << 20;      // rows without a token that sort_small writes, and join: what the memory takes
+constexpr long long kLateBytes = 32 << 20;       // while they would leave it idle
 constexpr int kLongRun = 33;         // parts from which a block, not a warp, adds them up
 
 // counters in the workspace, zero before the first use
@@ -94,16 +98,12 @@ struct ZeroArgs {
     unsigned char* grad;
     const unsigned* met;         // a bit for each row
     long long row_bytes, rows, batches;
+    long long early, late;       // rows that sort_small writes, first batch of join's
     int per_warp;                // rows of a warp, a power of two up to 32
 };
-// the batch's rows, 8 * per_warp of them (or 16 warps' in a block of 512 threads)
-__device__ __forceinline__ void zero_batch(const ZeroArgs& z, long long batch) {
+// zeros for the rows r0 + k of which bit k of `todo` is set
+__device__ __forceinline__ void zero_marked(const ZeroArgs& z, long long r0, unsigned todo) {
     const int lane = threadIdx.x & 31;
-    const long long r0 = (batch * 8 + (threadIdx.x >> 5)) * z.per_warp;
-    if (r0 >= z.rows) return;
-    unsigned todo = ~(z.met[r0 >> 5] >> (r0 & 31));
-    const int here = (int)min((long long)z.per_warp, z.rows - r0);
-    if (here < 32) todo &= (1u << here) - 1;
     while (todo) {
         // neighbouring rows are written as one stretch
         const int k = __ffs(todo) - 1, run = __ffs(~(todo >> k)) - 1;
@@ -118,10 +118,20 @@ __device__ __forceinline__ void zero_batch(const ZeroArgs& z, long long batch) {
             for (unsigned char* q = p + 2 * lane; q < end; q += 64) *reinterpret_cast<unsigned short*>(q) = 0;
         } else {
             if (p + 2 * lane < a0) *reinterpret_cast<unsigned short*>(p + 2 * lane) = 0;
+#pragma unroll 4
             for (unsigned char* q = a0 + 16 * lane; q < a1; q += 512) stg_stream4(reinterpret_cast<float*>(q), zero);
             if (a1 + 2 * lane < end) *reinterpret_cast<unsigned short*>(a1 + 2 * lane) = 0;
         }
     }
+}
+// the rows of a batch, 8 * per_warp of them (a block of 16 warps does two batches)
+__device__ __forceinline__ void zero_batch(const ZeroArgs& z, long long batch) {
+    const long long r0 = (batch * 8 + (threadIdx.x >> 5)) * z.per_warp;
+    if (r0 >= z.rows) return;
+    unsigned todo = ~(z.met[r0 >> 5] >> (r0 & 31));
+    const int here = (int)min((long long)z.per_warp, z.rows - r0);
+    if (here < 32) todo &= (1u << here) - 1;
+    zero_marked(z, r0, todo);
 }
 
 // ---- sort ------------------------------------------------------------------------------------------
@@ -160,8 +170,10 @@ __global__ void __launch_bounds__(256) emb_clear(const SortArgs a) {
 template <class I>
 __global__ void __launch_bounds__(kSortThreads) emb_sort_count(const SortArgs a) {
     __shared__ unsigned bin[kMaxBins];
+    __shared__ unsigned seen[1024];                   // ids that the block has marked, one to a slot: frequent ones are marked once
     const int bins = 1 << a.bits;
     for (int d = threadIdx.x; d < bins; d += kSortThreads) bin[d] = 0;
+    for (int d = threadIdx.x; d < 1024; d += kSortThreads) seen[d] = 0xffffffffu;
     __syncthreads();
     after_predecessor();
     const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile);
@@ -169,16 +181,28 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_count(const SortArgs a)
     for (int i = i0 + threadIdx.x; i < i1; i += kSortThreads) {
         const unsigned k = token_key<I>(a, i);
         atomicAdd(&bin[k & (bins - 1)], 1u);
-        if (k < (unsigned)a.rows && !(a.met[k >> 5] >> (k & 31) & 1u)) atomicOr(a.met + (k >> 5), 1u << (k & 31));
+        if (k < (unsigned)a.rows && *reinterpret_cast<volatile unsigned*>(&seen[k & 1023]) != k) {
+            *reinterpret_cast<volatile unsigned*>(&seen[k & 1023]) = k;
+            atomicOr(a.met + (k >> 5), 1u << (k & 31));
+        }
     }
     __syncthreads();
     for (int d = threadIdx.x; d < bins; d += kSortThreads) a.count[(size_t)blockIdx.x * bins + d] = bin[d];
 }
 
-// ranks of a warp's keys among those with the same digit, 32 keys at a time in their order; cnt: the warp's counts so far
+// Ranks of a warp's keys among those with the same digit, 32 keys at a time in their order; cnt: the warp's counts so far.
+// The lanes with the same digit are found with a vote for each of its bits: matching whole words at once
+// (__match_any_sync) took four times as long.
 template <class C>
-__device__ __forceinline__ unsigned rank_digit(C* cnt, unsigned d, bool in, int lane) {
-    const unsigned same = __match_any_sync(0xffffffffu, in ? d : 0xffffffffu);
+__device__ __forceinline__ unsigned rank_digit(C* cnt, unsigned d, int bits, bool in, int lane) {
+    unsigned same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+    for (int b = 0; b < 9; ++b)
+        if (b < bits) {
+            const bool set = d >> b & 1u;
+            const unsigned votes = __ballot_sync(0xffffffffu, set);
+            same &= set ? votes : ~votes;
+        }
     const unsigned rank = in ? cnt[d] + __popc(same & ((1u << lane) - 1)) : 0u;
     __syncwarp();
     if (in && (same >> lane) == 1u) cnt[d] += (C)__popc(same);         // the highest lane of each digit
@@ -204,7 +228,7 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_scatter(const SortArgs 
                 batch = done == (unsigned)a.tiles ? 0xffffffffu : atomicAdd(&a.counters->zero_next, 2u);
             }
             __syncthreads();
-            if (batch >= a.zero.batches) return;
+            if (batch >= a.zero.late) return;
             zero_batch(a.zero, batch);
         }
     }
@@ -260,7 +284,7 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_scatter(const SortArgs 
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r)
-            rank[r] = rank_digit(cnt[warp], (key[r] >> a.shift) & (bins - 1), at + warp * (32 * ROUNDS) + r * 32 + lane < i1, lane);
+            rank[r] = rank_digit(cnt[warp], (key[r] >> a.shift) & (bins - 1), a.bits, at + warp * (32 * ROUNDS) + r * 32 + lane < i1, lane);
         __syncthreads();
         if (d0 < bins) {                               // each warp's first place for each digit, relative to the tile's
             unsigned b = 0;
@@ -289,90 +313,57 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_scatter(const SortArgs 
     if (threadIdx.x == 0) atomicAdd(&a.counters->sorted[a.pass], 1u);
 }
 
-// All passes of up to 8192 tokens in one block: [bitmap of the rows][keys][positions][warps' counts], the keys in registers
-// while they are ranked.
+// Up to 8192 tokens: key and position make one 32-bit number, all of them are in every block's shared memory, and a warp
+// finds a token's place by counting the smaller ones.  Each block also has a share of the rows to be written here and a
+// share of the others, whose bits go to the bitmap; both begin at a multiple of 32 rows (2 x 4 KB for all kSmallRows).
 template <class I>
 __global__ void __launch_bounds__(1024) emb_sort_small(const SortArgs a) {
-    constexpr int WARPS = 32, ROUNDS = kSmallTokens / 1024;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ unsigned wsum[WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int words = (int)((a.rows + 31) / 32), bins = 1 << a.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned* met = reinterpret_cast<unsigned*>(smem);
-    unsigned* keys = met + words;
-    unsigned* base = keys + kSmallTokens;
-    unsigned short* poss = reinterpret_cast<unsigned short*>(base + kMaxBins);
-    unsigned short* cnt = poss + kSmallTokens;                 // [WARPS][kMaxBins]
-    const int rounds = (a.n + 1023) / 1024;                    // of 32 keys of each warp
-    for (int i = threadIdx.x; i < words; i += 1024) met[i] = 0;
-    unsigned key[ROUNDS], rank[ROUNDS];
-    unsigned short pos[ROUNDS];
+    const int blocks = gridDim.x, b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, padded = (a.n + 127) / 128 * 128;
+    auto cut = [&](long long rows, int k) { return (rows + 31) / 32 * k / blocks * 32; };
+    const long long first = cut(a.zero.early, b), last = min(a.zero.early, cut(a.zero.early, b + 1));
+    const long long other = a.zero.early + cut(a.rows - a.zero.early, b), end = min(a.rows, a.zero.early + cut(a.rows - a.zero.early, b + 1));
+    const int words = (int)((max(last - first, 0LL) + 31) / 32), others = (int)((max(end - other, 0LL) + 31) / 32);
+    unsigned* all = reinterpret_cast<unsigned*>(smem);
+    unsigned* met = all + padded;
+    unsigned* met2 = met + words;
+    for (int i = threadIdx.x; i < words + others; i += 1024) met[i] = 0;
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const int i = (warp * rounds + r) * 32 + lane;
-        key[r] = 0;
-        pos[r] = (unsigned short)i;
-        if (r < rounds && i < a.n) {
-            key[r] = token_key<I>(a, i);
-            if (key[r] < (unsigned)a.rows) atomicOr(met + (key[r] >> 5), 1u << (key[r] & 31));
+#pragma unroll 8
+    for (int i = threadIdx.x; i < padded; i += 1024) {
+        const long long k = i < a.n ? token_key<I>(a, i) : a.rows;
+        all[i] = i < a.n ? (unsigned)k << 13 | (unsigned)i : 0xffffffffu;
+        if (k >= first && k < last) atomicOr(met + (k - first) / 32, 1u << (k & 31));
+        if (k >= other && k < end) atomicOr(met2 + (k - other) / 32, 1u << (k & 31));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < others; i += 1024) a.met[other / 32 + i] = met2[i];
+    for (long long r0 = first + (long long)warp * a.zero.per_warp; r0 < last; r0 += 32LL * a.zero.per_warp) {
+        const int at = (int)(r0 - first), here = (int)min((long long)a.zero.per_warp, last - r0);
+        unsigned todo = ~(met[at >> 5] >> (at & 31));
+        if (here < 32) todo &= (1u << here) - 1;
+        zero_marked(a.zero, r0, todo);
+    }
+    // the stores are on their way; nothing below waits for them
+    for (int i = b * 32 + warp; i < a.n; i += blocks * 32) {
+        const unsigned mine = all[i];
+        unsigned before = 0;
+#pragma unroll 4
+        for (int j = lane * 4; j < padded; j += 128) {
+            const uint4 q = *reinterpret_cast<const uint4*>(all + j);
+            before += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
+        }
+        for (int o = 16; o >= 1; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+        if (lane == 0) {
+            a.key_out[before] = mine >> 13;
+            a.pos_out[before] = mine & (kSmallTokens - 1);
         }
     }
-    for (int pass = 0; pass < a.passes; ++pass) {
-        const int shift = pass * a.bits;
-        for (int d = threadIdx.x; d < WARPS * kMaxBins / 2; d += 1024) reinterpret_cast<unsigned*>(cnt)[d] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < ROUNDS; ++r)
-            if (r < rounds) rank[r] = rank_digit(cnt + warp * kMaxBins, (key[r] >> shift) & (bins - 1), (warp * rounds + r) * 32 + lane < a.n, lane);
-        __syncthreads();
-        unsigned total = 0;
-        if ((int)threadIdx.x < bins) {
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const unsigned c = cnt[w * kMaxBins + threadIdx.x];
-                cnt[w * kMaxBins + threadIdx.x] = (unsigned short)total;
-                total += c;
-            }
-        }
-        unsigned incl = total;
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned u = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += u;
-        }
-        if (lane == 31) wsum[warp] = incl;
-        __syncthreads();
-        unsigned off = incl - total;
-        for (int w = 0; w < warp; ++w) off += wsum[w];
-        if ((int)threadIdx.x < bins) base[threadIdx.x] = off;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < ROUNDS; ++r)
-            if (r < rounds && (warp * rounds + r) * 32 + lane < a.n) {
-                const unsigned d = (key[r] >> shift) & (bins - 1), to = base[d] + cnt[warp * kMaxBins + d] + rank[r];
-                keys[to] = key[r];
-                poss[to] = pos[r];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < ROUNDS; ++r) {
-            const int i = (warp * rounds + r) * 32 + lane;
-            if (r < rounds && i < a.n) {
-                key[r] = keys[i];
-                pos[r] = poss[i];
-            }
-        }
+    if (b == 0 && threadIdx.x == 0) {
+        a.counters->short_runs = a.counters->long_runs = 0;
+        a.counters->zero_next = (unsigned)((a.zero.early + 8 * a.zero.per_warp - 1) / (8 * a.zero.per_warp));
     }
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const int i = (warp * rounds + r) * 32 + lane;
-        if (r < rounds && i < a.n) {
-            a.key_out[i] = key[r];
-            a.pos_out[i] = pos[r];
-        }
-    }
-    for (int i = threadIdx.x; i < words; i += 1024) a.met[i] = met[i];
-    if (threadIdx.x == 0) a.counters->short_runs = a.counters->long_runs = a.counters->zero_next = 0;
 }
 
 // ---- sums ----------------------------------------------------------------------------------------------
@@ -381,14 +372,15 @@ struct EmbSumArgs {
     const unsigned *key, *pos;
     void* grad;
     float* part;                 // [chunks][2][D]: end of a run begun in an earlier chunk, begin of a run that goes on
-    unsigned* crossing;          // chunks in which a run begins that goes on, in any order: short runs from the front, long
+    uint2* crossing;             // (chunk, id) in which a run begins that goes on, in any order: short runs from the front, long
     Counters* counters;          // ones from the back
     long long items;
     unsigned rows;
-    int n, D, packs, chunks;
+    int n, D, packs, chunks, chunk;
     float scale;
     ZeroArgs zero;
     long long blocks;
+    int join_blocks;
 };
 
 template <class T, int EV>
@@ -401,22 +393,22 @@ __device__ __forceinline__ void write_row(const EmbSumArgs& a, unsigned v, long 
 
 template <class T, int EV>
 __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
-    constexpr int P = (EV + 1) / 2, U = 8;                // U rows of grad_out are under way together
+    constexpr int P = (EV + 1) / 2, U = EV >= 4 ? 8 : 16; // U rows of grad_out are under way together
     after_predecessor();
     // blocks that sum and blocks that write zeros take turns, so that reads and writes share the memory all the time
-    const long long total = a.blocks + a.zero.batches, z0 = blockIdx.x * a.zero.batches / total, z1 = (blockIdx.x + 1) * a.zero.batches / total;
+    const long long total = a.blocks + a.zero.late, z0 = blockIdx.x * a.zero.late / total, z1 = (blockIdx.x + 1) * a.zero.late / total;
     if (z1 > z0) {
-        zero_batch(a.zero, z0 + a.counters->zero_next);         // the batches before were written beside the sort
+        const long long batch = z0 + a.counters->zero_next;      // the batches before were written beside the sort
+        if (batch < a.zero.late) zero_batch(a.zero, batch);
         return;
     }
     const long long it = (blockIdx.x - z0) * 256 + threadIdx.x;
     if (it >= a.items) return;
     const int c = (int)(it / a.packs), p = (int)(it - (long long)c * a.packs) * EV;
-    const int s = c * kChunk, e = min(a.n, s + kChunk);
+    const int s = c * a.chunk, e = min(a.n, s + a.chunk);
     unsigned cur = a.key[s];
-    if (cur >= a.rows) return;
-    bool begun = s > 0 && a.key[s - 1] == cur;            // the run began in an earlier chunk
-    const unsigned after = e < a.n ? a.key[e] : a.rows;
+    const unsigned before = s > 0 ? a.key[s - 1] : a.rows, after = e < a.n ? a.key[e] : a.rows;
+    bool begun = before == cur;                           // the run began in an earlier chunk
     float2 acc[P];
 #pragma unroll
     for (int k = 0; k < P; ++k) acc[k] = make_float2(0.f, 0.f);
@@ -442,12 +434,13 @@ __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             if (i + j >= e) break;
+            if (cur >= a.rows) return;
             if (key[j] != cur) {
                 if (begun) keep(part);
                 else write_row<T, EV>(a, cur, p, acc);
                 begun = false;
                 cur = key[j];
-                if (cur >= a.rows) return;                // only such keys follow
+                if (cur >= a.rows) return;                // only keys that get no gradient follow
 #pragma unroll
                 for (int k = 0; k < P; ++k) acc[k] = make_float2(0.f, 0.f);
             }
@@ -460,9 +453,9 @@ __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
     } else if (after == cur) {
         keep(part + a.D);
         if (p == 0) {
-            const bool is_long = c + kLongRun < a.chunks && a.key[(long long)(c + kLongRun) * kChunk] == cur;
+            const bool is_long = c + kLongRun < a.chunks && a.key[(long long)(c + kLongRun) * a.chunk] == cur;
             const unsigned k = atomicAdd(is_long ? &a.counters->long_runs : &a.counters->short_runs, 1u);
-            a.crossing[is_long ? a.chunks - 1 - k : k] = (unsigned)c;
+            a.crossing[is_long ? a.chunks - 1 - k : k] = make_uint2((unsigned)c, cur);
         }
     } else {
         write_row<T, EV>(a, cur, p, acc);
@@ -478,13 +471,19 @@ __global__ void __launch_bounds__(32 * kRuns) emb_join(const EmbSumArgs a) {
     __shared__ int other;
     after_predecessor();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    if ((int)blockIdx.x >= a.join_blocks) {
+        const long long batch = a.zero.late + 2LL * (blockIdx.x - a.join_blocks);
+        if (batch < a.zero.batches) zero_batch(a.zero, batch);
+        return;
+    }
     const int wide_tiles = (a.D + 32 * COLS - 1) / (32 * COLS);
     const long long work = (long long)a.counters->short_runs * wide_tiles;
-    for (long long i = (long long)blockIdx.x * kRuns + ty; i < work; i += (long long)gridDim.x * kRuns) {
-        const int c = (int)a.crossing[i / wide_tiles], col = ((int)(i % wide_tiles) * 32 + tx) * COLS;
-        const unsigned v = a.key[(long long)(c + 1) * kChunk - 1];
+    for (long long i = (long long)blockIdx.x * kRuns + ty; i < work; i += (long long)a.join_blocks * kRuns) {
+        const uint2 run = a.crossing[i / wide_tiles];
+        const int c = (int)run.x, col = ((int)(i % wide_tiles) * 32 + tx) * COLS;
+        const unsigned v = run.y;
         // the chunks that begin with the run's id follow each other
-        const bool same = c + 1 + tx < a.chunks && a.key[(long long)(c + 1 + tx) * kChunk] == v;
+        const bool same = c + 1 + tx < a.chunks && a.key[(long long)(c + 1 + tx) * a.chunk] == v;
         const unsigned more = __ballot_sync(0xffffffffu, same);
         const int parts = 1 + (more == 0xffffffffu ? 32 : __ffs(~more) - 1);
         if (col >= a.D) continue;
@@ -507,15 +506,16 @@ __global__ void __launch_bounds__(32 * kRuns) emb_join(const EmbSumArgs a) {
     }
     const int tiles = (a.D + 31) / 32;
     const long long long_work = (long long)a.counters->long_runs * tiles;
-    for (long long i = blockIdx.x; i < long_work; i += gridDim.x) {
-        const int c = (int)a.crossing[a.chunks - 1 - i / tiles], col = (int)(i % tiles) * 32 + tx;
-        const unsigned v = a.key[(long long)(c + 1) * kChunk - 1];
+    for (long long i = blockIdx.x; i < long_work; i += a.join_blocks) {
+        const uint2 run = a.crossing[a.chunks - 1 - i / tiles];
+        const int c = (int)run.x, col = (int)(i % tiles) * 32 + tx;
+        const unsigned v = run.y;
         int end = c + kLongRun;                            // the first chunk that begins with another id, or none
         for (bool found = false; !found; end += found ? 0 : 32 * kRuns) {
             if (threadIdx.x == 0) other = 0x7fffffff;
             __syncthreads();
             const int k = end + (int)threadIdx.x;
-            if (k >= a.chunks || a.key[(long long)k * kChunk] != v) atomicMin(&other, min(k, a.chunks));
+            if (k >= a.chunks || a.key[(long long)k * a.chunk] != v) atomicMin(&other, min(k, a.chunks));
             __syncthreads();
             found = other != 0x7fffffff;
             if (found) end = other;
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(32 * kRuns) emb_join(const EmbSumArgs a) {
 }
 
 struct EmbPlan {
-    int tile, tiles, passes, bits, chunks;
+    int tile, tiles, passes, bits, chunk, chunks;
     bool small;
     size_t key[2], pos[2], count[kMaxPasses], crossing, counters, met, clear, clear_end, part, bytes;
 };
@@ -554,7 +554,8 @@ EmbPlan emb_plan(long long n, long long rows, int D) {
     while (bits < 32 && (rows >> bits) != 0) ++bits;          // keys are 0 .. rows
     p.passes = (bits + 8) / 9;
     p.bits = (bits + p.passes - 1) / p.passes;
-    p.chunks = (int)((n + kChunk - 1) / kChunk);
+    p.chunk = p.small ? kSmallChunk : kChunk;
+    p.chunks = (int)((n + p.chunk - 1) / p.chunk);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -562,10 +563,10 @@ EmbPlan emb_plan(long long n, long long rows, int D) {
         return r;
     };
     for (int k = 0; k < 2; ++k) {
-        p.key[k] = take((size_t)p.chunks * kChunk * 4);
-        p.pos[k] = take((size_t)p.chunks * kChunk * 4);
+        p.key[k] = take((size_t)p.chunks * p.chunk * 4);
+        p.pos[k] = take((size_t)p.chunks * p.chunk * 4);
     }
-    p.crossing = take((size_t)p.chunks * 4);
+    p.crossing = take((size_t)p.chunks * sizeof(uint2));
     p.count[0] = take((size_t)p.tiles * kMaxBins * 4);
     p.clear = at;                                              // what is cleared first: from here ..
     for (int k = 1; k < p.passes; ++k) p.count[k] = take((size_t)p.tiles * kMaxBins * 4);
@@ -657,6 +658,12 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
     z.per_warp = 1;
     while (z.per_warp < 32 && 2 * z.per_warp <= wanted) z.per_warp *= 2;
     z.batches = (rows + 8LL * z.per_warp - 1) / (8LL * z.per_warp);
+    z.early = p.small ? kEarlyBytes / z.row_bytes / 256 * 256 : 0;              // whole batches
+    if (z.early > rows) z.early = rows;
+    const long long late = kLateBytes / (8LL * z.per_warp * z.row_bytes);
+    z.late = late < z.batches ? z.batches - late : 0;
+    const long long early = (z.early + 8LL * z.per_warp - 1) / (8LL * z.per_warp);
+    if (z.late < early) z.late = early;
     SortArgs a{};
     a.ids = ids; a.rows = rows; a.padding = padding_id;
     a.n = (int)n; a.tile = p.tile; a.tiles = p.tiles; a.bits = p.bits; a.passes = p.passes; a.met = at(p.met);
@@ -667,9 +674,9 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
     const int last = p.small ? 0 : (p.passes - 1) & 1;
     if (p.small) {
         a.key_out = at(p.key[0]); a.pos_out = at(p.pos[0]);
-        const size_t smem = (size_t)(rows + 31) / 32 * 4 + kSmallTokens * 6 + kMaxBins * 4 + 32 * kMaxBins * 2;
-        rc = id_bytes == 8 ? launch_kernel(emb_sort_small<long long>, 1, 1024, smem, s, false, a)
-                           : launch_kernel(emb_sort_small<int>, 1, 1024, smem, s, false, a);
+        const size_t smem = (size_t)(n + 127) / 128 * 512 + (size_t)(rows + 31) / 32 * 4 + 16;      // a share's bits are a part of all
+        rc = id_bytes == 8 ? launch_kernel(emb_sort_small<long long>, f.sms, 1024, smem, s, false, a)
+                           : launch_kernel(emb_sort_small<int>, f.sms, 1024, smem, s, false, a);
         if (rc) return rc;
     } else {
         if ((rc = launch_kernel(emb_clear, f.sms, 256, 0, s, false, a))) return rc;
@@ -679,7 +686,7 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
             a.key = at(p.key[(k + 1) & 1]); a.pos = at(p.pos[(k + 1) & 1]);
             a.key_out = at(p.key[k & 1]); a.pos_out = at(p.pos[k & 1]);
             a.count = at(p.count[k]); a.next = k + 1 < p.passes ? at(p.count[k + 1]) : nullptr;
-            const int blocks = p.tiles + 2 * f.sms;
+            const int blocks = p.tiles + 3 * f.sms;
             if (k > 0) {
                 rc = launch_kernel(emb_sort_scatter<NoIds>, blocks, kSortThreads, 0, s, true, a);
             } else if (id_bytes == 8) {
@@ -695,14 +702,16 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
     const int ev = emb_access((int)es, D, grad_out, grad_table);
     EmbSumArgs b{};
     b.dy = grad_out; b.key = at(p.key[last]); b.pos = at(p.pos[last]); b.grad = grad_table;
-    b.part = reinterpret_cast<float*>(ws + p.part); b.crossing = at(p.crossing); b.counters = a.counters;
-    b.rows = (unsigned)rows; b.n = (int)n; b.D = D; b.chunks = p.chunks; b.scale = scale;
+    b.part = reinterpret_cast<float*>(ws + p.part); b.crossing = reinterpret_cast<uint2*>(ws + p.crossing); b.counters = a.counters;
+    b.rows = (unsigned)rows; b.n = (int)n; b.D = D; b.chunks = p.chunks; b.chunk = p.chunk; b.scale = scale;
     b.zero = z;
     b.packs = D / ev;
     b.items = (long long)p.chunks * b.packs;
     b.blocks = (b.items + 255) / 256;
-    const long long grid = b.blocks + z.batches;
-    if (grid > kMaxRows) return HFUSE_ERR_TOO_LARGE;
+    const long long grid = b.blocks + z.late;
+    b.join_blocks = 4 * f.sms;
+    const long long join_grid = b.join_blocks + (z.batches - z.late + 1) / 2;
+    if (grid > kMaxRows || join_grid > kMaxRows) return HFUSE_ERR_TOO_LARGE;
     return by_type(dtype, [&](auto t) {
         using T = typename decltype(t)::type;
         constexpr int EV = 16 / sizeof(T), EV4 = 4 / sizeof(T);
@@ -710,8 +719,8 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
              : ev == EV4 ? launch_kernel(emb_sum<T, EV4>, (int)grid, 256, 0, s, true, b)
                          : launch_kernel(emb_sum<T, 1>, (int)grid, 256, 0, s, true, b);
         if (rc) return rc;
-        return ev == EV ? launch_kernel(emb_join<T, 4>, 2 * f.sms, 32 * kRuns, 0, s, true, b)
-                        : launch_kernel(emb_join<T, 1>, 2 * f.sms, 32 * kRuns, 0, s, true, b);
+        return ev == EV ? launch_kernel(emb_join<T, 4>, (int)join_grid, 32 * kRuns, 0, s, true, b)
+                        : launch_kernel(emb_join<T, 1>, (int)join_grid, 32 * kRuns, 0, s, true, b);
     });
 }
 
