@@ -14,16 +14,16 @@
 //
 // The kernels of a call, each the programmatic dependent of the one before (its launch overlaps the other's end):
 //   up to 8192 tokens and 262144 rows
-//     sort_small  every block counts, for a few tokens, how many come before them; marks the rows that are met
+//     sort_small  some warps of each block count, for a few tokens, how many come before them, while the others
+//                 write the rows of the block's share that no token meets
 //   otherwise
 //     clear       the bitmap of the rows that are met and the counters
 //     count       digit counts of each tile of tokens for the first pass; marks the rows that are met
-//     scatter     one per pass: places the tile's tokens and counts the next pass's digits
-//   sum           chunks
+//     scatter     one per pass: places the tile's tokens and counts the next pass's digits; blocks beside the sorting ones
+//                 write rows that are not met until the tiles are done
+//   sum           chunks, and the other rows that are not met
 //   join          runs that cross chunks
-// Every row that no token meets is written with zeros, often the larger part of all bytes.  Sorting and joining leave the
-// memory idle most of the time, so every kernel that knows the bitmap writes such rows besides: sort_small a fixed part, the
-// scatters until their tiles are done, join a fixed part, and sum the rest.
+// Rows that no token meets are often the larger part of all bytes, and sorting leaves the memory idle most of the time.
 #include "launch.cuh"
 #include "lm_common.cuh"
 
@@ -39,8 +39,7 @@ constexpr int kMaxPasses = 4;
 constexpr int kSortThreads = 512;
 constexpr int kSmallTokens = 8192;   // 13 bits beside the 19 of a key
 constexpr long long kSmallRows = 262144;
-constexpr long long kEarlyBytes = 24 << 20;      // rows without a token that sort_small writes, and join: what the memory takes
-constexpr long long kLateBytes = 32 << 20;       // while they would leave it idle
+constexpr int kRankWarps = 8;        // of 32 in the small sort; the others write zeros
 constexpr int kLongRun = 33;         // parts from which a block, not a warp, adds them up
 
 // counters in the workspace, zero before the first use
@@ -98,7 +97,6 @@ struct ZeroArgs {
     unsigned char* grad;
     const unsigned* met;         // a bit for each row
     long long row_bytes, rows, batches;
-    long long early, late;       // rows that sort_small writes, first batch of join's
     int per_warp;                // rows of a warp, a power of two up to 32
 };
 // zeros for the rows r0 + k of which bit k of `todo` is set
@@ -228,7 +226,7 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_scatter(const SortArgs 
                 batch = done == (unsigned)a.tiles ? 0xffffffffu : atomicAdd(&a.counters->zero_next, 2u);
             }
             __syncthreads();
-            if (batch >= a.zero.late) return;
+            if (batch >= a.zero.batches) return;
             zero_batch(a.zero, batch);
         }
     }
@@ -314,55 +312,51 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_scatter(const SortArgs 
 }
 
 // Up to 8192 tokens: key and position make one 32-bit number, all of them are in every block's shared memory, and a warp
-// finds a token's place by counting the smaller ones.  Each block also has a share of the rows to be written here and a
-// share of the others, whose bits go to the bitmap; both begin at a multiple of 32 rows (2 x 4 KB for all kSmallRows).
+// finds a token's place by counting the smaller ones.  The other warps write the zeros of the block's share of the rows,
+// which begins at a multiple of 32 rows; its bits (4 KB for all kSmallRows) are in shared memory too.  A token costs a
+// warp some hundred instructions and a row of zeros none of the memory's reads, so the two hide each other.
 template <class I>
 __global__ void __launch_bounds__(1024) emb_sort_small(const SortArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int blocks = gridDim.x, b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, padded = (a.n + 127) / 128 * 128;
-    auto cut = [&](long long rows, int k) { return (rows + 31) / 32 * k / blocks * 32; };
-    const long long first = cut(a.zero.early, b), last = min(a.zero.early, cut(a.zero.early, b + 1));
-    const long long other = a.zero.early + cut(a.rows - a.zero.early, b), end = min(a.rows, a.zero.early + cut(a.rows - a.zero.early, b + 1));
-    const int words = (int)((max(last - first, 0LL) + 31) / 32), others = (int)((max(end - other, 0LL) + 31) / 32);
+    auto cut = [&](int k) { return min(a.rows, (a.rows + 31) / 32 * k / blocks * 32); };
+    const long long first = cut(b), last = cut(b + 1);
+    const int words = (int)((last - first + 31) / 32);
     unsigned* all = reinterpret_cast<unsigned*>(smem);
     unsigned* met = all + padded;
-    unsigned* met2 = met + words;
-    for (int i = threadIdx.x; i < words + others; i += 1024) met[i] = 0;
+    for (int i = threadIdx.x; i < words; i += 1024) met[i] = 0;
     __syncthreads();
 #pragma unroll 8
     for (int i = threadIdx.x; i < padded; i += 1024) {
         const long long k = i < a.n ? token_key<I>(a, i) : a.rows;
         all[i] = i < a.n ? (unsigned)k << 13 | (unsigned)i : 0xffffffffu;
         if (k >= first && k < last) atomicOr(met + (k - first) / 32, 1u << (k & 31));
-        if (k >= other && k < end) atomicOr(met2 + (k - other) / 32, 1u << (k & 31));
     }
+    if (b == 0 && threadIdx.x == 0) a.counters->short_runs = a.counters->long_runs = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < others; i += 1024) a.met[other / 32 + i] = met2[i];
-    for (long long r0 = first + (long long)warp * a.zero.per_warp; r0 < last; r0 += 32LL * a.zero.per_warp) {
-        const int at = (int)(r0 - first), here = (int)min((long long)a.zero.per_warp, last - r0);
-        unsigned todo = ~(met[at >> 5] >> (at & 31));
-        if (here < 32) todo &= (1u << here) - 1;
-        zero_marked(a.zero, r0, todo);
-    }
-    // the stores are on their way; nothing below waits for them
-    for (int i = b * 32 + warp; i < a.n; i += blocks * 32) {
-        const unsigned mine = all[i];
-        unsigned before = 0;
+    if (warp < kRankWarps) {
+        for (int i = b * kRankWarps + warp; i < a.n; i += blocks * kRankWarps) {
+            const unsigned mine = all[i];
+            unsigned before = 0;
 #pragma unroll 4
-        for (int j = lane * 4; j < padded; j += 128) {
-            const uint4 q = *reinterpret_cast<const uint4*>(all + j);
-            before += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
+            for (int j = lane * 4; j < padded; j += 128) {
+                const uint4 q = *reinterpret_cast<const uint4*>(all + j);
+                before += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
+            }
+            for (int o = 16; o >= 1; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+            if (lane == 0) {
+                a.key_out[before] = mine >> 13;
+                a.pos_out[before] = mine & (kSmallTokens - 1);
+            }
         }
-        for (int o = 16; o >= 1; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-        if (lane == 0) {
-            a.key_out[before] = mine >> 13;
-            a.pos_out[before] = mine & (kSmallTokens - 1);
+    } else {
+        for (long long r0 = first + (long long)(warp - kRankWarps) * a.zero.per_warp; r0 < last; r0 += (32LL - kRankWarps) * a.zero.per_warp) {
+            const int at = (int)(r0 - first), here = (int)min((long long)a.zero.per_warp, last - r0);
+            unsigned todo = ~(met[at >> 5] >> (at & 31));
+            if (here < 32) todo &= (1u << here) - 1;
+            zero_marked(a.zero, r0, todo);
         }
-    }
-    if (b == 0 && threadIdx.x == 0) {
-        a.counters->short_runs = a.counters->long_runs = 0;
-        a.counters->zero_next = (unsigned)((a.zero.early + 8 * a.zero.per_warp - 1) / (8 * a.zero.per_warp));
     }
 }
 
@@ -380,7 +374,6 @@ struct EmbSumArgs {
     float scale;
     ZeroArgs zero;
     long long blocks;
-    int join_blocks;
 };
 
 template <class T, int EV>
@@ -391,15 +384,21 @@ __device__ __forceinline__ void write_row(const EmbSumArgs& a, unsigned v, long 
     store_stream<T, EV>(static_cast<T*>(a.grad) + (long long)v * a.D + c, pack_pairs<T, EV>(r));
 }
 
+// a run that begins in chunk c goes on in the next one
+__device__ __forceinline__ void note_crossing(const EmbSumArgs& a, int c, unsigned id) {
+    const bool is_long = c + kLongRun < a.chunks && a.key[(long long)(c + kLongRun) * a.chunk] == id;
+    const unsigned k = atomicAdd(is_long ? &a.counters->long_runs : &a.counters->short_runs, 1u);
+    a.crossing[is_long ? a.chunks - 1 - k : k] = make_uint2((unsigned)c, id);
+}
+
 template <class T, int EV>
 __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
-    constexpr int P = (EV + 1) / 2, U = EV >= 4 ? 8 : 16; // U rows of grad_out are under way together
+    constexpr int P = (EV + 1) / 2, U = 8;                // U rows of grad_out are under way together
     after_predecessor();
     // blocks that sum and blocks that write zeros take turns, so that reads and writes share the memory all the time
-    const long long total = a.blocks + a.zero.late, z0 = blockIdx.x * a.zero.late / total, z1 = (blockIdx.x + 1) * a.zero.late / total;
+    const long long total = a.blocks + a.zero.batches, z0 = blockIdx.x * a.zero.batches / total, z1 = (blockIdx.x + 1) * a.zero.batches / total;
     if (z1 > z0) {
-        const long long batch = z0 + a.counters->zero_next;      // the batches before were written beside the sort
-        if (batch < a.zero.late) zero_batch(a.zero, batch);
+        zero_batch(a.zero, z0 + a.counters->zero_next);         // the batches before were written beside the sort
         return;
     }
     const long long it = (blockIdx.x - z0) * 256 + threadIdx.x;
@@ -452,13 +451,92 @@ __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
         keep(part);
     } else if (after == cur) {
         keep(part + a.D);
-        if (p == 0) {
-            const bool is_long = c + kLongRun < a.chunks && a.key[(long long)(c + kLongRun) * a.chunk] == cur;
-            const unsigned k = atomicAdd(is_long ? &a.counters->long_runs : &a.counters->short_runs, 1u);
-            a.crossing[is_long ? a.chunks - 1 - k : k] = make_uint2((unsigned)c, cur);
-        }
+        if (p == 0) note_crossing(a, c, cur);
     } else {
         write_row<T, EV>(a, cur, p, acc);
+    }
+}
+
+// The same for rows that allow narrow accesses only (EV elements of 2 or 4 bytes): a warp takes a chunk and kCols
+// accesses of each lane, a stretch of 32 apart; the chunk's keys and positions are in its lanes.
+constexpr int kCols = 4;
+template <class T, int EV>
+__global__ void __launch_bounds__(256) emb_sum_narrow(const EmbSumArgs a) {
+    constexpr int P = (EV + 1) / 2, U = 8;
+    after_predecessor();
+    const long long total = a.blocks + a.zero.batches, z0 = blockIdx.x * a.zero.batches / total, z1 = (blockIdx.x + 1) * a.zero.batches / total;
+    if (z1 > z0) {
+        zero_batch(a.zero, z0 + a.counters->zero_next);
+        return;
+    }
+    const long long it = (blockIdx.x - z0) * 8 + (threadIdx.x >> 5);
+    if (it >= a.items) return;
+    const int tiles = (a.packs + 32 * kCols - 1) / (32 * kCols), lane = threadIdx.x & 31;
+    const int c = (int)(it / tiles), first = (int)(it - (long long)c * tiles) * 32 * kCols + lane;
+    const int s = c * a.chunk, count = min(a.n - s, a.chunk);
+    const unsigned key = lane < count ? a.key[s + lane] : a.rows, pos = lane < count ? a.pos[s + lane] : 0;
+    const unsigned before = s > 0 ? a.key[s - 1] : a.rows, after = s + count < a.n ? a.key[s + count] : a.rows;
+    unsigned cur = __shfl_sync(0xffffffffu, key, 0);
+    bool begun = before == cur;
+    float2 acc[kCols][P];
+    auto clear = [&] {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+#pragma unroll
+            for (int k = 0; k < P; ++k) acc[j][k] = make_float2(0.f, 0.f);
+    };
+    auto keep = [&](float* part) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+            if (first + 32 * j < a.packs) {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) part[(first + 32 * j) * EV + k] = k & 1 ? acc[j][k / 2].y : acc[j][k / 2].x;
+            }
+    };
+    auto finish = [&] {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+            if (first + 32 * j < a.packs) write_row<T, EV>(a, cur, (long long)(first + 32 * j) * EV, acc[j]);
+    };
+    float* part = a.part + 2LL * c * a.D;
+    clear();
+    for (int i = 0; i < count; i += U) {
+        Pack<T, EV> g[U][kCols];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned k = __shfl_sync(0xffffffffu, key, min(i + u, 31));
+            const T* row = static_cast<const T*>(a.dy) + (long long)__shfl_sync(0xffffffffu, pos, min(i + u, 31)) * a.D;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) {
+                g[u][j] = {};
+                if (i + u < count && k < a.rows && first + 32 * j < a.packs) g[u][j] = load_stream<T, EV>(row + (long long)(first + 32 * j) * EV);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u >= count || cur >= a.rows) break;
+            const unsigned k = __shfl_sync(0xffffffffu, key, i + u);
+            if (k != cur) {
+                if (begun) keep(part);
+                else finish();
+                cur = k;
+                begun = false;
+                clear();
+            }
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                for (int q = 0; q < P; ++q) acc[j][q] = add2(acc[j][q], pair_of(g[u][j], q));
+        }
+    }
+    if (cur >= a.rows) return;
+    if (begun) {
+        keep(part);
+    } else if (after == cur) {
+        keep(part + a.D);
+        if (first == 0) note_crossing(a, c, cur);
+    } else {
+        finish();
     }
 }
 
@@ -471,14 +549,9 @@ __global__ void __launch_bounds__(32 * kRuns) emb_join(const EmbSumArgs a) {
     __shared__ int other;
     after_predecessor();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    if ((int)blockIdx.x >= a.join_blocks) {
-        const long long batch = a.zero.late + 2LL * (blockIdx.x - a.join_blocks);
-        if (batch < a.zero.batches) zero_batch(a.zero, batch);
-        return;
-    }
     const int wide_tiles = (a.D + 32 * COLS - 1) / (32 * COLS);
     const long long work = (long long)a.counters->short_runs * wide_tiles;
-    for (long long i = (long long)blockIdx.x * kRuns + ty; i < work; i += (long long)a.join_blocks * kRuns) {
+    for (long long i = (long long)blockIdx.x * kRuns + ty; i < work; i += (long long)gridDim.x * kRuns) {
         const uint2 run = a.crossing[i / wide_tiles];
         const int c = (int)run.x, col = ((int)(i % wide_tiles) * 32 + tx) * COLS;
         const unsigned v = run.y;
@@ -506,7 +579,7 @@ __global__ void __launch_bounds__(32 * kRuns) emb_join(const EmbSumArgs a) {
     }
     const int tiles = (a.D + 31) / 32;
     const long long long_work = (long long)a.counters->long_runs * tiles;
-    for (long long i = blockIdx.x; i < long_work; i += a.join_blocks) {
+    for (long long i = blockIdx.x; i < long_work; i += gridDim.x) {
         const uint2 run = a.crossing[a.chunks - 1 - i / tiles];
         const int c = (int)run.x, col = (int)(i % tiles) * 32 + tx;
         const unsigned v = run.y;
@@ -658,12 +731,6 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
     z.per_warp = 1;
     while (z.per_warp < 32 && 2 * z.per_warp <= wanted) z.per_warp *= 2;
     z.batches = (rows + 8LL * z.per_warp - 1) / (8LL * z.per_warp);
-    z.early = p.small ? kEarlyBytes / z.row_bytes / 256 * 256 : 0;              // whole batches
-    if (z.early > rows) z.early = rows;
-    const long long late = kLateBytes / (8LL * z.per_warp * z.row_bytes);
-    z.late = late < z.batches ? z.batches - late : 0;
-    const long long early = (z.early + 8LL * z.per_warp - 1) / (8LL * z.per_warp);
-    if (z.late < early) z.late = early;
     SortArgs a{};
     a.ids = ids; a.rows = rows; a.padding = padding_id;
     a.n = (int)n; a.tile = p.tile; a.tiles = p.tiles; a.bits = p.bits; a.passes = p.passes; a.met = at(p.met);
@@ -678,6 +745,7 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
         rc = id_bytes == 8 ? launch_kernel(emb_sort_small<long long>, f.sms, 1024, smem, s, false, a)
                            : launch_kernel(emb_sort_small<int>, f.sms, 1024, smem, s, false, a);
         if (rc) return rc;
+        z.batches = 0;                                          // nothing is left for the next kernel
     } else {
         if ((rc = launch_kernel(emb_clear, f.sms, 256, 0, s, false, a))) return rc;
         for (int k = 0; k < p.passes; ++k) {
@@ -706,21 +774,20 @@ int hfuse_embedding_backward(const void* grad_out, const void* ids, int64_t n, i
     b.rows = (unsigned)rows; b.n = (int)n; b.D = D; b.chunks = p.chunks; b.chunk = p.chunk; b.scale = scale;
     b.zero = z;
     b.packs = D / ev;
-    b.items = (long long)p.chunks * b.packs;
-    b.blocks = (b.items + 255) / 256;
-    const long long grid = b.blocks + z.late;
-    b.join_blocks = 4 * f.sms;
-    const long long join_grid = b.join_blocks + (z.batches - z.late + 1) / 2;
-    if (grid > kMaxRows || join_grid > kMaxRows) return HFUSE_ERR_TOO_LARGE;
+    const bool narrow = ev * es < 16;
+    b.items = (long long)p.chunks * (narrow ? (b.packs + 32 * kCols - 1) / (32 * kCols) : b.packs);      // of warps, of threads
+    b.blocks = narrow ? (b.items + 7) / 8 : (b.items + 255) / 256;
+    const long long grid = b.blocks + z.batches;
+    if (grid > kMaxRows) return HFUSE_ERR_TOO_LARGE;
     return by_type(dtype, [&](auto t) {
         using T = typename decltype(t)::type;
         constexpr int EV = 16 / sizeof(T), EV4 = 4 / sizeof(T);
         rc = ev == EV    ? launch_kernel(emb_sum<T, EV>, (int)grid, 256, 0, s, true, b)
-             : ev == EV4 ? launch_kernel(emb_sum<T, EV4>, (int)grid, 256, 0, s, true, b)
-                         : launch_kernel(emb_sum<T, 1>, (int)grid, 256, 0, s, true, b);
+             : ev == EV4 ? launch_kernel(emb_sum_narrow<T, EV4>, (int)grid, 256, 0, s, true, b)
+                         : launch_kernel(emb_sum_narrow<T, 1>, (int)grid, 256, 0, s, true, b);
         if (rc) return rc;
-        return ev == EV ? launch_kernel(emb_join<T, 4>, (int)join_grid, 32 * kRuns, 0, s, true, b)
-                        : launch_kernel(emb_join<T, 1>, (int)join_grid, 32 * kRuns, 0, s, true, b);
+        return ev == EV ? launch_kernel(emb_join<T, 4>, 4 * f.sms, 32 * kRuns, 0, s, true, b)
+                        : launch_kernel(emb_join<T, 1>, 4 * f.sms, 32 * kRuns, 0, s, true, b);
     });
 }
 
