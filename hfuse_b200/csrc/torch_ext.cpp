@@ -6,6 +6,7 @@
 // checks tensors, allocates the outputs and forwards raw pointers plus the current stream to the C
 // ABI in include/hfuse_b200.h; all device code lives in libhfuse_b200.so.  CUDA tensors only.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -239,6 +240,11 @@ std::tuple<Tensor, Tensor, Tensor> histc_bnstats(const Tensor& x, int64_t bins, 
 // ---- operators of a language model's token path ---------------------------------------------------------
 using OptTensor = const std::optional<Tensor>&;
 
+// These operators are called for single tokens too, where the host's time counts: no dispatch for each buffer.
+Tensor buffer(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
+}
+
 int lm_type(const Tensor& t, const char* what) {
     TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor: hfuse_b200 has no CPU path");
     switch (t.scalar_type()) {
@@ -299,8 +305,9 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm(const Tensor& x, OptTensor weight,
     const auto wt = norm_params(x, weight, bias);
     const int64_t D = x.size(-1), ld = row_stride(x, "layer_norm input");
     c10::cuda::CUDAGuard g(x.device());
-    Tensor y = at::empty(x.sizes(), x.options());
-    Tensor mean = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat)), invstd = at::empty_like(mean);
+    Tensor y = buffer(x.sizes(), x.scalar_type(), x);
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    Tensor mean = buffer(lead, at::kFloat, x), invstd = buffer(lead, at::kFloat, x);
     ok(hfuse_layernorm(x.data_ptr(), x.numel() / D, i32(D), ld, type, opt_ptr(weight), opt_ptr(bias), code_of(wt), (float)eps,
                        y.data_ptr(), mean.data_ptr<float>(), invstd.data_ptr<float>(), stream()), "hfuse_layernorm");
     return {y, mean, invstd};
@@ -318,9 +325,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& x, const Te
     const int64_t D = x.size(-1), rows = x.numel() / D;
     const int64_t ldx = row_stride(x, "layer_norm input"), ldg = row_stride(grad_out, "layer_norm grad_out");
     c10::cuda::CUDAGuard g(x.device());
-    Tensor dx = at::empty(x.sizes(), x.options());
-    Tensor dw = at::empty({D}, x.options().dtype(wt)), db = at::empty({D}, x.options().dtype(wt));
-    Tensor ws = at::empty({(int64_t)hfuse_layernorm_backward_workspace_bytes(rows, i32(D))}, x.options().dtype(at::kByte));
+    Tensor dx = buffer(x.sizes(), x.scalar_type(), x), dw = buffer({D}, wt, x), db = buffer({D}, wt, x);
+    Tensor ws = buffer({(int64_t)hfuse_layernorm_backward_workspace_bytes(rows, i32(D))}, at::kByte, x);
     ok(hfuse_layernorm_backward(x.data_ptr(), ldx, grad_out.data_ptr(), ldg, rows, i32(D), type, mean.data_ptr<float>(),
                                 invstd.data_ptr<float>(), opt_ptr(weight), code_of(wt), dx.data_ptr(), dw.data_ptr(),
                                 db.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), stream()), "hfuse_layernorm_backward");
@@ -341,7 +347,7 @@ Tensor embedding(const Tensor& table, const Tensor& ids, double scale) {
     c10::cuda::CUDAGuard g(table.device());
     auto shape = ids.sizes().vec();
     shape.push_back(table.size(1));
-    Tensor out = at::empty(shape, table.options());
+    Tensor out = buffer(shape, table.scalar_type(), table);
     ok(hfuse_embedding(table.data_ptr(), table.size(0), i32(table.size(1)), type, ids.data_ptr(), ids.numel(),
                        i32(ids.element_size()), (float)scale, out.data_ptr(), stream()), "hfuse_embedding");
     return out;
@@ -356,8 +362,8 @@ Tensor embedding_backward(const Tensor& grad_out, const Tensor& ids, int64_t row
     const int64_t D = grad_out.size(-1), n = ids.numel();
     TORCH_CHECK(D <= INT32_MAX, "embedding grad_out has too long rows");
     c10::cuda::CUDAGuard g(grad_out.device());
-    Tensor grad = at::empty({rows, D}, grad_out.options());
-    Tensor ws = at::empty({(int64_t)hfuse_embedding_backward_workspace_bytes(n, rows, i32(D))}, grad_out.options().dtype(at::kByte));
+    Tensor grad = buffer({rows, D}, grad_out.scalar_type(), grad_out);
+    Tensor ws = buffer({(int64_t)hfuse_embedding_backward_workspace_bytes(n, rows, i32(D))}, at::kByte, grad_out);
     ok(hfuse_embedding_backward(grad_out.data_ptr(), ids.data_ptr(), n, i32(ids.element_size()), rows, i32(D), type, (float)scale,
                                 padding_id, grad.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), stream()),
        "hfuse_embedding_backward");
@@ -381,9 +387,8 @@ std::tuple<Tensor, Tensor, Tensor> gated_recurrence(const Tensor& gate, const Te
     const int64_t B = x.size(0), T = x.size(1), D = x.size(2), BD[2] = {B, D};
     if (h0) check_vec(*h0, x, at::kFloat, BD, "h0");
     c10::cuda::CUDAGuard g(x.device());
-    const auto f32 = x.options().dtype(at::kFloat);
-    Tensor out = at::empty(x.sizes(), x.options()), last = at::empty({B, D}, f32);
-    Tensor states = save_states ? at::empty({B, hfuse_gated_recurrence_chunks(T), D}, f32) : at::empty({0}, f32);
+    Tensor out = buffer(x.sizes(), x.scalar_type(), x), last = buffer({B, D}, at::kFloat, x);
+    Tensor states = save_states ? buffer({B, hfuse_gated_recurrence_chunks(T), D}, at::kFloat, x) : buffer({0}, at::kFloat, x);
     ok(hfuse_gated_recurrence(gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), B, T, i32(D),
                               type, opt_f32(h0), out.data_ptr(), last.data_ptr<float>(),
                               save_states ? states.data_ptr<float>() : nullptr, stream()), "hfuse_gated_recurrence");
@@ -398,8 +403,8 @@ std::tuple<Tensor, Tensor, Tensor> gated_recurrence_backward(const Tensor& gate,
     check_vec(states, x, at::kFloat, S, "states");
     if (grad_last) check_vec(*grad_last, x, at::kFloat, BD, "grad_last");
     c10::cuda::CUDAGuard g(x.device());
-    Tensor dgate = at::empty(x.sizes(), x.options()), dx = at::empty(x.sizes(), x.options());
-    Tensor dh0 = at::empty({B, D}, x.options().dtype(at::kFloat));
+    Tensor dgate = buffer(x.sizes(), x.scalar_type(), x), dx = buffer(x.sizes(), x.scalar_type(), x);
+    Tensor dh0 = buffer({B, D}, at::kFloat, x);
     ok(hfuse_gated_recurrence_backward(gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1),
                                        states.data_ptr<float>(), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
                                        opt_f32(grad_last), B, T, i32(D), type, dgate.data_ptr(), dx.data_ptr(),

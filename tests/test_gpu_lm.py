@@ -42,7 +42,8 @@ def api(request):
 
 # ---- layer norm -------------------------------------------------------------------------------------------------
 NORM_SHAPES = [(1, 1), (1, 4096), (3, 7), (5, 32), (700, 64), (37, 129), (2, 1001), (333, 1000), (64, 2048), (300, 512), (9, 8192),
-               (5, 8190), (3, 16384), (3, 20000), (2, 70001), (2500, 96), (5000, 24), (1200, 256), (450, 1024), (301, 4095)]
+               (5, 8190), (3, 16384), (3, 20000), (2, 70001), (2500, 96), (5000, 24), (1200, 256), (450, 1024), (301, 4095),
+               (600, 4096), (601, 1001), (700, 2050), (300, 8192), (257, 8191), (130, 16384), (100, 24576)]
 
 
 def _norm_inputs(dev, rows, D, t, wt, seed, offset=0.3):
@@ -194,7 +195,9 @@ def _ids(dev, n, V, how, seed):
     (1, 1, 1, "one", "f32"), (2, 511, 8, "even", "bf16"), (31, 512, 16, "even", "f16"), (32, 513, 33, "one", "bf16"),
     (33, 3, 64, "one", "f32"), (64, 2, 8, "rising", "f32"), (65, 64, 8, "rising", "f16"), (2047, 1000, 40, "text", "f32"),
     (2048, 262143, 8, "even", "bf16"), (2049, 262144, 8, "even", "f32"), (4100, 50257, 1001, "text", "f16"),
-    (5000, 100, 128, "text", "bf16"), (70000, 30000, 64, "text", "bf16"), (40000, 4, 24, "one", "f32"), (300000, 1000, 8, "text", "f32"),
+    (5000, 100, 128, "text", "bf16"), (255, 60, 65, "text", "bf16"), (256, 9, 40, "one", "f16"), (257, 60, 65, "text", "f32"),
+    (8192, 4000, 48, "text", "bf16"), (8193, 4000, 50, "text", "f16"), (200, 600000, 8, "even", "bf16"), (8000, 300000, 8, "even", "f16"),
+ (70000, 30000, 64, "text", "bf16"), (40000, 4, 24, "one", "f32"), (300000, 1000, 8, "text", "f32"),
     (300000, 7, 8, "even", "bf16"), (777, 1 << 20, 9, "even", "f32"), (16384, 32000, 512, "text", "f16"), (9000, 9000, 2048, "rising", "bf16")])
 def test_embedding_backward(dev, n, V, D, how, kind):
     ids = _ids(dev, n, V, how, 22)
