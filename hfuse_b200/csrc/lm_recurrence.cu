@@ -13,9 +13,15 @@
 // with the state in registers.  The backward pass does the same from the end (its maps are e -> A e + E),
 // with the states before each step run again from the ones that the forward pass saved every 256 steps.
 //
-// The next pieces of the sequence are on their way into shared memory (cp.async) while one is worked on.  Where there
-// are fewer groups of channels than the GPU has room for, a cluster of blocks shares a group: each takes a piece in turn
-// and the blocks' maps are exchanged through distributed shared memory.
+// The next pieces of the sequence are on their way into shared memory while one is worked on: as TMA tiles where the tensors
+// allow it (the results take the places of the inputs and leave as tiles too, all issued by a warp of its own, so that
+// the others only compute), else by cp.async.  Where there are fewer groups of channels than the GPU has room for, a
+// cluster of blocks shares a group: each takes a piece in turn and the blocks' maps are exchanged through
+// distributed shared memory.
+#include <cuda.h>
+
+#include <initializer_list>
+
 #include "launch.cuh"
 #include "lm_common.cuh"
 
@@ -24,6 +30,8 @@ using namespace hfuse;
 namespace {
 
 constexpr int kSaved = HFUSE_RECURRENCE_CHUNK;
+constexpr int kWarpsFwd = 8, kWarpsBwd = 16, kSteps = 16;     // a whole piece of the backward pass is kSaved steps
+static_assert(kWarpsBwd * kSteps == kSaved && kSaved % kSteps == 0, "pieces begin where states are saved");
 constexpr int kMaxCluster = 8;
 
 struct RecArgs {
@@ -230,6 +238,13 @@ struct Peers {
     int split, rank;
     bool lost = false;             // a wait ran out: results become NaN
 
+    __device__ __forceinline__ Peers(float* at, int split_, int rank_)
+        : sets(at), bars(reinterpret_cast<unsigned long long*>(at + 2 * kMaxCluster * C * 2)), split(split_), rank(rank_) {}
+    __device__ __forceinline__ void spoil(float (&u)[CPL], float (&v)[CPL]) const {
+        if (!lost) return;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) u[c] = v[c] = __int_as_float(0x7fc00000);
+    }
     __device__ __forceinline__ void begin() {
         if (threadIdx.x == 0) {
             mbar_init(bars, 1);
@@ -257,27 +272,186 @@ struct Peers {
     }
 };
 
-// shared memory of a block: two stages of `tensors` tiles, the warps' maps (`maps` per channel; the barrier at the top of a
-// piece is behind their last reader), the state that goes on to the next piece, the blocks' maps
-template <class T, int CPL>
-size_t rec_smem(int warps, int steps, int tensors, int maps, int split) {
-    const size_t C = 32 * CPL;
-    return 2 * (size_t)tensors * warps * steps * C * sizeof(T) + (size_t)maps * warps * C * 8 + C * 4 +
-           (split > 1 ? 2 * (size_t)kMaxCluster * C * 8 + 16 : 0);
+// ---- the steps of a piece, shared by both kinds of staging ------------------------------------------------
+// forward: results from zero and products of the a so far, for the warp's steps
+template <class T, int CPL, int N>
+__device__ __forceinline__ void run_forward(const T* sg, const T* sx, float2 (&h)[N], float2 (&a)[N], float (&A)[CPL], float (&H)[CPL]) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) { H[c] = 0.f; A[c] = 1.f; }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float2 at, zt;
+        gates2(read_pair<T, CPL>(sg, i), at, zt);
+        h[i] = run_pair<CPL>(at, mul2(zt, read_pair<T, CPL>(sx, i)), H);
+        a[i] = scale_pair<CPL>(at, A);
+    }
+}
+// After the barrier behind write_map: the state before the warp's first step (in), and the one before the next piece
+// (carry), which a single block's last warp hands on through `next`, [2][C], and a cluster's warps all know.
+template <int CPL>
+__device__ __forceinline__ void join_forward(const float* map, float* next, int it, int W, int warp, int lane, float (&A)[CPL], float (&H)[CPL],
+                                             float (&in)[CPL], float (&carry)[CPL], Peers<CPL>& peers) {
+    constexpr int C = 32 * CPL;
+    if (peers.split == 1) {
+        if (it > 0) read_state<CPL>(next + (it & 1) * C, carry, CPL);
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) in[c] = carry[c];
+#pragma unroll 4
+        for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
+        if (warp == W - 1) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) next[(~it & 1) * C + c] = carry[c] = fmaf(A[c], in[c], H[c]);
+        }
+        return;
+    }
+    if (warp < peers.split) {                             // W >= split: see rec_launch
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = 0.f; }
+#pragma unroll 4
+        for (int w = 0; w < W; ++w) join_map<CPL>(map + w * 2 * C, A, H);
+        peers.send(it, warp, lane, A, H);
+    }
+    const float* set = peers.receive(it, lane);
+#pragma unroll 4
+    for (int j = 0; j < peers.rank; ++j) apply_map<CPL>(set + j * 2 * C, carry);
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) in[c] = carry[c];
+#pragma unroll 4
+    for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
+#pragma unroll 4
+    for (int j = peers.rank; j < peers.split; ++j) apply_map<CPL>(set + j * 2 * C, carry);
+    peers.spoil(in, carry);
 }
 
+// backward: a, 1 - a and the maps of the warp's steps.  E, what e of zero becomes over the steps, is the sum of dy_t times
+// the product of the a up to a_t.
+template <class T, int CPL, int N>
+__device__ __forceinline__ void run_backward(const T* sg, const T* sx, const T* sd, float2 (&a)[N], float2 (&z)[N], float (&A)[CPL],
+                                             float (&H)[CPL], float (&E)[CPL]) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = E[c] = 0.f; }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        gates2(read_pair<T, CPL>(sg, i), a[i], z[i]);
+        run_pair<CPL>(a[i], mul2(z[i], read_pair<T, CPL>(sx, i)), H);
+        const float2 P = scale_pair<CPL>(a[i], A), u = read_pair<T, CPL>(sd, i);
+        if constexpr (CPL == 2) {
+            const float2 r = fma2(P, u, make_float2(E[0], E[1]));
+            E[0] = r.x;
+            E[1] = r.y;
+        } else {
+            E[0] = fmaf(P.y, u.y, fmaf(P.x, u.x, E[0]));
+        }
+    }
+}
+// The warps' A, H and E, [W][C] each.
+template <int CPL>
+struct Maps3 {
+    static constexpr int C = 32 * CPL;
+    float* at;                   // this lane's place
+    int W;
+    __device__ __forceinline__ void write(int warp, const float (&A)[CPL], const float (&H)[CPL], const float (&E)[CPL]) const {
+        write_state<CPL>(at + warp * C, A, CPL);
+        write_state<CPL>(at + (W + warp) * C, H, CPL);
+        write_state<CPL>(at + (2 * W + warp) * C, E, CPL);
+    }
+    // v -> A v + H (which = 1) or A v + E (which = 2) of warp w
+    __device__ __forceinline__ void apply(int w, int which, float (&v)[CPL]) const {
+        const float *A = at + w * C, *B = at + (which * W + w) * C;
+        if constexpr (CPL == 2) {
+            const float2 r = fma2(*reinterpret_cast<const float2*>(A), make_float2(v[0], v[1]), *reinterpret_cast<const float2*>(B));
+            v[0] = r.x;
+            v[1] = r.y;
+        } else {
+            v[0] = fmaf(A[0], v[0], B[0]);
+        }
+    }
+};
+// After the barrier behind Maps3::write: hb from the state before the piece to the one before the warp's first step, and e
+// from behind its last step.
+template <int CPL>
+__device__ __forceinline__ void join_backward(const Maps3<CPL>& maps, float* next, int k, int warp, int lane, float (&A)[CPL], float (&E)[CPL],
+                                              float (&hb)[CPL], float (&e)[CPL], float (&carry)[CPL], Peers<CPL>& peers) {
+    constexpr int C = 32 * CPL;
+    const int W = maps.W;
+#pragma unroll 4
+    for (int w = 0; w < warp; ++w) maps.apply(w, 1, hb);
+    if (peers.split == 1) {
+        if (k > 0) read_state<CPL>(next + (k & 1) * C, carry, CPL);
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+#pragma unroll 4
+        for (int w = W - 1; w > warp; --w) maps.apply(w, 2, e);
+        if (warp == 0) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) next[(~k & 1) * C + c] = carry[c] = fmaf(A[c], e[c], E[c]);
+        }
+        return;
+    }
+    if (warp < peers.split) {
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) { A[c] = 1.f; E[c] = 0.f; }
+#pragma unroll 4
+        for (int w = W - 1; w >= 0; --w) {
+            maps.apply(w, 2, E);
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) A[c] *= maps.at[w * C + c];
+        }
+        peers.send(k, warp, lane, A, E);
+    }
+    const float* set = peers.receive(k, lane);
+#pragma unroll 4
+    for (int j = peers.split - 1; j > peers.rank; --j) apply_map<CPL>(set + j * 2 * C, carry);
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+#pragma unroll 4
+    for (int w = W - 1; w > warp; --w) maps.apply(w, 2, e);
+#pragma unroll 4
+    for (int j = peers.rank; j >= 0; --j) apply_map<CPL>(set + j * 2 * C, carry);
+    peers.spoil(e, carry);
+}
+// dgate and dx of the warp's steps, put(i, dgate, dx) for every pair from the last one on
+template <class T, int CPL, int N, class Put>
+__device__ __forceinline__ void sweep_backward(const T* sx, const T* sd, const float2 (&a)[N], const float2 (&z)[N], float (&hb)[CPL], float (&e)[CPL],
+                                               Put&& put) {
+    float2 f[N];                                          // dgate's factor (h_{t-1} - x_t) a z, the states run again
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float2 v = read_pair<T, CPL>(sx, i);
+        float2 before;
+        run_pair<CPL>(a[i], mul2(z[i], v), hb, &before);
+        f[i] = mul2(fma2(v, make_float2(-1.f, -1.f), before), mul2(a[i], z[i]));
+    }
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) {
+        const float2 u = read_pair<T, CPL>(sd, i);
+        float2 et;                                        // e of the pair's steps
+        if constexpr (CPL == 2) {
+            et = add2(make_float2(e[0], e[1]), u);
+            const float2 r = mul2(et, a[i]);
+            e[0] = r.x;
+            e[1] = r.y;
+        } else {
+            et.y = e[0] + u.y;
+            et.x = fmaf(et.y, a[i].y, u.x);
+            e[0] = et.x * a[i].x;
+        }
+        put(i, mul2(et, f[i]), mul2(et, z[i]));
+    }
+}
+
+// ---- staging by cp.async -----------------------------------------------------------------------------------
+// [2 stages][tensors][rows][C], the warps' maps (the barrier at the top of a piece is behind their last reader), next, peers
 template <class T, int CPL, int S, int ALIGN>
 __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
     constexpr int C = 32 * CPL, N = S * CPL / 2;
     extern __shared__ __align__(128) unsigned char smem[];
     const int W = blockDim.x >> 5, warp = warp_index(), lane = threadIdx.x & 31, rows = W * S;
-    T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x][rows][C]
-    float* map = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T)) + lane * CPL * 2;   // [W][C]{A, H}
-    float* next = map - lane * CPL * 2 + 2 * W * C + lane * CPL;              // [C]
-    const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
-    Peers<CPL> peers{next - lane * CPL + C, nullptr, p.split, rank};
-    peers.bars = reinterpret_cast<unsigned long long*>(peers.sets + 2 * kMaxCluster * C * 2);
-    const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
+    T* stage = reinterpret_cast<T*>(smem);
+    float* map = reinterpret_cast<float*>(smem + 4 * (size_t)rows * C * sizeof(T));      // [W][C]{A, H}
+    float* next = map + 2 * W * C;
+    Peers<CPL> peers(next + 2 * C, p.split, blockIdx.x % p.split);
+    const int group = blockIdx.x / p.split, b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
     const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
     const T* x = static_cast<const T*>(p.x) + b * p.x_b;
     T* y = static_cast<T*>(p.y) + (long long)b * p.T * p.D + d;
@@ -287,7 +461,7 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
     auto issue = [&](int it) {
         if (it < n) {
             T* s = stage + (it & 1) * 2 * rows * C;
-            const int t0 = (it * p.split + rank) * rows;
+            const int t0 = (it * p.split + peers.rank) * rows;
             stage_rows<T, CPL, ALIGN, S>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
             stage_rows<T, CPL, ALIGN, S>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
         }
@@ -299,58 +473,17 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
     read_state<CPL>(p.h0 ? p.h0 + at_state : nullptr, carry, left);
     if (p.split > 1) peers.begin();
     for (int it = 0; it < n; ++it) {
-        const int t0 = (it * p.split + rank) * rows + warp * S;
+        const int t0 = (it * p.split + peers.rank) * rows + warp * S;
         const T* sg = stage + (it & 1) * 2 * rows * C + warp * S * C + lane * CPL;
-        const T* sx = sg + rows * C;
         cp_wait<1>();
         __syncthreads();
-        if (p.split == 1 && it > 0) read_state<CPL>(next, carry, CPL);
-        float2 h[N], a[N];                                // results from zero, products of the a so far
-        float H[CPL], A[CPL];
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) { H[c] = 0.f; A[c] = 1.f; }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float2 at, zt;
-            gates2(read_pair<T, CPL>(sg, i), at, zt);
-            h[i] = run_pair<CPL>(at, mul2(zt, read_pair<T, CPL>(sx, i)), H);
-            a[i] = scale_pair<CPL>(at, A);
-        }
-        write_map<CPL>(map + warp * 2 * C, A, H);
+        float2 h[N], a[N];
+        float H[CPL], A[CPL], in[CPL];
+        run_forward<T, CPL, N>(sg, sg + rows * C, h, a, A, H);
+        write_map<CPL>(map + (warp * C + lane * CPL) * 2, A, H);
         __syncthreads();
         issue(it + 2);                                    // every warp has read this stage
-        float in[CPL];
-        if (p.split == 1) {
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) in[c] = carry[c];
-#pragma unroll 4
-            for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
-            if (warp == W - 1) {                          // what the block's last step leaves
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) next[c] = carry[c] = fmaf(A[c], in[c], H[c]);
-            }
-        } else {
-            if (warp < p.split) {                         // W >= split: see rec_launch
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = 0.f; }
-#pragma unroll 4
-                for (int w = 0; w < W; ++w) join_map<CPL>(map + w * 2 * C, A, H);
-                peers.send(it, warp, lane, A, H);
-            }
-            const float* set = peers.receive(it, lane);
-#pragma unroll 4
-            for (int j = 0; j < rank; ++j) apply_map<CPL>(set + j * 2 * C, carry);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) in[c] = carry[c];
-#pragma unroll 4
-            for (int w = 0; w < warp; ++w) apply_map<CPL>(map + w * 2 * C, in);
-#pragma unroll 4
-            for (int j = rank; j < p.split; ++j) apply_map<CPL>(set + j * 2 * C, carry);
-            if (peers.lost) {
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) in[c] = carry[c] = __int_as_float(0x7fc00000);
-            }
-        }
+        join_forward<CPL>(map + lane * CPL * 2, next + lane * CPL, it, W, warp, lane, A, H, in, carry, peers);
         if (p.states && t0 < p.T && t0 % kSaved == 0)
             write_state<CPL>(p.states + ((long long)b * p.chunks + t0 / kSaved) * p.D + d, in, left);
         T* to = y + (long long)t0 * p.D;
@@ -364,7 +497,7 @@ __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
             for (int i = 0; i < N; ++i) write_pair<T, CPL, (ALIGN >= 4)>(to, p.D, i, h[i], p.T - t0, left);
         }
     }
-    if (warp == W - 1 && rank == 0) write_state<CPL>(p.last + at_state, carry, left);
+    if (warp == W - 1 && peers.rank == 0) write_state<CPL>(p.last + at_state, carry, left);
     if (p.split > 1) cluster_sync();                      // no block ends while a peer may still write to it
 }
 
@@ -373,14 +506,12 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
     constexpr int C = 32 * CPL, N = S * CPL / 2;
     extern __shared__ __align__(128) unsigned char smem[];
     const int W = blockDim.x >> 5, warp = warp_index(), lane = threadIdx.x & 31, rows = W * S;
-    T* stage = reinterpret_cast<T*>(smem);                                    // [2][gate, x, dy][rows][C]
-    float* mapH = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T)) + lane * CPL * 2;  // [W][C]{A, H}
-    float* mapE = mapH + 2 * W * C;                                           // [W][C]{A, E}
-    float* next = mapH - lane * CPL * 2 + 4 * W * C + lane * CPL;             // [C]
-    const int group = blockIdx.x / p.split, rank = blockIdx.x - group * p.split;
-    Peers<CPL> peers{next - lane * CPL + C, nullptr, p.split, rank};
-    peers.bars = reinterpret_cast<unsigned long long*>(peers.sets + 2 * kMaxCluster * C * 2);
-    const int b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
+    T* stage = reinterpret_cast<T*>(smem);
+    float* base = reinterpret_cast<float*>(smem + 6 * (size_t)rows * C * sizeof(T));
+    const Maps3<CPL> maps{base + lane * CPL, W};
+    float* next = base + 3 * W * C;
+    Peers<CPL> peers(next + 2 * C, p.split, blockIdx.x % p.split);
+    const int group = blockIdx.x / p.split, b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
     const T* gate = static_cast<const T*>(p.gate) + b * p.gate_b;
     const T* x = static_cast<const T*>(p.x) + b * p.x_b;
     const T* dy = static_cast<const T*>(p.dy) + b * p.dy_b;
@@ -392,7 +523,7 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
     auto issue = [&](int k) {                              // the k-th piece from the end
         if (k < n) {
             T* s = stage + (k & 1) * 3 * rows * C;
-            const int t0 = ((n - 1 - k) * p.split + rank) * rows;
+            const int t0 = ((n - 1 - k) * p.split + peers.rank) * rows;
             stage_rows<T, CPL, ALIGN, S>(s, gate, p.gate_t, t0, rows, d0, p.T, p.D, __int_as_float(0x7f800000));
             stage_rows<T, CPL, ALIGN, S>(s + rows * C, x, p.x_t, t0, rows, d0, p.T, p.D, 0.f);
             stage_rows<T, CPL, ALIGN, S>(s + 2 * rows * C, dy, p.dy_t, t0, rows, d0, p.T, p.D, 0.f);
@@ -404,112 +535,252 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
     read_state<CPL>(p.dlast ? p.dlast + at_state : nullptr, carry, left);
     if (p.split > 1) peers.begin();
     for (int k = 0; k < n; ++k) {
-        const int first = ((n - 1 - k) * p.split + rank) * rows, t0 = first + warp * S;
+        const int first = ((n - 1 - k) * p.split + peers.rank) * rows, t0 = first + warp * S;
         const T* sg = stage + (k & 1) * 3 * rows * C + warp * S * C + lane * CPL;
-        const T* sx = sg + rows * C;
-        const T* sd = sx + rows * C;
+        const T *sx = sg + rows * C, *sd = sx + rows * C;
         // a block's piece begins where the forward pass saved a state
         float hb[CPL];
         read_state<CPL>(first < p.T ? p.states + ((long long)b * p.chunks + first / kSaved) * p.D + d : nullptr, hb, left);
         cp_wait<0>();
         __syncthreads();                                  // the stage is there, and the other one has been read
         issue(k + 1);
-        if (p.split == 1 && k > 0) read_state<CPL>(next, carry, CPL);
-        // E, what e of zero becomes over the steps, is the sum of dy_t times the product of the a up to a_t
         float2 a[N], z[N];
-        float A[CPL], H[CPL], E[CPL];
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) { A[c] = 1.f; H[c] = E[c] = 0.f; }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            gates2(read_pair<T, CPL>(sg, i), a[i], z[i]);
-            run_pair<CPL>(a[i], mul2(z[i], read_pair<T, CPL>(sx, i)), H);
-            const float2 P = scale_pair<CPL>(a[i], A), u = read_pair<T, CPL>(sd, i);
-            if constexpr (CPL == 2) {
-                const float2 r = fma2(P, u, make_float2(E[0], E[1]));
-                E[0] = r.x;
-                E[1] = r.y;
-            } else {
-                E[0] = fmaf(P.y, u.y, fmaf(P.x, u.x, E[0]));
-            }
-        }
-        write_map<CPL>(mapH + warp * 2 * C, A, H);
-        write_map<CPL>(mapE + warp * 2 * C, A, E);
+        float A[CPL], H[CPL], E[CPL], e[CPL];
+        run_backward<T, CPL, N>(sg, sx, sd, a, z, A, H, E);
+        maps.write(warp, A, H, E);
         __syncthreads();
-#pragma unroll 4
-        for (int w = 0; w < warp; ++w) apply_map<CPL>(mapH + w * 2 * C, hb);
-        float e[CPL];
-        if (p.split == 1) {
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) e[c] = carry[c];
-#pragma unroll 4
-            for (int w = W - 1; w > warp; --w) apply_map<CPL>(mapE + w * 2 * C, e);
-            if (warp == 0) {
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) next[c] = carry[c] = fmaf(A[c], e[c], E[c]);
-            }
-        } else {
-            if (warp < p.split) {
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) { A[c] = 1.f; E[c] = 0.f; }
-#pragma unroll 4
-                for (int w = W - 1; w >= 0; --w) join_map<CPL>(mapE + w * 2 * C, A, E);
-                peers.send(k, warp, lane, A, E);
-            }
-            const float* set = peers.receive(k, lane);
-#pragma unroll 4
-            for (int j = p.split - 1; j > rank; --j) apply_map<CPL>(set + j * 2 * C, carry);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) e[c] = carry[c];
-#pragma unroll 4
-            for (int w = W - 1; w > warp; --w) apply_map<CPL>(mapE + w * 2 * C, e);
-#pragma unroll 4
-            for (int j = rank; j >= 0; --j) apply_map<CPL>(set + j * 2 * C, carry);
-            if (peers.lost) {
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) e[c] = carry[c] = __int_as_float(0x7fc00000);
-            }
-        }
-        // dgate's factor (h_{t-1} - x_t) a z of each step, the states run again
-        float2 f[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float2 v = read_pair<T, CPL>(sx, i);
-            float2 before;
-            run_pair<CPL>(a[i], mul2(z[i], v), hb, &before);
-            f[i] = mul2(fma2(v, make_float2(-1.f, -1.f), before), mul2(a[i], z[i]));
-        }
+        join_backward<CPL>(maps, next + lane * CPL, k, warp, lane, A, E, hb, e, carry, peers);
         T *to_g = dgate + (long long)t0 * p.D, *to_x = dx + (long long)t0 * p.D;
         auto sweep = [&](int steps) {
-#pragma unroll
-            for (int i = N - 1; i >= 0; --i) {
-                const float2 u = read_pair<T, CPL>(sd, i);
-                float2 et;                                // e of the pair's steps
-                if constexpr (CPL == 2) {
-                    et = add2(make_float2(e[0], e[1]), u);
-                    const float2 r = mul2(et, a[i]);
-                    e[0] = r.x;
-                    e[1] = r.y;
-                } else {
-                    et.y = e[0] + u.y;
-                    et.x = fmaf(et.y, a[i].y, u.x);
-                    e[0] = et.x * a[i].x;
-                }
-                write_pair<T, CPL, (ALIGN >= 4)>(to_g, p.D, i, mul2(et, f[i]), steps, left);
-                write_pair<T, CPL, (ALIGN >= 4)>(to_x, p.D, i, mul2(et, z[i]), steps, left);
-            }
+            sweep_backward<T, CPL, N>(sx, sd, a, z, hb, e, [&](int i, float2 dg, float2 dv) {
+                write_pair<T, CPL, (ALIGN >= 4)>(to_g, p.D, i, dg, steps, left);
+                write_pair<T, CPL, (ALIGN >= 4)>(to_x, p.D, i, dv, steps, left);
+            });
         };
         if (p.T - t0 >= S) sweep(S);
         else sweep(p.T - t0);
     }
-    if (warp == 0 && rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
+    if (warp == 0 && peers.rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
+    if (p.split > 1) cluster_sync();
+}
+
+// ---- staging by TMA tiles ----------------------------------------------------------------------------------
+struct RecTiles {
+    CUtensorMap gate, x, dy, out0, out1;                  // [B][T][D], a box of a piece's steps and 32 lanes' channels
+};
+__device__ __forceinline__ void load_tile(void* to, const CUtensorMap* m, int d, int t, int b, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     smem_u32(to)),
+                 "l"(m), "r"(d), "r"(t), "r"(b), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void store_tile(const CUtensorMap* m, const void* from, int d, int t, int b) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(m), "r"(smem_u32(from)), "r"(d),
+                 "r"(t), "r"(b)
+                 : "memory");
+}
+constexpr unsigned long long kTileWaitNs = 2000000000ull;
+constexpr int kFwdStages = 3, kBwdStages = 2;
+
+// The warp beside the W computing ones: loads pieces ahead, stores a piece's results when all warps have written them
+// (`written`, an mbarrier for each stage: a warp may be pieces ahead of another one, so a barrier that only counts
+// arrivals would take one piece's for another's) and loads the next piece into their place when the copy has read them.
+template <int STAGES, class Load, class Store>
+__device__ __forceinline__ void move_tiles(int n, int lane, unsigned long long* written, Load&& load, Store&& store) {
+    if (lane == 0) {
+        for (int k = 0; k < STAGES && k < n; ++k) load(k);
+        int stage = 0, parity = 0;
+        for (int k = 0; k < n; ++k) {
+            if (!mbar_wait(written + stage, parity, kTileWaitNs)) break;      // the others find no more tiles and give up
+            store(k);
+            bulk_commit();
+            if (k + STAGES < n) {
+                bulk_wait_read<0>();
+                load(k + STAGES);
+            }
+            if (++stage == STAGES) {
+                stage = 0;
+                parity ^= 1;
+            }
+        }
+        bulk_wait<0>();
+    }
+    __syncwarp();
+}
+// a computing warp's side of it
+__device__ __forceinline__ void results_written(unsigned long long* written, int lane) {
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(written);
+}
+__device__ __forceinline__ void computing_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
+// a pair into the place of the input it was made of
+template <class T, int CPL>
+__device__ __forceinline__ void put_pair(T* at, int i, float2 v) {
+    constexpr int C = 32 * CPL;
+    if constexpr (CPL == 2) {
+        const float2 w[1] = {v};
+        *reinterpret_cast<Pack<T, 2>*>(at + i * C) = pack_pairs<T, 2>(w);
+    } else {
+        at[2 * i * C] = from_f32<T>(v.x);
+        at[(2 * i + 1) * C] = from_f32<T>(v.y);
+    }
+}
+// A tile brings zeros for steps from T on; a gate of +infinity makes them leave the state as it is.  Each warp sees to its own.
+template <class T, int CPL, int S>
+__device__ __forceinline__ void hold_beyond(T* sg, int steps) {
+    constexpr int C = 32 * CPL;
+    for (int s = steps < 0 ? 0 : steps; s < S; ++s)
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) sg[s * C + c] = from_f32<T>(__int_as_float(0x7f800000));
+}
+
+template <class T, int CPL, int S>
+__global__ void __launch_bounds__(kWarpsFwd * 32 + 32, 2) rec_fwd_tiles(const RecArgs p, const __grid_constant__ RecTiles m) {
+    constexpr int C = 32 * CPL, N = S * CPL / 2, W = kWarpsFwd, rows = W * S, TILE = rows * C;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    T* stage = reinterpret_cast<T*>(smem);                                    // [stages][gate, x][rows][C]
+    float* maps = reinterpret_cast<float*>(stage + kFwdStages * 2 * TILE);    // [2][W][C]{A, H}
+    float* next = maps + 4 * W * C;
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(next + 2 * C);
+    Peers<CPL> peers(reinterpret_cast<float*>(full + 2 * kFwdStages), p.split, blockIdx.x % p.split);
+    const int group = blockIdx.x / p.split, b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
+    const int n = (p.T + rows * p.split - 1) / (rows * p.split);
+    unsigned long long* written = full + kFwdStages;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kFwdStages; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(written + s, W);
+        }
+        fence_mbar_init();
+    }
+    if (p.split > 1) peers.begin();
+    else __syncthreads();
+    if (warp == W) {
+        move_tiles<kFwdStages>(
+            n, lane, written,
+            [&](int it) {
+                const int k = it % kFwdStages, t0 = (it * p.split + peers.rank) * rows;
+                mbar_expect_tx(full + k, 2 * TILE * sizeof(T));
+                load_tile(stage + 2 * k * TILE, &m.gate, d0, t0, b, full + k);
+                load_tile(stage + (2 * k + 1) * TILE, &m.x, d0, t0, b, full + k);
+            },
+            [&](int it) {
+                const int t0 = (it * p.split + peers.rank) * rows;
+                if (t0 < p.T) store_tile(&m.out0, stage + (2 * (it % kFwdStages) + 1) * TILE, d0, t0, b);
+            });
+    } else {
+        const long long at_state = (long long)b * p.D + d;
+        float carry[CPL];
+        read_state<CPL>(p.h0 ? p.h0 + at_state : nullptr, carry, left);
+        bool there = true;
+        int k = 0, parity = 0;
+        for (int it = 0; it < n; ++it) {
+            const int t0 = (it * p.split + peers.rank) * rows + warp * S;
+            T* sg = stage + 2 * k * TILE + warp * S * C + lane * CPL;
+            T* sx = sg + TILE;
+            float* map = maps + (it & 1) * 2 * W * C;
+            if (there) there = mbar_wait(full + k, parity, kTileWaitNs);
+            if (p.T - t0 < S) hold_beyond<T, CPL, S>(sg, p.T - t0);
+            float2 h[N], a[N];
+            float H[CPL], A[CPL], in[CPL];
+            run_forward<T, CPL, N>(sg, sx, h, a, A, H);
+            write_map<CPL>(map + (warp * C + lane * CPL) * 2, A, H);
+            computing_sync(W * 32);
+            join_forward<CPL>(map + lane * CPL * 2, next + lane * CPL, it, W, warp, lane, A, H, in, carry, peers);
+            if (!there) in[0] = in[CPL - 1] = carry[0] = carry[CPL - 1] = __int_as_float(0x7fc00000);
+            if (p.states && t0 < p.T && t0 % kSaved == 0)
+                write_state<CPL>(p.states + ((long long)b * p.chunks + t0 / kSaved) * p.D + d, in, left);
+#pragma unroll
+            for (int i = 0; i < N; ++i) put_pair<T, CPL>(sx, i, fma2(a[i], both<CPL>(in), h[i]));
+            results_written(written + k, lane);
+            if (++k == kFwdStages) {
+                k = 0;
+                parity ^= 1;
+            }
+        }
+        if (warp == W - 1 && peers.rank == 0) write_state<CPL>(p.last + at_state, carry, left);
+        __syncwarp();
+    }
+    if (p.split > 1) cluster_sync();                      // no block ends while a peer may still write to it
+}
+
+template <class T, int CPL, int S>
+__global__ void __launch_bounds__(kWarpsBwd * 32 + 32, 1) rec_bwd_tiles(const RecArgs p, const __grid_constant__ RecTiles m) {
+    constexpr int C = 32 * CPL, N = S * CPL / 2, W = kWarpsBwd, rows = W * S, TILE = rows * C;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    T* stage = reinterpret_cast<T*>(smem);                                    // [stages][gate, x, dy][rows][C]
+    float* base = reinterpret_cast<float*>(stage + kBwdStages * 3 * TILE);    // [2][A, H, E][W][C]
+    float* next = base + 6 * W * C;
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(next + 2 * C);
+    Peers<CPL> peers(reinterpret_cast<float*>(full + 2 * kBwdStages), p.split, blockIdx.x % p.split);
+    const int group = blockIdx.x / p.split, b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
+    const int n = (p.T + rows * p.split - 1) / (rows * p.split);
+    unsigned long long* written = full + kBwdStages;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kBwdStages; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(written + s, W);
+        }
+        fence_mbar_init();
+    }
+    if (p.split > 1) peers.begin();
+    else __syncthreads();
+    if (warp == W) {
+        auto first_of = [&](int k) { return ((n - 1 - k) * p.split + peers.rank) * rows; };      // the k-th piece from the end
+        move_tiles<kBwdStages>(
+            n, lane, written,
+            [&](int k) {
+                T* s = stage + 3 * (k & 1) * TILE;
+                const int t0 = first_of(k);
+                mbar_expect_tx(full + (k & 1), 3 * TILE * sizeof(T));
+                load_tile(s, &m.gate, d0, t0, b, full + (k & 1));
+                load_tile(s + TILE, &m.x, d0, t0, b, full + (k & 1));
+                load_tile(s + 2 * TILE, &m.dy, d0, t0, b, full + (k & 1));
+            },
+            [&](int k) {
+                const T* s = stage + 3 * (k & 1) * TILE;
+                const int t0 = first_of(k);
+                if (t0 >= p.T) return;
+                store_tile(&m.out0, s, d0, t0, b);
+                store_tile(&m.out1, s + TILE, d0, t0, b);
+            });
+    } else {
+        const long long at_state = (long long)b * p.D + d;
+        float carry[CPL];
+        read_state<CPL>(p.dlast ? p.dlast + at_state : nullptr, carry, left);
+        bool there = true;
+        for (int k = 0; k < n; ++k) {
+            const int first = ((n - 1 - k) * p.split + peers.rank) * rows, t0 = first + warp * S;
+            T* sg = stage + 3 * (k & 1) * TILE + warp * S * C + lane * CPL;
+            T *sx = sg + TILE, *sd = sx + TILE;
+            const Maps3<CPL> maps{base + (k & 1) * 3 * W * C + lane * CPL, W};
+            float hb[CPL];
+            read_state<CPL>(first < p.T ? p.states + ((long long)b * p.chunks + first / kSaved) * p.D + d : nullptr, hb, left);
+            if (there) there = mbar_wait(full + (k & 1), (k >> 1) & 1, kTileWaitNs);
+            if (p.T - t0 < S) hold_beyond<T, CPL, S>(sg, p.T - t0);
+            float2 a[N], z[N];
+            float A[CPL], H[CPL], E[CPL], e[CPL];
+            run_backward<T, CPL, N>(sg, sx, sd, a, z, A, H, E);
+            maps.write(warp, A, H, E);
+            computing_sync(W * 32);
+            join_backward<CPL>(maps, next + lane * CPL, k, warp, lane, A, E, hb, e, carry, peers);
+            if (!there) e[0] = e[CPL - 1] = hb[0] = hb[CPL - 1] = carry[0] = carry[CPL - 1] = __int_as_float(0x7fc00000);
+            sweep_backward<T, CPL, N>(sx, sd, a, z, hb, e, [&](int i, float2 dg, float2 dv) {
+                put_pair<T, CPL>(sg, i, dg);
+                put_pair<T, CPL>(sx, i, dv);
+            });
+            results_written(written + (k & 1), lane);
+        }
+        if (warp == 0 && peers.rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
+        __syncwarp();
+    }
     if (p.split > 1) cluster_sync();
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
-constexpr int kWarpsFwd = 8, kWarpsBwd = 16, kSteps = 16;     // a whole piece of the backward pass is kSaved steps
-static_assert(kWarpsBwd * kSteps == kSaved && kSaved % kSteps == 0, "pieces begin where states are saved");
-
 bool rec_shape_ok(int64_t B, int64_t T, int D) { return B > 0 && T > 0 && D > 0; }
 constexpr long long kMax32 = (1LL << 31) - 1;
 
@@ -543,6 +814,39 @@ int rec_align(int es, int D, std::initializer_list<const void*> ptrs, std::initi
     return (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : es;
 }
 
+// ---- TMA tiles ----
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+// [B][T][D] with a box of `rows` steps and C channels; false where the strides do not nest (a shared gate, steps ahead of
+// batch items in memory), which the other kernel takes
+template <class T>
+bool make_tiles(CUtensorMap& m, const void* at, long long stride_b, long long stride_t, const RecArgs& a, int rows, int C) {
+    constexpr CUtensorMapDataType type = std::is_same_v<T, float>    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (a.B == 1) stride_b = a.T * stride_t;
+    if (stride_t < a.D || stride_b / a.T < stride_t || stride_b * (long long)sizeof(T) >= 1LL << 40) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.T, (cuuint64_t)a.B};
+    const cuuint64_t strides[2] = {(cuuint64_t)stride_t * sizeof(T), (cuuint64_t)stride_b * sizeof(T)};
+    const cuuint32_t box[3] = {(cuuint32_t)C, (cuuint32_t)rows, 1}, step[3] = {1, 1, 1};
+    return encode_tiled()(&m, type, 3, const_cast<void*>(at), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+constexpr int kTileSteps = 512;      // below, the host's time for the maps is worth more than what they save
+
 template <class T, int CPL, int ALIGN, bool BWD>
 int rec_launch(RecArgs a, cudaStream_t s) {
     constexpr int S = kSteps, MAXW = BWD ? kWarpsBwd : kWarpsFwd;
@@ -558,8 +862,26 @@ int rec_launch(RecArgs a, cudaStream_t s) {
     int split = 1;
     while (2 * split <= kMaxCluster && 2 * split <= pieces && groups * 2 * split <= room) split *= 2;
     a.split = split;
-    const size_t smem = rec_smem<T, CPL>(W, S, BWD ? 3 : 2, BWD ? 2 : 1, split);
     if (groups * split > kMax32) return HFUSE_ERR_TOO_LARGE;
+    const size_t peers = split > 1 ? 2 * (size_t)kMaxCluster * C * 8 + 16 : 0;
+    if constexpr (ALIGN == 16) {
+        RecTiles m;
+        const long long all = (long long)a.T * a.D;
+        constexpr int rows = MAXW * S;
+        bool ok = a.T >= kTileSteps && encode_tiled() && make_tiles<T>(m.gate, a.gate, a.gate_b, a.gate_t, a, rows, C) &&
+                  make_tiles<T>(m.x, a.x, a.x_b, a.x_t, a, rows, C) && make_tiles<T>(m.out0, BWD ? a.dgate : a.y, all, a.D, a, rows, C);
+        if (BWD)
+            ok = ok && make_tiles<T>(m.dy, a.dy, a.dy_b, a.dy_t, a, rows, C) && make_tiles<T>(m.out1, a.dx, all, a.D, a, rows, C);
+        else if (ok)
+            m.dy = m.out1 = m.out0;
+        if (ok) {
+            const size_t smem = (size_t)(BWD ? kBwdStages * 3 : kFwdStages * 2) * rows * C * sizeof(T) + (BWD ? 6 : 4) * (size_t)MAXW * C * 4 +
+                                2 * (size_t)C * 4 + (BWD ? kBwdStages : kFwdStages) * 16 + peers;
+            if constexpr (BWD) return launch_cluster(rec_bwd_tiles<T, CPL, S>, (int)(groups * split), MAXW * 32 + 32, smem, split, s, a, m);
+            else return launch_cluster(rec_fwd_tiles<T, CPL, S>, (int)(groups * split), MAXW * 32 + 32, smem, split, s, a, m);
+        }
+    }
+    const size_t smem = (size_t)(BWD ? 6 : 4) * W * S * C * sizeof(T) + (BWD ? 3 : 2) * (size_t)W * C * 4 + 2 * (size_t)C * 4 + peers;
     if constexpr (BWD) return launch_cluster(rec_bwd<T, CPL, S, ALIGN>, (int)(groups * split), W * 32, smem, split, s, a);
     else return launch_cluster(rec_fwd<T, CPL, S, ALIGN>, (int)(groups * split), W * 32, smem, split, s, a);
 }
