@@ -367,54 +367,28 @@ struct Maps3 {
         }
     }
 };
-// After the barrier behind Maps3::write: hb from the state before the piece to the one before the warp's first step, and e
-// from behind its last step.
+// After the barrier behind Maps3::write.  First what the other blocks wait for: the map of the whole piece.
 template <int CPL>
-__device__ __forceinline__ void join_backward(const Maps3<CPL>& maps, float* next, int k, int warp, int lane, float (&A)[CPL], float (&E)[CPL],
-                                              float (&hb)[CPL], float (&e)[CPL], float (&carry)[CPL], Peers<CPL>& peers) {
-    constexpr int C = 32 * CPL;
-    const int W = maps.W;
+__device__ __forceinline__ void send_backward(const Maps3<CPL>& maps, int k, int warp, int lane, Peers<CPL>& peers) {
+    if (warp >= peers.split || peers.split == 1) return;
+    float A[CPL], E[CPL];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) { A[c] = 1.f; E[c] = 0.f; }
+#pragma unroll 4
+    for (int w = maps.W - 1; w >= 0; --w) {
+        maps.apply(w, 2, E);
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) A[c] *= maps.at[w * maps.C + c];
+    }
+    peers.send(k, warp, lane, A, E);
+}
+// Then, while it is on its way, dgate's factor (h_{t-1} - x_t) a z of each step: the states run again from hb, the one
+// before the piece.
+template <class T, int CPL, int N>
+__device__ __forceinline__ void factors_backward(const Maps3<CPL>& maps, int warp, const T* sx, const float2 (&a)[N], const float2 (&z)[N],
+                                                 float (&hb)[CPL], float2 (&f)[N]) {
 #pragma unroll 4
     for (int w = 0; w < warp; ++w) maps.apply(w, 1, hb);
-    if (peers.split == 1) {
-        if (k > 0) read_state<CPL>(next + (k & 1) * C, carry, CPL);
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) e[c] = carry[c];
-#pragma unroll 4
-        for (int w = W - 1; w > warp; --w) maps.apply(w, 2, e);
-        if (warp == 0) {
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) next[(~k & 1) * C + c] = carry[c] = fmaf(A[c], e[c], E[c]);
-        }
-        return;
-    }
-    if (warp < peers.split) {
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) { A[c] = 1.f; E[c] = 0.f; }
-#pragma unroll 4
-        for (int w = W - 1; w >= 0; --w) {
-            maps.apply(w, 2, E);
-#pragma unroll
-            for (int c = 0; c < CPL; ++c) A[c] *= maps.at[w * C + c];
-        }
-        peers.send(k, warp, lane, A, E);
-    }
-    const float* set = peers.receive(k, lane);
-#pragma unroll 4
-    for (int j = peers.split - 1; j > peers.rank; --j) apply_map<CPL>(set + j * 2 * C, carry);
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) e[c] = carry[c];
-#pragma unroll 4
-    for (int w = W - 1; w > warp; --w) maps.apply(w, 2, e);
-#pragma unroll 4
-    for (int j = peers.rank; j >= 0; --j) apply_map<CPL>(set + j * 2 * C, carry);
-    peers.spoil(e, carry);
-}
-// dgate and dx of the warp's steps, put(i, dgate, dx) for every pair from the last one on
-template <class T, int CPL, int N, class Put>
-__device__ __forceinline__ void sweep_backward(const T* sx, const T* sd, const float2 (&a)[N], const float2 (&z)[N], float (&hb)[CPL], float (&e)[CPL],
-                                               Put&& put) {
-    float2 f[N];                                          // dgate's factor (h_{t-1} - x_t) a z, the states run again
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float2 v = read_pair<T, CPL>(sx, i);
@@ -422,6 +396,38 @@ __device__ __forceinline__ void sweep_backward(const T* sx, const T* sd, const f
         run_pair<CPL>(a[i], mul2(z[i], v), hb, &before);
         f[i] = mul2(fma2(v, make_float2(-1.f, -1.f), before), mul2(a[i], z[i]));
     }
+}
+// e from behind the warp's last step; A and E are the warp's own
+template <int CPL>
+__device__ __forceinline__ void join_backward(const Maps3<CPL>& maps, float* next, int k, int warp, int lane, const float (&A)[CPL],
+                                              const float (&E)[CPL], float (&e)[CPL], float (&carry)[CPL], Peers<CPL>& peers) {
+    constexpr int C = 32 * CPL;
+    if (peers.split == 1) {
+        if (k > 0) read_state<CPL>(next + (k & 1) * C, carry, CPL);
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+#pragma unroll 4
+        for (int w = maps.W - 1; w > warp; --w) maps.apply(w, 2, e);
+        if (warp == 0) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) next[(~k & 1) * C + c] = carry[c] = fmaf(A[c], e[c], E[c]);
+        }
+        return;
+    }
+    const float* set = peers.receive(k, lane);
+#pragma unroll 4
+    for (int j = peers.split - 1; j > peers.rank; --j) apply_map<CPL>(set + j * 2 * C, carry);
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) e[c] = carry[c];
+#pragma unroll 4
+    for (int w = maps.W - 1; w > warp; --w) maps.apply(w, 2, e);
+#pragma unroll 4
+    for (int j = peers.rank; j >= 0; --j) apply_map<CPL>(set + j * 2 * C, carry);
+    peers.spoil(e, carry);
+}
+// dgate and dx of the warp's steps, put(i, dgate, dx) for every pair from the last one on
+template <class T, int CPL, int N, class Put>
+__device__ __forceinline__ void sweep_backward(const T* sd, const float2 (&a)[N], const float2 (&z)[N], const float2 (&f)[N], float (&e)[CPL], Put&& put) {
 #pragma unroll
     for (int i = N - 1; i >= 0; --i) {
         const float2 u = read_pair<T, CPL>(sd, i);
@@ -544,15 +550,17 @@ __global__ void __launch_bounds__(512, 1) rec_bwd(const RecArgs p) {
         cp_wait<0>();
         __syncthreads();                                  // the stage is there, and the other one has been read
         issue(k + 1);
-        float2 a[N], z[N];
+        float2 a[N], z[N], f[N];
         float A[CPL], H[CPL], E[CPL], e[CPL];
         run_backward<T, CPL, N>(sg, sx, sd, a, z, A, H, E);
         maps.write(warp, A, H, E);
         __syncthreads();
-        join_backward<CPL>(maps, next + lane * CPL, k, warp, lane, A, E, hb, e, carry, peers);
+        send_backward<CPL>(maps, k, warp, lane, peers);
+        factors_backward<T, CPL, N>(maps, warp, sx, a, z, hb, f);
+        join_backward<CPL>(maps, next + lane * CPL, k, warp, lane, A, E, e, carry, peers);
         T *to_g = dgate + (long long)t0 * p.D, *to_x = dx + (long long)t0 * p.D;
         auto sweep = [&](int steps) {
-            sweep_backward<T, CPL, N>(sx, sd, a, z, hb, e, [&](int i, float2 dg, float2 dv) {
+            sweep_backward<T, CPL, N>(sd, a, z, f, e, [&](int i, float2 dg, float2 dv) {
                 write_pair<T, CPL, (ALIGN >= 4)>(to_g, p.D, i, dg, steps, left);
                 write_pair<T, CPL, (ALIGN >= 4)>(to_x, p.D, i, dv, steps, left);
             });
@@ -706,77 +714,91 @@ __global__ void __launch_bounds__(kWarpsFwd * 32 + 32, 2) rec_fwd_tiles(const Re
     if (p.split > 1) cluster_sync();                      // no block ends while a peer may still write to it
 }
 
+// The backward pass needs all registers that 16 warps leave each other, so no warp is left to move tiles: the last warp to
+// finish a piece stores it, and loads another one into its place when it has gone through the first half of the next.
 template <class T, int CPL, int S>
-__global__ void __launch_bounds__(kWarpsBwd * 32 + 32, 1) rec_bwd_tiles(const RecArgs p, const __grid_constant__ RecTiles m) {
+__global__ void __launch_bounds__(kWarpsBwd * 32, 1) rec_bwd_tiles(const RecArgs p, const __grid_constant__ RecTiles m) {
     constexpr int C = 32 * CPL, N = S * CPL / 2, W = kWarpsBwd, rows = W * S, TILE = rows * C;
     extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ unsigned finished;                                             // warps, over all pieces
     const int warp = warp_index(), lane = threadIdx.x & 31;
     T* stage = reinterpret_cast<T*>(smem);                                    // [stages][gate, x, dy][rows][C]
     float* base = reinterpret_cast<float*>(stage + kBwdStages * 3 * TILE);    // [2][A, H, E][W][C]
     float* next = base + 6 * W * C;
     unsigned long long* full = reinterpret_cast<unsigned long long*>(next + 2 * C);
-    Peers<CPL> peers(reinterpret_cast<float*>(full + 2 * kBwdStages), p.split, blockIdx.x % p.split);
+    Peers<CPL> peers(reinterpret_cast<float*>(full + kBwdStages), p.split, blockIdx.x % p.split);
     const int group = blockIdx.x / p.split, b = group / p.groups, d0 = (group - b * p.groups) * C, d = d0 + lane * CPL, left = p.D - d;
     const int n = (p.T + rows * p.split - 1) / (rows * p.split);
-    unsigned long long* written = full + kBwdStages;
+    const long long at_state = (long long)b * p.D + d;
+    auto first_of = [&](int k) { return ((n - 1 - k) * p.split + peers.rank) * rows; };      // the k-th piece from the end
+    auto load = [&](int k) {
+        T* s = stage + 3 * (k & 1) * TILE;
+        const int t0 = first_of(k);
+        mbar_expect_tx(full + (k & 1), 3 * TILE * sizeof(T));
+        load_tile(s, &m.gate, d0, t0, b, full + (k & 1));
+        load_tile(s + TILE, &m.x, d0, t0, b, full + (k & 1));
+        load_tile(s + 2 * TILE, &m.dy, d0, t0, b, full + (k & 1));
+    };
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kBwdStages; ++s) {
-            mbar_init(full + s, 1);
-            mbar_init(written + s, W);
-        }
+        finished = 0;
+        for (int s = 0; s < kBwdStages; ++s) mbar_init(full + s, 1);
         fence_mbar_init();
     }
     if (p.split > 1) peers.begin();
     else __syncthreads();
-    if (warp == W) {
-        auto first_of = [&](int k) { return ((n - 1 - k) * p.split + peers.rank) * rows; };      // the k-th piece from the end
-        move_tiles<kBwdStages>(
-            n, lane, written,
-            [&](int k) {
-                T* s = stage + 3 * (k & 1) * TILE;
-                const int t0 = first_of(k);
-                mbar_expect_tx(full + (k & 1), 3 * TILE * sizeof(T));
-                load_tile(s, &m.gate, d0, t0, b, full + (k & 1));
-                load_tile(s + TILE, &m.x, d0, t0, b, full + (k & 1));
-                load_tile(s + 2 * TILE, &m.dy, d0, t0, b, full + (k & 1));
-            },
-            [&](int k) {
-                const T* s = stage + 3 * (k & 1) * TILE;
-                const int t0 = first_of(k);
-                if (t0 >= p.T) return;
-                store_tile(&m.out0, s, d0, t0, b);
-                store_tile(&m.out1, s + TILE, d0, t0, b);
-            });
-    } else {
-        const long long at_state = (long long)b * p.D + d;
-        float carry[CPL];
-        read_state<CPL>(p.dlast ? p.dlast + at_state : nullptr, carry, left);
-        bool there = true;
-        for (int k = 0; k < n; ++k) {
-            const int first = ((n - 1 - k) * p.split + peers.rank) * rows, t0 = first + warp * S;
-            T* sg = stage + 3 * (k & 1) * TILE + warp * S * C + lane * CPL;
-            T *sx = sg + TILE, *sd = sx + TILE;
-            const Maps3<CPL> maps{base + (k & 1) * 3 * W * C + lane * CPL, W};
-            float hb[CPL];
-            read_state<CPL>(first < p.T ? p.states + ((long long)b * p.chunks + first / kSaved) * p.D + d : nullptr, hb, left);
-            if (there) there = mbar_wait(full + (k & 1), (k >> 1) & 1, kTileWaitNs);
-            if (p.T - t0 < S) hold_beyond<T, CPL, S>(sg, p.T - t0);
-            float2 a[N], z[N];
-            float A[CPL], H[CPL], E[CPL], e[CPL];
-            run_backward<T, CPL, N>(sg, sx, sd, a, z, A, H, E);
-            maps.write(warp, A, H, E);
-            computing_sync(W * 32);
-            join_backward<CPL>(maps, next + lane * CPL, k, warp, lane, A, E, hb, e, carry, peers);
-            if (!there) e[0] = e[CPL - 1] = hb[0] = hb[CPL - 1] = carry[0] = carry[CPL - 1] = __int_as_float(0x7fc00000);
-            sweep_backward<T, CPL, N>(sx, sd, a, z, hb, e, [&](int i, float2 dg, float2 dv) {
-                put_pair<T, CPL>(sg, i, dg);
-                put_pair<T, CPL>(sx, i, dv);
-            });
-            results_written(written + (k & 1), lane);
+    if (threadIdx.x == 0)
+        for (int k = 0; k < kBwdStages && k < n; ++k) load(k);
+    float carry[CPL];
+    read_state<CPL>(p.dlast ? p.dlast + at_state : nullptr, carry, left);
+    bool there = true, stored = false;                    // stored: this lane has stored the last piece
+    for (int k = 0; k < n; ++k) {
+        const int first = first_of(k), t0 = first + warp * S;
+        T* sg = stage + 3 * (k & 1) * TILE + warp * S * C + lane * CPL;
+        T *sx = sg + TILE, *sd = sx + TILE;
+        const Maps3<CPL> maps{base + (k & 1) * 3 * W * C + lane * CPL, W};
+        float hb[CPL];
+        read_state<CPL>(first < p.T ? p.states + ((long long)b * p.chunks + first / kSaved) * p.D + d : nullptr, hb, left);
+        if (there) there = mbar_wait(full + (k & 1), (k >> 1) & 1, kTileWaitNs);
+        if (p.T - t0 < S) hold_beyond<T, CPL, S>(sg, p.T - t0);
+        float2 a[N], z[N], f[N];
+        float A[CPL], H[CPL], E[CPL], e[CPL];
+        run_backward<T, CPL, N>(sg, sx, sd, a, z, A, H, E);
+        maps.write(warp, A, H, E);
+        __syncthreads();
+        send_backward<CPL>(maps, k, warp, lane, peers);
+        if (stored) {
+            bulk_wait_read<0>();
+            if (k + 1 < n) load(k + 1);
+            stored = false;
         }
-        if (warp == 0 && peers.rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
+        __syncwarp();
+        factors_backward<T, CPL, N>(maps, warp, sx, a, z, hb, f);
+        join_backward<CPL>(maps, next + lane * CPL, k, warp, lane, A, E, e, carry, peers);
+        if (!there) e[0] = e[CPL - 1] = carry[0] = carry[CPL - 1] = __int_as_float(0x7fc00000);
+        sweep_backward<T, CPL, N>(sd, a, z, f, e, [&](int i, float2 dg, float2 dv) {
+            put_pair<T, CPL>(sg, i, dg);
+            put_pair<T, CPL>(sx, i, dv);
+        });
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            __threadfence_block();
+            // the pieces' counts do not mix: a warp counts the next piece only behind a barrier that all have reached
+            stored = atomicAdd(&finished, 1u) % W == W - 1;
+            if (stored) {
+                __threadfence_block();
+                if (first < p.T) {
+                    store_tile(&m.out0, stage + 3 * (k & 1) * TILE, d0, first, b);
+                    store_tile(&m.out1, stage + (3 * (k & 1) + 1) * TILE, d0, first, b);
+                }
+                bulk_commit();
+            }
+        }
         __syncwarp();
     }
+    if (stored) bulk_wait<0>();
+    if (warp == 0 && peers.rank == 0) write_state<CPL>(p.dh0 + at_state, carry, left);
+    __syncwarp();
     if (p.split > 1) cluster_sync();
 }
 
@@ -876,8 +898,8 @@ int rec_launch(RecArgs a, cudaStream_t s) {
             m.dy = m.out1 = m.out0;
         if (ok) {
             const size_t smem = (size_t)(BWD ? kBwdStages * 3 : kFwdStages * 2) * rows * C * sizeof(T) + (BWD ? 6 : 4) * (size_t)MAXW * C * 4 +
-                                2 * (size_t)C * 4 + (BWD ? kBwdStages : kFwdStages) * 16 + peers;
-            if constexpr (BWD) return launch_cluster(rec_bwd_tiles<T, CPL, S>, (int)(groups * split), MAXW * 32 + 32, smem, split, s, a, m);
+                                2 * (size_t)C * 4 + (BWD ? kBwdStages * 8 : kFwdStages * 16) + peers;
+            if constexpr (BWD) return launch_cluster(rec_bwd_tiles<T, CPL, S>, (int)(groups * split), MAXW * 32, smem, split, s, a, m);
             else return launch_cluster(rec_fwd_tiles<T, CPL, S>, (int)(groups * split), MAXW * 32 + 32, smem, split, s, a, m);
         }
     }
