@@ -184,6 +184,8 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
     return s;
 }
 
+constexpr int kMaxWidth = 1 << 30;       // elements of a row: the kernels step beyond the last one in 32 bits
+
 // ---- host: element types -------------------------------------------------------------------
 inline bool lm_type_ok(int t) { return t == HFUSE_F32 || t == HFUSE_BF16 || t == HFUSE_F16; }
 inline int lm_type_size(int t) { return t == HFUSE_F32 ? 4 : 2; }

@@ -944,6 +944,7 @@ int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype,
                     int weight_dtype, float eps, void* y, float* mean, float* invstd, hfuse_stream_t stream) {
     if (!lm_type_ok(dtype) || (weight_dtype != dtype && weight_dtype != HFUSE_F32)) return HFUSE_ERR_BAD_ARG;
     if (!ln_shape_ok(rows, D, ld_x) || !(eps >= 0.f)) return HFUSE_ERR_BAD_ARG;
+    if (D > kMaxWidth) return HFUSE_ERR_TOO_LARGE;
     if (rows == 0) return HFUSE_OK;
     if (!x || !y || !mean || !invstd) return HFUSE_ERR_BAD_ARG;
     const size_t es = lm_type_size(dtype), ws = lm_type_size(weight_dtype);
@@ -993,6 +994,7 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
                              hfuse_stream_t stream) {
     if (!lm_type_ok(dtype) || (weight_dtype != dtype && weight_dtype != HFUSE_F32)) return HFUSE_ERR_BAD_ARG;
     if (!ln_shape_ok(rows, D, ld_x) || !ln_shape_ok(rows, D, ld_grad_out)) return HFUSE_ERR_BAD_ARG;
+    if (D > kMaxWidth) return HFUSE_ERR_TOO_LARGE;
     if (rows > 0 && (!x || !grad_out || !mean || !invstd)) return HFUSE_ERR_BAD_ARG;
     const bool want_w = grad_weight || grad_bias;
     if (!want_w && (rows == 0 || !grad_in)) return HFUSE_OK;

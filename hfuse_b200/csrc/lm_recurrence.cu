@@ -933,7 +933,7 @@ int hfuse_gated_recurrence(const void* gate, int64_t gate_stride_b, int64_t gate
                            float* states, hfuse_stream_t stream) {
     if (!lm_type_ok(dtype) || !rec_shape_ok(B, T, D) || !gate || !x || !out || !h_last) return HFUSE_ERR_BAD_ARG;
     if (gate_stride_b < 0 || gate_stride_t < 0 || x_stride_b < 0 || x_stride_t < 0) return HFUSE_ERR_BAD_ARG;
-    if (B > kMax32 || T > kMax32 - 65536 || B * D > kMax32) return HFUSE_ERR_TOO_LARGE;
+    if (B > kMax32 || T > kMax32 - 65536 || B * D > kMax32 || D > kMaxWidth) return HFUSE_ERR_TOO_LARGE;
     const int es = lm_type_size(dtype);
     if (!aligned_to(gate, es) || !aligned_to(x, es) || !aligned_to(out, es) || !aligned_to(h0, 4) || !aligned_to(h_last, 4) ||
         !aligned_to(states, 4))
@@ -955,7 +955,7 @@ int hfuse_gated_recurrence_backward(const void* gate, int64_t gate_stride_b, int
         return HFUSE_ERR_BAD_ARG;
     if (gate_stride_b < 0 || gate_stride_t < 0 || x_stride_b < 0 || x_stride_t < 0 || grad_out_stride_b < 0 || grad_out_stride_t < 0)
         return HFUSE_ERR_BAD_ARG;
-    if (B > kMax32 || T > kMax32 - 65536 || B * D > kMax32) return HFUSE_ERR_TOO_LARGE;
+    if (B > kMax32 || T > kMax32 - 65536 || B * D > kMax32 || D > kMaxWidth) return HFUSE_ERR_TOO_LARGE;
     const int es = lm_type_size(dtype);
     if (!aligned_to(gate, es) || !aligned_to(x, es) || !aligned_to(grad_out, es) || !aligned_to(grad_gate, es) ||
         !aligned_to(grad_x, es) || !aligned_to(states, 4) || !aligned_to(grad_h_last, 4) || !aligned_to(grad_h0, 4))

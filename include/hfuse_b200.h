@@ -198,6 +198,7 @@ HFUSE_API int hfuse_maxpool_backward_bn_backward_f32(
  *   - outputs and workspaces must not overlap inputs or each other; a workspace needs no
  *     initialisation and holds nothing between calls; two calls that overlap on the GPU must not
  *     share one;
+ *   - D is at most 2^30; a call that the kernels cannot index returns HFUSE_ERR_TOO_LARGE;
  *   - results do not depend on timing: the same call gives the same bits.
  * ------------------------------------------------------------------------------------- */
 enum { HFUSE_F32 = 0, HFUSE_BF16 = 1, HFUSE_F16 = 2 };

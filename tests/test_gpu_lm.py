@@ -263,7 +263,7 @@ def _check_rec(api, gate, x, dy, h0, dl):
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("B,T,D", [(1, 1, 1), (2, 1, 64), (64, 1, 257), (1, 2, 3), (3, 15, 32), (2, 16, 33), (5, 17, 34), (3, 255, 33),
-                                   (2, 256, 64), (2, 257, 40), (1, 513, 130), (300, 5, 8), (4, 700, 96), (1, 3001, 8), (2, 1500, 66)])
+                                   (2, 256, 64), (2, 257, 40), (1, 513, 130), (300, 5, 8), (4, 700, 96), (1, 3001, 8), (2, 1500, 66), (3, 2049, 64), (1, 4096, 200), (40, 513, 256)])
 def test_gated_recurrence(dev, B, T, D, kind):
     gate, x, dy, h0, dl = _rec_inputs(dev, B, T, D, TYPES[kind], 31)
     _check_rec(ops, gate, x, dy, h0, dl)
@@ -336,3 +336,53 @@ def test_gated_recurrence_refusals(dev, api):
                 lambda: api.gated_recurrence_backward(g, g, st, g[:1]), lambda: api.gated_recurrence_backward(g, g, st, g, st)):
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             bad()
+
+
+# ---- more than 2^31 elements ------------------------------------------------------------------------------------
+def test_layer_norm_beyond_32_bits(dev):
+    rows, D, last = 1_100_000, 2048, 96
+    x, dy = torch.zeros(rows, D, dtype=torch.float16, device=dev), torch.zeros(rows, D, dtype=torch.float16, device=dev)
+    xs, w, b, dys = _norm_inputs(dev, last, D, torch.float16, torch.float16, 18)
+    x[-last:], dy[-last:] = xs, dys
+    y, mean, invstd = ops.layer_norm(x, w, b)
+    for got, exact, bound in zip((y[-last:], mean[-last:], invstd[-last:]), lm.layer_norm(xs, w, b, 1e-5), lm.layer_norm_bound(xs, w, b, 1e-5)):
+        within(got, exact, bound)
+    del y
+    dx, dw, db = ops.layer_norm_backward(x, dy, mean, invstd, w)
+    m, r = mean[-last:], invstd[-last:]
+    # all other rows add zeros
+    for got, exact, bound in zip((dx[-last:], dw, db), lm.layer_norm_backward(xs, dys, m, r, w), lm.layer_norm_backward_bound(xs, dys, m, r, w)):
+        within(got, exact, bound)
+    assert (dx[:64] == 0).all()
+
+
+def test_embedding_beyond_32_bits(dev):
+    V, D = 70_000, 32_768
+    ids = torch.tensor([V - 1, 3, V - 2, V - 1, 66_000] * 60, device=dev)
+    table = torch.zeros(V, D, dtype=torch.float16, device=dev)
+    rows = torch.unique(ids)
+    table[rows] = torch.randn(len(rows), D, generator=_gen(dev, 26), device=dev).half()
+    assert torch.equal(ops.embedding(table, ids[:7], 2.0), (table[ids[:7]].float() * 2).half())
+    del table
+    dy = torch.randn(300, D, generator=_gen(dev, 27), device=dev).half()
+    grad = ops.embedding_backward(dy, ids, V)
+    small = torch.searchsorted(rows, ids)
+    within(grad[rows], lm.embedding_backward(dy, small, len(rows), 1.0), lm.embedding_backward_bound(dy, small, len(rows), 1.0))
+    grad[rows] = 0
+    assert not grad.any()
+
+
+def test_gated_recurrence_beyond_32_bits(dev):
+    B, T, D, pick = 2, 4100, 270_336, slice(270_336 - 64, 270_336)
+    g = _gen(dev, 37)
+    gate, x = (torch.randn(B, T, D, generator=g, device=dev, dtype=torch.float16) for _ in range(2))
+    h, last, states = ops.gated_recurrence(gate, x, None, True)
+    gs, xs = gate[..., pick].contiguous(), x[..., pick].contiguous()
+    exact, bound = lm.gated_recurrence(gs, xs), lm.gated_recurrence_bound(gs, xs)
+    within(h[..., pick], exact[0], bound[0])
+    within(last[:, pick], exact[2], bound[2])
+    dg, dx, dh0 = ops.gated_recurrence_backward(gate, x, states, h)
+    hs = h[..., pick].contiguous()
+    for got, e, o in zip((dg[..., pick], dx[..., pick], dh0[:, pick]), lm.gated_recurrence_backward(gs, xs, None, hs),
+                         lm.gated_recurrence_backward_bound(gs, xs, None, hs)):
+        within(got, e, o)

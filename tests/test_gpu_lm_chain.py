@@ -83,11 +83,12 @@ def test_generation_step_by_step_equals_the_whole_sequence(dev):
     assert (torch.cat(out, 1) - whole).abs().max() <= tol and (h - last).abs().max() <= tol
 
 
-def test_captured_step_replays_on_new_data_beside_another_graph(dev):
+@pytest.mark.parametrize("steps", [60, 290, 700])
+def test_captured_step_replays_on_new_data_beside_another_graph(dev, steps):
     params = _model(dev, 300, 72, torch.bfloat16)
     g = torch.Generator(device=dev).manual_seed(47)
-    ids = [torch.randint(0, 300, (2, 290), generator=g, device=dev) for _ in range(2)]
-    dh = [torch.randn(2, 290, 72, generator=g, device=dev).bfloat16() for _ in range(2)]
+    ids = [torch.randint(0, 300, (2, steps), generator=g, device=dev) for _ in range(2)]
+    dh = [torch.randn(2, steps, 72, generator=g, device=dev).bfloat16() for _ in range(2)]
     want = [[t.clone() for t in _step(i, d, *params)] for i, d in zip(ids, dh)]
     other = [[t.clone() for t in _step(i.flip(0), d, *params)] for i, d in zip(ids, dh)]
     slots, graphs, outs, streams = [], [], [], []

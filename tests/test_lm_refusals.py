@@ -36,7 +36,9 @@ def _recb(g=P, gb=8, gt=8, x=P, xb=8, xt=8, st=P, dy=P, yb=8, yt=8, dl=None, B=1
     (_ln, dict(x=None), BAD), (_ln, dict(y=None), BAD), (_ln, dict(m=None), BAD), (_ln, dict(r=None), BAD), (_ln, dict(D=0), BAD),
     (_ln, dict(rows=-1), BAD), (_ln, dict(ld=7), BAD), (_ln, dict(t=3), BAD), (_ln, dict(t=0, wt=1), BAD), (_ln, dict(t=1, wt=2), BAD),
     (_ln, dict(eps=-1.0), BAD), (_ln, dict(eps=float("nan")), BAD), (_ln, dict(x=P + 2), ALIGN), (_ln, dict(w=P + 1, t=1, wt=1), ALIGN),
-    (_ln, dict(m=P + 2), ALIGN), (_ln, dict(rows=0, x=None), 0),
+    (_ln, dict(m=P + 2), ALIGN), (_ln, dict(rows=0, x=None), 0), (_ln, dict(D=(1 << 30) + 1, ld=1 << 31), LARGE),
+    (_lnb, dict(D=(1 << 30) + 1, ldx=1 << 31, ldy=1 << 31), LARGE), (_emb, dict(D=(1 << 30) + 1), LARGE), (_embb, dict(D=(1 << 30) + 1), LARGE),
+    (_rec, dict(D=(1 << 30) + 1), LARGE), (_recb, dict(D=(1 << 30) + 1), LARGE),
     (_lnb, dict(x=None), BAD), (_lnb, dict(dy=None), BAD), (_lnb, dict(m=None), BAD), (_lnb, dict(ldx=7), BAD), (_lnb, dict(ldy=7), BAD),
     (_lnb, dict(D=-1), BAD), (_lnb, dict(t=5), BAD), (_lnb, dict(wt=1), BAD), (_lnb, dict(ws=None), WORK), (_lnb, dict(nb=8), WORK),
     (_lnb, dict(dx=P + 2), ALIGN), (_lnb, dict(ws=P + 8), ALIGN),
