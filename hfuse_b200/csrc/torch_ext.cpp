@@ -277,6 +277,7 @@ const float* opt_f32(OptTensor t) { return t ? t->data_ptr<float>() : nullptr; }
 // elements between two rows (all dimensions but the last, which must follow each other evenly)
 int64_t row_stride(const Tensor& t, const char* what) {
     int64_t ld = -1, span = 0;
+    if (t.numel() == 0) return t.size(-1);
     for (int64_t d = t.dim() - 2; d >= 0; --d) {
         if (t.size(d) == 1) continue;
         if (ld < 0) ld = t.stride(d);

@@ -349,6 +349,8 @@ def _contiguous(x, name):
 def _row_stride(x, name):
     """Elements between two rows (all dimensions but the last one, which must follow each other evenly)."""
     ld, span = None, None
+    if x.numel() == 0:
+        return x.shape[-1]
     for d in range(x.dim() - 2, -1, -1):
         if x.shape[d] == 1:
             continue

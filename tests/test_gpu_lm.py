@@ -134,6 +134,15 @@ def test_layer_norm_of_no_rows(dev, api):
     assert dx.shape == (0, 16) and (dw == 0).all() and (db == 0).all()
 
 
+@pytest.mark.parametrize("shape", [(5, 0, 16), (0, 5, 16), (2, 0, 3, 16)])
+def test_layer_norm_of_an_empty_batch(dev, api, shape):
+    x, w = torch.empty(shape, device=dev), torch.ones(16, device=dev)
+    y, mean, invstd = api.layer_norm(x, w, w)
+    assert y.shape == x.shape and mean.shape == invstd.shape == x.shape[:-1]
+    dx, dw, db = api.layer_norm_backward(x, x, mean, invstd, w)
+    assert dx.shape == x.shape and (dw == 0).all() and (db == 0).all()
+
+
 def test_layer_norm_shapes_and_refusals(dev, api):
     x = torch.randn(2, 3, 5, 16, device=dev)
     y, mean, _ = api.layer_norm(x)
