@@ -31,6 +31,7 @@ struct LnFwdArgs {
     int lanes;               // short rows: threads that share a row
     int team, stages;        // rows: warps that share a row, buffers of each team
     int buf, wbytes;         // bytes of a row buffer and of the weights in shared memory
+    int period;              // rows: see Cut
 };
 
 struct LnBwdArgs {
@@ -42,6 +43,7 @@ struct LnBwdArgs {
     int D, slices;
     float inv_d;
     int lanes, stages, buf;
+    int period;              // rows: see Cut
 };
 
 // ---- short rows: NV accesses of EV elements in the registers of each of the 2^k <= 32 lanes that share a row ---------
@@ -291,6 +293,30 @@ __device__ __forceinline__ void patch_row(unsigned char* buf, const T* base, lon
     }
     fence_proxy_async_shared();        // a later copy may write there
 }
+// the 16-byte boundary's distance from row r, in bytes; the low bits of a product need no wide multiplication
+template <class T>
+__device__ __forceinline__ int shift_of(const T* base, long long ld, long long r) {
+    return (int)(((unsigned)reinterpret_cast<uintptr_t>(base) + (unsigned)r * ((unsigned)ld * (unsigned)sizeof(T))) & 15u);
+}
+// Rows of a width that is no multiple of 16 bytes.  Where all tensors' rows begin equally far behind a 16-byte boundary, that
+// distance comes back after `period` rows (8 for an odd number of 16-bit elements), so a team that takes every period-th row
+// has one distance, and its threads the same columns in each of its rows: `packs` whole 16-byte accesses from element
+// `lead` on, and up to 14 elements before and behind them, one to a lane of the team's first warp.  16384 rows of 2047 16-bit
+// elements take 35 us forward and 57 backward (of 2048: 25 and 47); as single elements they took 58 and 76.
+struct Cut {
+    int lead, packs, edges;       // edges: elements before and behind
+    int column;                   // this thread's one, or -1
+};
+template <bool PHASED, int EV, class T>
+__device__ __forceinline__ Cut cut_rows(const T* x, long long ld, int D, int first, int at) {
+    if constexpr (!PHASED) return {0, D / EV, 0, -1};
+    const int lead = (EV - shift_of(x, ld, first) / (int)sizeof(T)) & (EV - 1), packs = (D - lead) / EV, edges = D - packs * EV;
+    return {lead, packs, edges, at < lead ? at : at < edges ? at + packs * EV : -1};
+}
+template <class W>
+__device__ __forceinline__ float weight_of(const void* w, int c, float none) {
+    return w ? to_f32(static_cast<const W*>(w)[c]) : none;
+}
 constexpr unsigned long long kRowWaitNs = 2000000000ull;
 
 // the warps of a team meet at their own named barrier
@@ -319,11 +345,6 @@ template <class T, int EV, int NV>
 __device__ __forceinline__ void places(int (&place)[NV], int at, int lanes, int packs) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) place[k] = min(at + k * lanes, packs - 1) * EV * (int)sizeof(T);
-}
-// the 16-byte boundary's distance from row r, in bytes; the low bits of a product need no wide multiplication
-template <class T>
-__device__ __forceinline__ int shift_of(const T* base, long long ld, long long r) {
-    return (int)(((unsigned)reinterpret_cast<uintptr_t>(base) + (unsigned)r * ((unsigned)ld * (unsigned)sizeof(T))) & 15u);
 }
 // which of a pair's elements exist
 template <int EV>
@@ -357,28 +378,51 @@ __device__ __forceinline__ void weight_pairs(const float* w, int p, int packs, f
     }
 }
 
-template <class T, class W, int EV, int NV>
+template <class T, class W, int EV, int NV, bool PHASED>
 __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int VALUES = NV * EV / 2;
     const T* x = static_cast<const T*>(a.x);
     const int M = a.team, lane = threadIdx.x & 31, warp = warp_index(), warps = blockDim.x >> 5, teams = warps / M;
-    const int team = warp / M, part = warp - team * M, lanes = 32 * M, at = part * 32 + lane, packs = a.D / EV;
+    const int team = warp / M, part = warp - team * M, lanes = 32 * M, at = part * 32 + lane;
+    const int period = PHASED ? a.period : 1, first = blockIdx.x & (period - 1);                // of the block's rows
+    const Cut cut = cut_rows<PHASED, EV>(x, a.ldx, a.D, first, at);
+    const int packs = cut.packs;
     float* sw = reinterpret_cast<float*>(smem);
     float* sb = reinterpret_cast<float*>(smem + a.wbytes);
     unsigned char* ring = smem + 2 * a.wbytes + (size_t)team * a.stages * a.buf;
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + 2 * a.wbytes + (size_t)teams * a.stages * a.buf) + team * a.stages;
     float2* moments = reinterpret_cast<float2*>(smem + 2 * a.wbytes + (size_t)teams * a.stages * (a.buf + 8));    // [2][warps]
-    const long long step = (long long)gridDim.x * teams;
-    long long r = (long long)blockIdx.x * teams + team;
+    const long long step = (long long)period * teams * (((int)gridDim.x - first + period - 1) / period);
+    long long r = first + (long long)period * (blockIdx.x / period * teams + team);
     const bool lead = part == 0 && lane == 0;
+    auto fetch = [&](long long row, int s) {
+        if constexpr (PHASED) {
+            mbar_expect_tx(bars + s, (uint32_t)packs * 16);
+            bulk_load(ring + (size_t)s * a.buf, x + row * a.ldx + cut.lead, (uint32_t)packs * 16, bars + s);
+        } else {
+            fetch_row(ring + (size_t)s * a.buf, bars + s, x, a.ldx, a.rows, a.D, row);
+        }
+    };
     if (lead) {
         for (int s = 0; s < a.stages; ++s) mbar_init(bars + s, 1);
         fence_mbar_init();
         for (int s = 0; s < a.stages; ++s)
-            if (r + s * step < a.rows) fetch_row(ring + (size_t)s * a.buf, bars + s, x, a.ldx, a.rows, a.D, r + s * step);
+            if (r + s * step < a.rows) fetch(r + s * step, s);
     }
-    for (int p = threadIdx.x; p < packs; p += blockDim.x) {
+    // the thread's single element, a row ahead
+    const T* edge_at = x + r * a.ldx + max(cut.column, 0);
+    float edge_w = 0.f, edge_b = 0.f, edge = 0.f, edge_next = 0.f;
+    if (PHASED && cut.column >= 0) {
+        edge_w = weight_of<W>(a.w, cut.column, 1.f);
+        edge_b = weight_of<W>(a.b, cut.column, 0.f);
+        if (r < a.rows) edge_next = to_f32(*edge_at);
+    }
+    for (int i = threadIdx.x; PHASED && i < packs * EV; i += blockDim.x) {
+        sw[weight_at<EV>(i, packs)] = weight_of<W>(a.w, cut.lead + i, 1.f);
+        sb[weight_at<EV>(i, packs)] = weight_of<W>(a.b, cut.lead + i, 0.f);
+    }
+    for (int p = threadIdx.x; !PHASED && p < packs; p += blockDim.x) {
         float2 w[kPairs<EV>], b[kPairs<EV>];
         weights_of<W, EV>(static_cast<const W*>(a.w), p, w, 1.f);
         weights_of<W, EV>(static_cast<const W*>(a.b), p, b, 0.f);
@@ -394,7 +438,7 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
         int n = 0;
 #pragma unroll
         for (int k = 0; k < NV; ++k) n += min(max(packs - k * lanes - 32 * lane, 0), 32);
-        count = (float)(n * EV);
+        count = (float)(n * EV + (lane == 0 ? cut.edges : 0));
         inv_count = n ? 1.f / count : 0.f;
     }
     const float mine = M > 1 ? __shfl_sync(0xffffffffu, inv_count, part) : a.inv_d;
@@ -415,6 +459,12 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
             }
         }
         float2 f[VALUES], s2 = make_float2(0.f, 0.f), q2 = s2;
+        if constexpr (PHASED) {
+            edge = edge_next;
+            s2.x = edge;
+            edge_at += step * a.ldx;
+            if (cut.column >= 0 && r + step < a.rows) edge_next = to_f32(*edge_at);
+        }
         {
             Team<T, EV, NV> row;
             row.read(smem_u32(buf) + shift, place);
@@ -431,6 +481,10 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
             }
         }
         const float s = warp_sum(s2.x + s2.y), mid = s * mine;                   // the mean of the warp's part
+        if constexpr (PHASED) {
+            edge = cut.column >= 0 ? edge - mid : 0.f;
+            q2.x = edge * edge;
+        }
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
             f[i] = add2(f[i], make_float2(-mid, -mid));
@@ -457,7 +511,7 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
             q = few_sum(fmaf(count * d, d, m.y), M);
         }
         // the whole team has read the buffer
-        if (lead && r + a.stages * step < a.rows) fetch_row(buf, bars + stage, x, a.ldx, a.rows, a.D, r + a.stages * step);
+        if (lead && r + a.stages * step < a.rows) fetch(r + a.stages * step, stage);
         if (++stage == a.stages) {
             stage = 0;
             parity ^= 1;
@@ -466,7 +520,8 @@ __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
         if (!there) mu = is = __int_as_float(0x7fc00000);
         // f is relative to the mean of the warp's part: y = (f + (mid - mu)) is w + b
         const float2 is2 = make_float2(is, is), move = make_float2((mid - mu) * is, (mid - mu) * is);
-        T* y = static_cast<T*>(a.y) + r * a.D;
+        T* y = static_cast<T*>(a.y) + r * a.D + cut.lead;
+        if (PHASED && cut.column >= 0) y[cut.column - cut.lead] = from_f32<T>(fmaf(fmaf(edge, is, move.x), edge_w, edge_b));
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int p = at + k * lanes;
@@ -506,7 +561,7 @@ __device__ __forceinline__ float warp_sum4(float a, float b, float c, float d, i
 
 // Teams of warps take two rows at a time, [team][stage][x, dy][row] buffers; the block's teams add up their dw and db in
 // the same memory at the end.
-template <class T, class W, int EV, int NV>
+template <class T, class W, int EV, int NV, bool PHASED>
 __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int VALUES = NV * EV / 2;
@@ -514,7 +569,10 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     const T* dy = static_cast<const T*>(a.dy);
     const W* w = static_cast<const W*>(a.w);
     const int lanes = a.lanes, warps = lanes >> 5, lane = threadIdx.x & 31, team = warp_index() / warps, warp = warp_index() - team * warps;
-    const int teams = blockDim.x / lanes, at = warp * 32 + lane, packs = a.D / EV;
+    const int teams = blockDim.x / lanes, at = warp * 32 + lane;
+    const int period = PHASED ? a.period : 1, number = blockIdx.x * teams + team, first = number & (period - 1);
+    const Cut cut = cut_rows<PHASED, EV>(x, a.ldx, a.D, first, at);
+    const int packs = cut.packs;
     unsigned char* ring = smem + (size_t)team * a.stages * 4 * a.buf;
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)teams * a.stages * 4 * a.buf) + team * 2;
     float* sums = reinterpret_cast<float*>(smem + (size_t)teams * (a.stages * 4 * (size_t)a.buf + 16)) + team * 8 * warps;   // [2][warps][4]
@@ -525,32 +583,55 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             t.v[k] = {};
-            if (w && at + k * lanes < packs) t.v[k] = load_cached<W, EV>(w + (at + k * lanes) * EV);
+            if (!PHASED && w && at + k * lanes < packs) t.v[k] = load_cached<W, EV>(w + (at + k * lanes) * EV);
         }
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
             bool ex, ey;
             exists<EV>(i, at, lanes, packs, ex, ey);
             kw[i] = w ? t.get(i) : make_float2(ex ? 1.f : 0.f, ey ? 1.f : 0.f);
+            if (PHASED && w && ex) {
+                const int c = cut.lead + (at + i / (EV / 2) * lanes) * EV + 2 * (i % (EV / 2));
+                kw[i] = make_float2(to_f32(w[c]), to_f32(w[c + 1]));
+            }
             dw[i] = db[i] = make_float2(0.f, 0.f);
         }
     }
     int place[NV];
     places<T, EV, NV>(place, at, lanes, packs);
-    // a pair of rows; lanes 0 to 3 of the team's first warp fetch one row each
-    const long long step = 2LL * gridDim.x * teams;
+    // the thread's single elements of the next two rows
+    float edge_w = 0.f, edge_dw = 0.f, edge_db = 0.f, ex[2] = {0.f, 0.f}, ed[2] = {0.f, 0.f};
+    if (PHASED && cut.column >= 0) edge_w = weight_of<W>(w, cut.column, 1.f);
+    auto edges = [&](long long r) {
+        if (PHASED && cut.column >= 0) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const long long row = r + g * period;
+                if (row >= a.rows) continue;
+                ex[g] = to_f32(x[row * a.ldx + cut.column]);
+                ed[g] = to_f32(dy[row * a.lddy + cut.column]);
+            }
+        }
+    };
+    // a pair of rows, r and r + period; lanes 0 to 3 of the team's first warp fetch one row each
+    const long long step = 2LL * period * (((int)gridDim.x * teams - first + period - 1) / period);
     auto fetch = [&](long long r, int s) {
         if (warp == 0 && lane < 4) {
-            const long long row = r + (lane & 1);
+            const long long row = r + (lane & 1) * period;
             unsigned char* buf = ring + (size_t)(4 * s + lane) * a.buf;
-            if (row >= a.rows) mbar_arrive(bars + s);
+            if (row >= a.rows) {
+                mbar_arrive(bars + s);
+            } else if constexpr (PHASED) {
+                mbar_expect_tx(bars + s, (uint32_t)packs * 16);
+                bulk_load(buf, (lane < 2 ? x + row * a.ldx : dy + row * a.lddy) + cut.lead, (uint32_t)packs * 16, bars + s);
+            }
             else if (lane < 2) fetch_row(buf, bars + s, x, a.ldx, a.rows, a.D, row);
             else fetch_row(buf, bars + s, dy, a.lddy, a.rows, a.D, row);
         }
     };
     // mean and invstd of a pair of rows in lanes 0 to 3
     auto stats = [&](long long r) {
-        const long long row = r + (lane & 1);
+        const long long row = r + (lane & 1) * period;
         return lane < 4 && row < a.rows ? __ldg((lane < 2 ? a.mean : a.invstd) + row) : 0.f;
     };
     if (at == 0) {
@@ -560,17 +641,18 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     }
     team_sync(team, warps);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the sums' last step waits for this grid's end
-    long long r = 2LL * ((long long)blockIdx.x * teams + team);
+    long long r = first + 2LL * period * (number / period);
     for (int s = 0; s < a.stages; ++s)
         if (r + s * step < a.rows) fetch(r + s * step, s);
     float now = stats(r), next = 0.f;
+    edges(r);
     int stage = 0, parity = 0;
     for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
         next = stats(r + step);
         unsigned char* buf = ring + (size_t)4 * stage * a.buf;
         const bool there = mbar_wait(bars + stage, parity, kRowWaitNs);
         const uint32_t at_buf = smem_u32(buf);
-        const int two = r + 1 < a.rows ? 2 : 1;
+        const int two = r + period < a.rows ? 2 : 1;
         int shift[4] = {0, 0, 0, 0};
         if constexpr (EV == 1) {
             bool lacks = false;
@@ -589,12 +671,22 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
             if (lacks) team_sync(team, warps);
         }
         float2 s[2], d[2];
+        float exh[2], egw[2];                              // of the single elements
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             s[g] = d[g] = make_float2(0.f, 0.f);
+            exh[g] = egw[g] = 0.f;
             if (g >= two) continue;
             const float mu = __shfl_sync(0xffffffffu, now, g), is = __shfl_sync(0xffffffffu, now, 2 + g);
             const float2 is2 = make_float2(is, is), off = make_float2(-mu, -mu);
+            if (PHASED && cut.column >= 0) {
+                exh[g] = (ex[g] - mu) * is;
+                egw[g] = ed[g] * edge_w;
+                edge_dw = fmaf(ed[g], exh[g], edge_dw);
+                edge_db += ed[g];
+                s[g].x = egw[g];
+                d[g].x = egw[g] * exh[g];
+            }
             Team<T, EV, NV> vx, vd;
             vx.read(at_buf + g * a.buf + shift[g], place);
             vd.read(at_buf + (2 + g) * a.buf + shift[2 + g], place);
@@ -607,6 +699,7 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
                 d[g] = fma2(gw, xh, d[g]);
             }
         }
+        edges(r + step);
         const float t4 = warp_sum4(s[0].x + s[0].y, d[0].x + d[0].y, s[1].x + s[1].y, d[1].x + d[1].y, lane);
         float* set = sums + turn * warps * 4;
         if ((lane & 7) == 0) set[warp * 4 + (lane >> 3)] = t4;
@@ -622,6 +715,7 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
             total = __int_as_float(0x7fc00000);
 #pragma unroll
             for (int i = 0; i < VALUES; ++i) dw[i] = db[i] = make_float2(total, total);
+            edge_dw = edge_db = total;
         }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -632,7 +726,8 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
             Team<T, EV, NV> vx, vd;
             vx.read(at_buf + g * a.buf + shift[g], place);
             vd.read(at_buf + (2 + g) * a.buf + shift[2 + g], place);
-            T* dx = static_cast<T*>(a.dx) + (r + g) * a.D;
+            T* dx = static_cast<T*>(a.dx) + (r + g * period) * a.D + cut.lead;
+            if (PHASED && cut.column >= 0) dx[cut.column - cut.lead] = from_f32<T>(is * fmaf(exh[g], md, egw[g] + ms));
             float2 o[VALUES];
 #pragma unroll
             for (int i = 0; i < VALUES; ++i) {
@@ -665,12 +760,16 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     __syncthreads();
     float* all = reinterpret_cast<float*>(smem);
     auto put = [&](float* to) {
+        if (PHASED && cut.column >= 0) {
+            to[cut.column] = edge_dw;
+            to[a.D + cut.column] = edge_db;
+        }
 #pragma unroll
         for (int k = 0; k < NV; ++k)
             if (at + k * lanes < packs) {
 #pragma unroll
                 for (int j = 0; j < EV; ++j) {
-                    const int c = (at + k * lanes) * EV + j, i = (k * EV + j) / 2;
+                    const int c = cut.lead + (at + k * lanes) * EV + j, i = (k * EV + j) / 2;
                     to[c] = (k * EV + j) & 1 ? dw[i].y : dw[i].x;
                     to[a.D + c] = (k * EV + j) & 1 ? db[i].y : db[i].x;
                 }
@@ -885,7 +984,7 @@ int ln_fwd_short_launch(LnFwdArgs a, int sms, cudaStream_t s) {
 }
 
 // One block of up to 16 warps to an SM; as many teams as there are rows for, as many buffers as fit (up to 4).
-template <class T, class W, int EV, int NV>
+template <class T, class W, int EV, int NV, bool PHASED = false>
 int ln_fwd_rows_launch(LnFwdArgs a, int team, int sms, cudaStream_t s) {
     const long long per_sm = (a.rows + sms - 1) / sms;
     int teams = 16 / team;
@@ -898,7 +997,9 @@ int ln_fwd_rows_launch(LnFwdArgs a, int team, int sms, cudaStream_t s) {
     a.stages = (int)(room > 4 ? 4 : room);
     const size_t smem = 2 * (size_t)a.wbytes + (size_t)teams * a.stages * (a.buf + 8) + 2 * (size_t)teams * team * sizeof(float2);
     const long long want = (a.rows + teams - 1) / teams;
-    return launch_kernel(ln_fwd_rows<T, W, EV, NV>, (int)(want < sms ? want : sms), teams * team * 32, smem, s, false, a);
+    int grid = (int)(want < sms ? want : sms);
+    if (PHASED && grid < a.period) grid = a.period;          // each distance has a block
+    return launch_kernel(ln_fwd_rows<T, W, EV, NV, PHASED>, grid, teams * team * 32, smem, s, false, a);
 }
 
 template <class T, class W, int EV, int NV>
@@ -916,9 +1017,9 @@ int ln_bwd_short_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
 
 // Teams of as many warps as the row's columns need, 16 columns to a thread: up to 16 warps and as many teams to a block as
 // fit with two stages each (one team with one stage for the longest rows).
-template <class T, class W, int EV, int NV>
+template <class T, class W, int EV, int NV, bool PHASED = false>
 int ln_bwd_rows_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
-    auto kern = ln_bwd_rows<T, W, EV, NV>;
+    auto kern = ln_bwd_rows<T, W, EV, NV, PHASED>;
     a.lanes = (int)((a.D / EV + 32 * NV - 1) / (32 * NV) * 32);
     a.buf = (int)((a.D * sizeof(T) + 15) / 16 * 16 + (EV == 1 ? 16 : 0));
     a.stages = 8 * (size_t)a.buf <= kRowSmem ? 2 : 1;
@@ -931,9 +1032,20 @@ int ln_bwd_rows_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
     long long most = (long long)sms * resident_blocks((const void*)kern, teams * a.lanes, smem);
     most = most < kMaxParts ? most : kMaxParts;
     a.slices = (int)(want < most ? want : most);
+    if (PHASED && a.slices * teams < a.period) a.slices = (a.period + teams - 1) / teams;      // each distance has a team
     return launch_kernel(kern, a.slices, teams * a.lanes, smem, s, false, a);
 }
 
+// rows at p begin as far behind a 16-byte boundary as those of x [..][D] without gaps
+bool rows_alike(const void* x, const void* p, int64_t ld, int D, size_t es) {
+    return ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0 && (ld - D) * (int64_t)es % 16 == 0;
+}
+// rows after which that distance comes back
+int rows_period(int D, size_t es) {
+    int n = 1;
+    while (n * (D * es % 16) % 16 != 0) n *= 2;
+    return n;
+}
 bool ln_shape_ok(int64_t rows, int D, int64_t ld) { return rows >= 0 && D > 0 && (rows <= 1 || ld >= D); }
 
 }  // namespace
@@ -959,6 +1071,8 @@ int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype,
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = aligned_to(x, 16) && aligned_to(y, 16) && aligned_to(weight, 16) && aligned_to(bias, 16) &&
                       D * es % 16 == 0 && ld_x * es % 16 == 0;
+    const bool phased = !wide && rows_alike(x, x, ld_x, D, es) && rows_alike(x, y, D, D, es);
+    a.period = rows_period(D, es);
     return by_types(dtype, weight_dtype, [&](auto t, auto w) {
         using T = typename decltype(t)::type;
         using W = typename decltype(w)::type;
@@ -971,8 +1085,11 @@ int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype,
         if (!wide && packs <= 64) return ln_fwd_short_launch<T, W, 1, 2>(a, f.sms, s);
         // rows that fit shared memory beside their weights.  Few rows are spread over more warps each.
         const bool few = rows < 4LL * f.sms;
-        auto team = [&](int nv) { return (int)((packs + 32LL * nv - 1) / (32LL * nv)); };
+        auto team = [&](int nv) { return (int)(((phased ? D / EV : packs) + 32LL * nv - 1) / (32LL * nv)); };
         if (8 * (size_t)D + D * es + 64 <= kRowSmem) {
+            if (phased && D / EV <= 32 * 4 * 16 && (few || D / EV <= 32 * 4))
+                return ln_fwd_rows_launch<T, W, EV, 4, true>(a, team(4), f.sms, s);
+            if (phased && D / EV <= 32 * 8 * 16) return ln_fwd_rows_launch<T, W, EV, 8, true>(a, team(8), f.sms, s);
             if (wide && packs <= 32 * 4 * 16 && (few || packs <= 32 * 4)) return ln_fwd_rows_launch<T, W, EV, 4>(a, team(4), f.sms, s);
             if (wide && packs <= 32 * 8 * 16) return ln_fwd_rows_launch<T, W, EV, 8>(a, team(8), f.sms, s);
             if (!wide && packs <= 32 * 8 * 16 && (few || packs <= 32 * 8)) return ln_fwd_rows_launch<T, W, 1, 8>(a, team(8), f.sms, s);
@@ -1015,6 +1132,8 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
     a.slices = slices; a.slice_rows = (rows + slices - 1) / slices;
     const bool wide = aligned_to(x, 16) && aligned_to(grad_out, 16) && aligned_to(grad_in, 16) && aligned_to(weight, 16) &&
                       D * es % 16 == 0 && ld_x * es % 16 == 0 && ld_grad_out * es % 16 == 0;
+    const bool phased = rows_alike(x, x, ld_x, D, es) && rows_alike(x, grad_out, ld_grad_out, D, es) && (!grad_in || rows_alike(x, grad_in, D, D, es));
+    a.period = rows_period(D, es);
     return by_types(dtype, weight_dtype, [&](auto t, auto w) {
         using T = typename decltype(t)::type;
         using W = typename decltype(w)::type;
@@ -1028,7 +1147,8 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
             rc = wide ? packs <= 32 ? ln_bwd_short_launch<T, W, EV, 1>(a, f.sms, s) : ln_bwd_short_launch<T, W, EV, 2>(a, f.sms, s)
                       : packs <= 32 ? ln_bwd_short_launch<T, W, 1, 1>(a, f.sms, s) : ln_bwd_short_launch<T, W, 1, 2>(a, f.sms, s);
         } else if (rows > 0 && D <= 16 * 512) {
-            rc = wide ? ln_bwd_rows_launch<T, W, EV, NV>(a, f.sms, s)
+            rc = wide           ? ln_bwd_rows_launch<T, W, EV, NV>(a, f.sms, s)
+                 : phased       ? ln_bwd_rows_launch<T, W, EV, NV, true>(a, f.sms, s)
                  : D <= 8 * 512 ? ln_bwd_rows_launch<T, W, 1, 8>(a, f.sms, s) : ln_bwd_rows_launch<T, W, 1, 16>(a, f.sms, s);
         } else {
             if (grad_in && rows > 0) {

@@ -126,6 +126,48 @@ def test_layer_norm_keeps_a_bad_row_to_itself(dev):
     assert torch.equal(dx[keep], ref[0][keep]) and dx[rows].isnan().all() and torch.equal(db, ref[2])
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [1001, 250, 333])
+def test_layer_norm_keeps_bad_rows_to_themselves_where_rows_share_accesses(dev, D, kind):
+    x, w, b, dy = _norm_inputs(dev, 1500, D, TYPES[kind], torch.float32, 29)
+    ref = _check_norm(ops, x, w, b, dy)
+    rows = torch.arange(3, 1500, 7, device=dev)
+    bx, bd, keep = x.clone(), dy.clone(), torch.ones(1500, dtype=torch.bool, device=dev)
+    keep[rows] = False
+    bx[rows], bd[rows] = float("inf"), float("nan")
+    y, mean, invstd = ops.layer_norm(bx, w, b)
+    assert torch.equal(y[keep], ref[0][keep]) and torch.equal(mean[keep], ref[1][keep]) and y[rows].isnan().all()
+    dx, _, _ = ops.layer_norm_backward(bx, bd, mean, invstd, w)
+    assert torch.equal(dx[keep], ref[3][keep]) and dx[rows].isnan().all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("rows,D,at", [(300, 1001, (1, 1)), (300, 1001, (1, 2)), (1100, 512, (3, 3)), (400, 2046, (0, 0)), (5000, 515, (2, 2))])
+def test_layer_norm_of_tensors_that_begin_anywhere(dev, rows, D, at, kind):
+    """rows that begin equally or unequally far behind an aligned address, nothing behind them touched"""
+    def place(t, k):
+        flat = torch.full((t.numel() + 8,), 7.0, dtype=t.dtype, device=dev)
+        flat[k:k + t.numel()] = t.flatten()
+        return flat, flat[k:k + t.numel()].view(t.shape)
+
+    x, w, b, dy = _norm_inputs(dev, rows, D, TYPES[kind], torch.float32, 31)
+    (fx, px), (fd, pd) = place(x, at[0]), place(dy, at[1])
+    _check_norm(ops, px, w, b, pd)
+    # outputs placed by the caller too
+    m, r = lm.layer_norm(x, w, b, 1e-5)[1:]
+    m, r = m.float(), r.float()
+    (fg, pg), dw, db = place(torch.empty_like(x), at[0]), torch.empty(D, device=dev), torch.empty(D, device=dev)
+    L = _lib.lib()
+    ws = torch.empty(L.hfuse_layernorm_backward_workspace_bytes(rows, D), dtype=torch.uint8, device=dev)
+    t = ops._LM_TYPES[x.dtype]
+    _lib.check(L.hfuse_layernorm_backward(px.data_ptr(), D, pd.data_ptr(), D, rows, D, t, m.data_ptr(), r.data_ptr(), w.data_ptr(), 0,
+                                          pg.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(),
+                                          torch.cuda.current_stream().cuda_stream), "hfuse_layernorm_backward")
+    for got, exact, bound in zip((pg, dw, db), lm.layer_norm_backward(x, dy, m, r, w), lm.layer_norm_backward_bound(x, dy, m, r, w)):
+        within(got, exact, bound)
+    assert (fg[:at[0]] == 7).all() and (fg[at[0] + x.numel():] == 7).all()
+
+
 def test_layer_norm_of_no_rows(dev, api):
     x, w = torch.empty(0, 16, device=dev), torch.ones(16, device=dev)
     y, mean, invstd = api.layer_norm(x, w, None)
