@@ -378,6 +378,7 @@ __device__ __forceinline__ void weight_pairs(const float* w, int p, int packs, f
     }
 }
 
+// Bound by memory: 16384 rows of 4096 bf16 in 50 us, 5.4 TB/s (with rows loaded to registers: 60).
 template <class T, class W, int EV, int NV, bool PHASED>
 __global__ void __launch_bounds__(512) ln_fwd_rows(const LnFwdArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -560,7 +561,9 @@ __device__ __forceinline__ float warp_sum4(float a, float b, float c, float d, i
 }
 
 // Teams of warps take two rows at a time, [team][stage][x, dy][row] buffers; the block's teams add up their dw and db in
-// the same memory at the end.
+// the same memory at the end.  x and dy are read from shared memory twice, which leaves registers for the columns' sums.  8192
+// rows of 2048 floats take 34 us, 5.9 TB/s, bound by memory; 16-bit rows (16384 of 2048: 47 us with the join below) by the latency
+// of 16 warps with two barriers for a pair of rows.
 template <class T, class W, int EV, int NV, bool PHASED>
 __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -931,7 +934,7 @@ __global__ void __launch_bounds__(256) ln_bwd_cols(const LnBwdArgs a) {
 }
 
 // The slices' (or blocks') sums: 32 columns and 32 runs of slices to a block, the runs added in a fixed order.  Launched
-// as the programmatic dependent of the kernel that makes the sums.
+// as the programmatic dependent of the kernel that makes the sums.  148 blocks' sums of 2048 columns: 4.4 us.
 template <class W>
 __global__ void __launch_bounds__(1024) ln_bwd_fold(const LnBwdArgs a) {
     __shared__ float sh[32][33];

@@ -447,7 +447,10 @@ __device__ __forceinline__ void sweep_backward(const T* sd, const float2 (&a)[N]
 }
 
 // ---- staging by cp.async -----------------------------------------------------------------------------------
-// [2 stages][tensors][rows][C], the warps' maps (the barrier at the top of a piece is behind their last reader), next, peers
+// [2 stages][tensors][rows][C], the warps' maps (the barrier at the top of a piece is behind their last reader), next, peers.
+// For single steps (64 x 2048 bf16: 6.8 us, the host's launch), short sequences and strides that tiles do not take.
+// 8 x 4096 steps of 2048 bf16 channels took 73 us with it, its gradient's 4 x 8192 steps of 1024 86 us: the staging's
+// instructions are what tiles save.
 template <class T, int CPL, int S, int ALIGN>
 __global__ void __launch_bounds__(256, 2) rec_fwd(const RecArgs p) {
     constexpr int C = 32 * CPL, N = S * CPL / 2;
@@ -643,6 +646,8 @@ __device__ __forceinline__ void hold_beyond(T* sg, int steps) {
         for (int c = 0; c < CPL; ++c) sg[s * C + c] = from_f32<T>(__int_as_float(0x7f800000));
 }
 
+// Bound by memory: 8 x 4096 steps of 2048 bf16 channels in 71 us, 5.7 TB/s (issue slots are next: two blocks of 9 warps to an
+// SM).  Few channels, 65537 steps of 768 floats by clusters of 8: 111 us, 5.4 TB/s.
 template <class T, int CPL, int S>
 __global__ void __launch_bounds__(kWarpsFwd * 32 + 32, 2) rec_fwd_tiles(const RecArgs p, const __grid_constant__ RecTiles m) {
     constexpr int C = 32 * CPL, N = S * CPL / 2, W = kWarpsFwd, rows = W * S, TILE = rows * C;
@@ -716,6 +721,7 @@ __global__ void __launch_bounds__(kWarpsFwd * 32 + 32, 2) rec_fwd_tiles(const Re
 
 // The backward pass needs all registers that 16 warps leave each other, so no warp is left to move tiles: the last warp to
 // finish a piece stores it, and loads another one into its place when it has gone through the first half of the next.
+// Bound by issue slots: 4 x 8192 steps of 1024 bf16 channels in 76 us, 4.4 TB/s.
 template <class T, int CPL, int S>
 __global__ void __launch_bounds__(kWarpsBwd * 32, 1) rec_bwd_tiles(const RecArgs p, const __grid_constant__ RecTiles m) {
     constexpr int C = 32 * CPL, N = S * CPL / 2, W = kWarpsBwd, rows = W * S, TILE = rows * C;
