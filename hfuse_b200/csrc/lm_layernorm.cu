@@ -90,7 +90,7 @@ __device__ __forceinline__ void weights_of(const W* from, int p, float2 (&to)[kP
 }
 
 template <class T, class W, int EV, int NV>
-__global__ void __launch_bounds__(256) ln_fwd_short(const LnFwdArgs a) {
+__global__ void __launch_bounds__(256, NV * EV == 16 ? 3 : 1) ln_fwd_short(const LnFwdArgs a) {
     const T* x = static_cast<const T*>(a.x);
     const int lanes = a.lanes, packs = a.D / EV, per = 256 / lanes, at = threadIdx.x & (lanes - 1);
     const long long step = (long long)gridDim.x * per;
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(256) ln_fwd_short(const LnFwdArgs a) {
 // The same layout backwards: x and dy of a row are in registers, the two row sums are reduced together, and each
 // thread adds up dy xh and dy of its columns over all its rows.  The blocks' sums go to the workspace, [block][2][D].
 template <class T, class W, int EV, int NV>
-__global__ void __launch_bounds__(256) ln_bwd_short(const LnBwdArgs a) {
+__global__ void __launch_bounds__(256, NV * EV == 16 ? 2 : 1) ln_bwd_short(const LnBwdArgs a) {
     extern __shared__ float shared_sums[];                  // 2 EV NV floats of every thread, [value][thread]
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.dy);
