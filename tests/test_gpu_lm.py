@@ -218,6 +218,24 @@ def test_embedding(dev, api, shape, V, D, kind):
     within(want, lm.embedding(table, ids, scale), lm.U * lm.embedding(table, ids, scale).abs())
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [16, 31, 32, 33, 35, 64, 250, 1001, 2046, 4097])
+@pytest.mark.parametrize("at", [(0, 0), (1, 0), (3, 3), (2, 5), (7, 4)])
+def test_embedding_of_tables_and_outputs_that_begin_anywhere(dev, D, at, kind):
+    V, t = 9, TYPES[kind]
+    flat = torch.randn(V * D + 16, generator=_gen(dev, 41), device=dev).to(t)
+    flat[:at[0]], flat[at[0] + V * D:] = float("nan"), float("nan")
+    table = flat[at[0]:at[0] + V * D].view(V, D)
+    ids = torch.tensor([0, V - 1, 4, 4, -1, V, 3, 0, V - 1, 7, 1], dtype=torch.int32, device=dev)
+    room = torch.full((len(ids) * D + 16,), 7.0, dtype=t, device=dev)
+    out = room[at[1]:at[1] + len(ids) * D].view(len(ids), D)
+    _lib.check(_lib.lib().hfuse_embedding(table.data_ptr(), V, D, ops._LM_TYPES[t], ids.data_ptr(), len(ids), 4, 1.5, out.data_ptr(),
+                                          torch.cuda.current_stream().cuda_stream), "hfuse_embedding")
+    exact = torch.where(((ids >= 0) & (ids < V))[:, None], table[ids.clamp(0, V - 1).long()].double() * 1.5, 0.0)
+    assert torch.equal(out, exact.to(t))              # a product with 1.5 of a 16-bit value is exact in 32 bits, of a float one rounding
+    assert (room[:at[1]] == 7).all() and (room[at[1] + len(ids) * D:] == 7).all()
+
+
 def test_embedding_ids_outside_the_table(dev, api):
     table = torch.randn(10, 24, device=dev)
     ids = torch.tensor([0, -1, 9, 10, 1 << 40, -(1 << 40), 5], device=dev)
