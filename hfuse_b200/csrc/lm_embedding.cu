@@ -68,7 +68,7 @@ struct EmbFwdArgs {
 };
 
 // `lanes` threads to a token, kAhead accesses each, the block's second index over longer rows: all loads of a thread are
-// under way together.  16384 tokens of 2048 floats from 50257 rows: 33.6 us, 5.4 TB/s; bound by memory.
+// under way together.  16384 tokens of 2048 floats from 50257 rows: 33 us, 5.5 TB/s; bound by memory.
 constexpr int kAhead = 4;
 template <class T, int EV, class I>
 __global__ void __launch_bounds__(256) emb_fwd(const EmbFwdArgs a) {

@@ -126,6 +126,20 @@ def test_layer_norm_keeps_a_bad_row_to_itself(dev):
     assert torch.equal(dx[keep], ref[0][keep]) and dx[rows].isnan().all() and torch.equal(db, ref[2])
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [1, 5, 7, 300, 1201])
+@pytest.mark.parametrize("D,wide", [(129, 193), (1001, 1009), (2047, 4095)])
+def test_layer_norm_of_a_slice_with_rows_of_equal_offset(dev, rows, D, wide, kind):
+    t = TYPES[kind]
+    x, w, b, dy = _norm_inputs(dev, rows, D, t, torch.float32, 37)
+    room = torch.full((rows, wide), float("nan"), dtype=t, device=dev)
+    grads = room.clone()
+    room[:, :D], grads[:, :D] = x, dy
+    got, ref = _check_norm(ops, room[:, :D], w, b, grads[:, :D]), _check_norm(ops, x, w, b, dy)
+    for g, r in zip(got[:4], ref[:4]):
+        assert torch.equal(g, r)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("D", [1001, 250, 333])
 def test_layer_norm_keeps_bad_rows_to_themselves_where_rows_share_accesses(dev, D, kind):
