@@ -244,7 +244,8 @@ HFUSE_API int hfuse_embedding_backward(const void* grad_out, const void* ids, in
  * after the last one: a sequence may be worked off in pieces, down to single steps.  `states` (float, may
  * be NULL: not wanted) receives what the backward pass needs, [B][hfuse_gated_recurrence_chunks(T)][D]:
  * the state before every step that is a multiple of HFUSE_RECURRENCE_CHUNK.  A gate of -infinity
- * starts afresh (h_t = x_t), one of +infinity holds the state. */
+ * starts afresh (h_t = x_t), one of +infinity holds the state; both multiply what they leave out by
+ * zero, so a state or an x that is infinite or NaN gives NaN all the same. */
 #define HFUSE_RECURRENCE_CHUNK 256
 HFUSE_API int64_t hfuse_gated_recurrence_chunks(int64_t T);
 HFUSE_API int hfuse_gated_recurrence(const void* gate, int64_t gate_stride_b, int64_t gate_stride_t, const void* x,
