@@ -45,9 +45,10 @@ struct RecArgs {
     int split;               // blocks that share a group
 };
 
-// a = sigmoid(g) and z = 1 - a = sigmoid(-g), both to a few units in their last place: with e = exp(-g),
-// a = 1 / (1 + e) and z = e a.  A gate of -infinity has e = infinity, a = 0 and z = min(infinity * 0, 1) = 1 (the minimum
-// of a NaN and a number is the number); a gate that is a NaN makes a one.
+// a = sigmoid(g) and z = 1 - a = sigmoid(-g): with e = exp(-g), a = 1 / (1 + e) and z = e a.  From e = 2^126 on (gates below
+// -87.3, -infinity among them) the reciprocal is flushed to zero; e a would then be zero or no number, and z is one.  The
+// exponent is a product rounded to 32 bits, so e's relative error grows with the gate: about (4 + 1.3 |g|) 2^-24, and a few
+// roundings more for a and z.  A gate that is a NaN makes both one.
 __device__ __forceinline__ void gates2(float2 g, float2& a, float2& z) {
     const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
     float2 e;
@@ -57,8 +58,8 @@ __device__ __forceinline__ void gates2(float2 g, float2& a, float2& z) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a.x) : "f"(d.x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a.y) : "f"(d.y));
     z = mul2(e, a);
-    z.x = fminf(z.x, 1.f);
-    z.y = fminf(z.y, 1.f);
+    z.x = a.x == 0.f ? 1.f : z.x;
+    z.y = a.y == 0.f ? 1.f : z.y;
 }
 
 // ---- staging: `rows` steps of 32 * CPL channels into shared memory ----------------------------------------

@@ -245,7 +245,8 @@ HFUSE_API int hfuse_embedding_backward(const void* grad_out, const void* ids, in
  * be NULL: not wanted) receives what the backward pass needs, [B][hfuse_gated_recurrence_chunks(T)][D]:
  * the state before every step that is a multiple of HFUSE_RECURRENCE_CHUNK.  A gate of -infinity
  * starts afresh (h_t = x_t), one of +infinity holds the state; both multiply what they leave out by
- * zero, so a state or an x that is infinite or NaN gives NaN all the same. */
+ * zero, so a state or an x that is infinite or NaN gives NaN all the same.  Of a_t and 1 - a_t, one
+ * that is below 2^-126 counts as zero. */
 #define HFUSE_RECURRENCE_CHUNK 256
 HFUSE_API int64_t hfuse_gated_recurrence_chunks(int64_t T);
 HFUSE_API int hfuse_gated_recurrence(const void* gate, int64_t gate_stride_b, int64_t gate_stride_t, const void* x,

@@ -1,0 +1,64 @@
+"""The language-model operators at the ends of their inputs' ranges, against the 64-bit definitions."""
+import pytest
+import torch
+
+from hfuse_b200 import ops
+from oracle import lm
+from test_gpu_lm import TYPES, _check_rec, _gen
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- gates in the tails of the sigmoid --------------------------------------------------------------------------
+def _tail_inputs(dev, B, T, D, t, seed):
+    """Gates from -104 to -80 and from 80 to 104 in steps of 1/16, far ones, infinities, and a few moderate ones in between.
+    Only one of a and 1 - a is there in 32 bits (the other one's exponential may be flushed below 2^-126): with |x|, |h| <= 1/2
+    and |e| <= 1 what is flushed is at most 2^-126 of any result, and `store` grants 2^-125."""
+    g = _gen(dev, seed)
+    near = torch.arange(80, 104, 1 / 16)
+    values = torch.cat([-near, -near, near, torch.tensor([-1e4, 1e4, -110.0, 110.0, float("-inf"), float("inf")] * 16)]).to(dev)
+    gate = values[torch.randint(0, len(values), (B, T, D), generator=g, device=dev)]
+    some = torch.rand(B, T, D, generator=g, device=dev) < 0.2
+    gate = torch.where(some, 3 * torch.randn(B, T, D, generator=g, device=dev), gate).to(t)
+    x, dy = ((torch.rand(B, T, D, generator=g, device=dev) - 0.5).to(t) for _ in range(2))
+    h0, dl = (torch.rand(B, D, generator=g, device=dev) - 0.5 for _ in range(2))
+    return gate, x, (dy / 32).to(t), h0, dl / 32
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,D", [(64, 1, 40), (3, 40, 33), (2, 300, 64), (3, 300, 34), (2, 530, 72), (40, 513, 256), (1, 4096, 64), (1, 3001, 33)])
+def test_gates_in_the_tails(dev, B, T, D, kind):
+    """single steps, staged pieces, tiles, and both shared by the blocks of a cluster"""
+    gate, x, dy, h0, dl = _tail_inputs(dev, B, T, D, TYPES[kind], 51)
+    sens = lm.gated_recurrence_backward(gate, x, h0, dy, dl)[3]
+    assert sens.abs().max() <= 1
+    h, _, _ = _check_rec(ops, gate, x, dy, h0, dl)
+    reset = gate <= -104
+    assert torch.equal(h[reset], x[reset])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("gate", [-87.5, -88.0, -88.5, -87.0, -89.0])
+def test_a_gate_that_leaves_nothing_of_the_state(dev, gate, kind):
+    for T in (1, 20, 600):
+        x = torch.randn(2, T, 64, generator=_gen(dev, 52), device=dev).to(TYPES[kind])
+        g = torch.full_like(x, gate)
+        h, last, states = ops.gated_recurrence(g, x, None, True)
+        # 1 - a is 1 up to the roundings of e, of the sum, of the reciprocal and of the product: 8 half steps
+        assert ((h.double() - x.double()).abs() <= lm.store(8 * lm.U * x.double().abs(), x.double(), x.dtype)).all()
+        _, dx, _ = ops.gated_recurrence_backward(g, x, states, x)
+        assert ((dx.double() - x.double()).abs() <= lm.store(8 * lm.U * x.double().abs(), x.double(), x.dtype)).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 20, 600])
+def test_a_gate_that_is_no_number(dev, T, kind):
+    g = _gen(dev, 53)
+    gate, x, dy = (torch.randn(2, T, 64, generator=g, device=dev).to(TYPES[kind]) for _ in range(3))
+    at = T // 2
+    gate[1, at, 5] = float("nan")
+    h, last, states = ops.gated_recurrence(gate, x, None, True)
+    dg, dx, dh0 = ops.gated_recurrence_backward(gate, x, states, dy)
+    for got in (h[1, at:, 5], last[1, 5], dg[1, :at + 1, 5], dx[1, :at + 1, 5], dh0[1, 5]):
+        assert got.isnan().all()
+    assert h.isnan().sum() == T - at and dx.isnan().sum() == at + 1
