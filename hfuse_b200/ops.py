@@ -340,6 +340,13 @@ def _check_lm(x, name, dim=None, dtypes=None, shape=None, like=None):
     return x
 
 
+def _row_length(x, name):
+    """Elements of a row; the C entry points take a 32-bit number, of which ctypes would pass the lower bits."""
+    if x.shape[-1] > 0x7fffffff:
+        raise ValueError(f"{name} has too long rows")
+    return x.shape[-1]
+
+
 def _contiguous(x, name):
     if not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -404,7 +411,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stream=None):
     if not eps >= 0:
         raise ValueError("layer_norm: eps must not be negative")
     wt = _check_norm_params(x, weight, bias)
-    D, ld = x.shape[-1], _row_stride(x, "layer_norm input")
+    D, ld = _row_length(x, "layer_norm input"), _row_stride(x, "layer_norm input")
     with _on(x, stream) as s:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
@@ -425,7 +432,8 @@ def layer_norm_backward(x, grad_out, mean, invstd, weight=None, stream=None):
     for t, name in ((mean, "mean"), (invstd, "invstd")):
         _contiguous(_check_lm(t, name, dtypes=(torch.float32,), shape=x.shape[:-1], like=x), name)
     wt = _check_norm_params(x, weight, None)
-    D, rows = x.shape[-1], x.numel() // x.shape[-1]
+    D = _row_length(x, "layer_norm input")
+    rows = x.numel() // D
     ldx, ldg = _row_stride(x, "layer_norm input"), _row_stride(grad_out, "layer_norm grad_out")
     L = _lib.lib()
     with _on(x, stream) as s:
@@ -450,7 +458,7 @@ def embedding(table, ids, scale=1.0, stream=None):
     if 0 in table.shape:
         raise ValueError("embedding table must not be empty")
     _check_ids(ids, table)
-    rows, D = table.shape
+    rows, D = table.shape[0], _row_length(table, "embedding table")
     with _on(table, stream) as s:
         out = torch.empty(tuple(ids.shape) + (D,), dtype=table.dtype, device=table.device)
         _lib.check(_lib.lib().hfuse_embedding(table.data_ptr(), rows, D, _LM_TYPES[table.dtype], ids.data_ptr(), ids.numel(),
@@ -466,7 +474,7 @@ def embedding_backward(grad_out, ids, rows, scale=1.0, padding_id=-1, stream=Non
         raise ValueError("embedding grad_out must have the shape of ids and one dimension more")
     if rows < 1:
         raise ValueError("embedding_backward: rows must be positive")
-    D, n, L = grad_out.shape[-1], ids.numel(), _lib.lib()
+    D, n, L = _row_length(grad_out, "embedding grad_out"), ids.numel(), _lib.lib()
     with _on(grad_out, stream) as s:
         grad = torch.empty(rows, D, dtype=grad_out.dtype, device=grad_out.device)
         ws = torch.empty(L.hfuse_embedding_backward_workspace_bytes(n, rows, D), dtype=torch.uint8, device=grad_out.device)
@@ -480,6 +488,7 @@ def _check_steps(x, name, like=None):
     _check_lm(x, name, dim=3, dtypes=None if like is None else (like.dtype,), shape=None if like is None else like.shape, like=like)
     if 0 in x.shape:
         raise ValueError(f"{name} must not be empty")
+    _row_length(x, name)
     return x
 
 

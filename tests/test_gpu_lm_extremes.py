@@ -4,7 +4,7 @@ import torch
 
 from hfuse_b200 import ops
 from oracle import lm
-from test_gpu_lm import TYPES, _check_rec, _gen
+from test_gpu_lm import TYPES, _check_rec, _gen, api  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,15 @@ def test_a_gate_that_is_no_number(dev, T, kind):
     for got in (h[1, at:, 5], last[1, 5], dg[1, :at + 1, 5], dx[1, :at + 1, 5], dh0[1, 5]):
         assert got.isnan().all()
     assert h.isnan().sum() == T - at and dx.isnan().sum() == at + 1
+
+
+# ---- rows that no kernel takes ----------------------------------------------------------------------------------
+def test_rows_whose_length_passes_32_bits_are_refused(dev, api):
+    """not taken for rows of the length's lower 32 bits"""
+    x = torch.zeros(1, (1 << 32) + 8, dtype=torch.float16, device=dev)
+    ids, one = torch.zeros(1, dtype=torch.int64, device=dev), torch.ones(1, device=dev)
+    for call in (lambda: api.layer_norm(x), lambda: api.layer_norm_backward(x, x, one, one), lambda: api.embedding(x, ids),
+                 lambda: api.embedding_backward(x, ids, 1), lambda: api.gated_recurrence(x[None], x[None]),
+                 lambda: api.gated_recurrence_backward(x[None], x[None], x[None].view(torch.float32), x[None])):
+        with pytest.raises((ValueError, RuntimeError), match="too long rows"):
+            call()
