@@ -381,6 +381,8 @@ class _on:
     """Device and stream of a call: buffers made inside belong to the stream that the kernels run on."""
 
     def __init__(self, x, stream):
+        if stream is not None and stream.device != x.device:
+            raise ValueError(f"the stream must be one of {x.device}, is one of {stream.device}")
         self.stream = stream if stream is not None else torch.cuda.current_stream(x.device)
 
     def __enter__(self):
