@@ -326,7 +326,7 @@ __device__ __forceinline__ void team_sync(int team, int warps) {
 }
 
 // A row's elements in the registers of a team: accesses of EV elements, or (EV = 1) single elements in pairs of
-// accesses.  VALUES pairs.  A place beyond the row holds the row's last access again: who adds up has to leave it out.
+// accesses.  VALUES pairs.
 template <class T, int EV, int NV>
 struct Team {
     static constexpr int VALUES = NV * EV / 2;
@@ -340,7 +340,8 @@ struct Team {
         else return pair_of<T, EV>(v[i / (EV / 2)], i % (EV / 2));
     }
 };
-// where in a row's buffer a thread's accesses are
+// where in a row's buffer a thread's accesses are; a place beyond the row is the row's last access again: who adds up has to
+// leave it out
 template <class T, int EV, int NV>
 __device__ __forceinline__ void places(int (&place)[NV], int at, int lanes, int packs) {
 #pragma unroll
@@ -579,7 +580,6 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     unsigned char* ring = smem + (size_t)team * a.stages * 4 * a.buf;
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)teams * a.stages * 4 * a.buf) + team * 2;
     float* sums = reinterpret_cast<float*>(smem + (size_t)teams * (a.stages * 4 * (size_t)a.buf + 16)) + team * 8 * warps;   // [2][warps][4]
-    // a weight of zero keeps places beyond the row out of the row sums; nothing is stored for them
     float2 kw[VALUES], dw[VALUES], db[VALUES];
     {
         Team<W, EV, NV> t;
@@ -600,8 +600,12 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
             dw[i] = db[i] = make_float2(0.f, 0.f);
         }
     }
+    // places beyond the row read zeros, which keep out of the row sums whatever the row holds; nothing is stored for them
+    const int none = EV > 1 ? packs * EV * (int)sizeof(T) : a.buf - 32;
     int place[NV];
-    places<T, EV, NV>(place, at, lanes, packs);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+        place[k] = EV > 1 ? min(at + k * lanes, packs) * EV * (int)sizeof(T) : at + k * lanes < packs ? (at + k * lanes) * (int)sizeof(T) : none;
     // the thread's single elements of the next two rows
     float edge_w = 0.f, edge_dw = 0.f, edge_db = 0.f, ex[2] = {0.f, 0.f}, ed[2] = {0.f, 0.f};
     if (PHASED && cut.column >= 0) edge_w = weight_of<W>(w, cut.column, 1.f);
@@ -647,6 +651,11 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     long long r = first + 2LL * period * (number / period);
     for (int s = 0; s < a.stages; ++s)
         if (r + s * step < a.rows) fetch(r + s * step, s);
+    if (at + (NV - 1) * lanes >= packs)                    // who reads the zeros writes them
+        for (int b = 0; b < 4 * a.stages; ++b)
+#pragma unroll
+            for (int h = 0; h < (EV == 1 ? 2 : 1); ++h)
+                reinterpret_cast<float4*>(ring + (size_t)b * a.buf + none)[h] = make_float4(0.f, 0.f, 0.f, 0.f);
     float now = stats(r), next = 0.f;
     edges(r);
     int stage = 0, parity = 0;
@@ -1024,11 +1033,13 @@ template <class T, class W, int EV, int NV, bool PHASED = false>
 int ln_bwd_rows_launch(LnBwdArgs& a, int sms, cudaStream_t s) {
     auto kern = ln_bwd_rows<T, W, EV, NV, PHASED>;
     a.lanes = (int)((a.D / EV + 32 * NV - 1) / (32 * NV) * 32);
-    a.buf = (int)((a.D * sizeof(T) + 15) / 16 * 16 + (EV == 1 ? 16 : 0));
-    a.stages = 8 * (size_t)a.buf <= kRowSmem ? 2 : 1;
+    // a row (EV = 1: that begins up to 15 bytes into its buffer), then zeros for one access where there are places beyond it
+    const size_t row = (a.D * sizeof(T) + 15) / 16 * 16 + (EV == 1 ? 16 : 0);
+    a.buf = PHASED || a.D / EV % (NV * a.lanes) != 0 ? (int)(row + (EV == 1 ? 32 : 16) + 127) / 128 * 128 : (int)row;
+    a.stages = 8 * row <= kRowSmem ? 2 : 1;
     const long long pairs = (a.rows + 1) / 2;
     int teams = 512 / a.lanes;
-    while (teams > 1 && ((size_t)teams * a.stages * 4 * a.buf > kRowSmem || (long long)(teams - 1) * sms >= pairs)) --teams;
+    while (teams > 1 && ((size_t)teams * a.stages * 4 * row > kRowSmem || (long long)(teams - 1) * sms >= pairs)) --teams;
     // a team's dw and db, 8 D bytes, fit its buffers: 16 D with two stages of 16-bit rows
     const size_t smem = (size_t)teams * (a.stages * 4 * (size_t)a.buf + 16 + (size_t)(a.lanes / 32) * 32);
     const long long want = (pairs + teams - 1) / teams;

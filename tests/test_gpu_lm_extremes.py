@@ -74,3 +74,28 @@ def test_rows_whose_length_passes_32_bits_are_refused(dev, api):
                  lambda: api.gated_recurrence_backward(x[None], x[None], x[None].view(torch.float32), x[None])):
         with pytest.raises((ValueError, RuntimeError), match="too long rows"):
             call()
+
+
+# ---- infinite gradients -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,D", [(300, 40), (300, 304), (500, 1000), (300, 2050), (400, 1001), (300, 515), (200, 8190), (130, 16400), (20, 1000)])
+@pytest.mark.parametrize("weighted", [True, False])
+def test_layer_norm_gradient_of_rows_with_infinite_elements(dev, rows, D, kind, weighted):
+    """What the definition gives for a row whose gradient is infinite in its last or first element: an infinite element
+    where all terms agree in sign, no number elsewhere; rows without one are not touched."""
+    g = _gen(dev, 54)
+    x, dy = (torch.randn(rows, D, generator=g, device=dev).to(TYPES[kind]) for _ in range(2))
+    w = 1 + torch.rand(D, generator=g, device=dev) if weighted else None
+    _, mean, invstd = ops.layer_norm(x, w)
+    ref = ops.layer_norm_backward(x, dy, mean, invstd, w)
+    at = torch.arange(rows, device=dev)
+    bad = dy.clone()
+    bad[at % 5 == 1, -1], bad[at % 5 == 3, 0] = float("inf"), float("-inf")
+    dx, dw, db = ops.layer_norm_backward(x, bad, mean, invstd, w)
+    exact = lm.layer_norm_backward(x, bad, mean, invstd, w)
+    hit = (at % 5 == 1) | (at % 5 == 3)
+    assert torch.equal(dx[~hit], ref[0][~hit]) and exact[0][hit].isinf().any() and exact[2][-1] == float("inf")
+    for got, want in ((dx[hit], exact[0][hit]), (dw[[0, -1]], exact[1][[0, -1]]), (db[[0, -1]], exact[2][[0, -1]])):
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got[want.isinf()].double(), want[want.isinf()])
+    assert torch.equal(dw[1:-1], ref[1][1:-1]) and torch.equal(db[1:-1], ref[2][1:-1])
