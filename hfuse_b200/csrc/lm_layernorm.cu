@@ -335,6 +335,15 @@ struct Team {
 #pragma unroll
         for (int k = 0; k < NV; ++k) v[k] = load_shared<T, EV>(row + place[k]);
     }
+    // places behind `last` read that one; the minimum is kept from being taken ahead, which would cost a register each
+    __device__ __forceinline__ void read_until(uint32_t row, const int (&place)[NV], int last) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            int p;
+            asm volatile("min.s32 %0, %1, %2;" : "=r"(p) : "r"(place[k]), "r"(last));
+            v[k] = load_shared<T, EV>(row + p);
+        }
+    }
     __device__ __forceinline__ float2 get(int i) const {
         if constexpr (EV == 1) return make_float2(pair_of<T, 1>(v[2 * i], 0).x, pair_of<T, 1>(v[2 * i + 1], 0).x);
         else return pair_of<T, EV>(v[i / (EV / 2)], i % (EV / 2));
@@ -600,8 +609,10 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
             dw[i] = db[i] = make_float2(0.f, 0.f);
         }
     }
-    // places beyond the row read zeros, which keep out of the row sums whatever the row holds; nothing is stored for them
+    // Places beyond the row read x's last access again and zeros as dy, which keep out of the row sums whatever the row
+    // holds (as x, a zero could be infinitely many deviations from the mean); nothing is stored for them.
     const int none = EV > 1 ? packs * EV * (int)sizeof(T) : a.buf - 32;
+    const int last = (packs - 1) * EV * (int)sizeof(T);
     int place[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -700,7 +711,7 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
                 d[g].x = egw[g] * exh[g];
             }
             Team<T, EV, NV> vx, vd;
-            vx.read(at_buf + g * a.buf + shift[g], place);
+            vx.read_until(at_buf + g * a.buf + shift[g], place, last);
             vd.read(at_buf + (2 + g) * a.buf + shift[2 + g], place);
 #pragma unroll
             for (int i = 0; i < VALUES; ++i) {
@@ -736,7 +747,7 @@ __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
             if (g >= two || !a.dx) continue;
             const float2 is2 = make_float2(is, is), off = make_float2(-mu, -mu), ms2 = make_float2(ms, ms), md2 = make_float2(md, md);
             Team<T, EV, NV> vx, vd;
-            vx.read(at_buf + g * a.buf + shift[g], place);
+            vx.read_until(at_buf + g * a.buf + shift[g], place, last);
             vd.read(at_buf + (2 + g) * a.buf + shift[2 + g], place);
             T* dx = static_cast<T*>(a.dx) + (r + g * period) * a.D + cut.lead;
             if (PHASED && cut.column >= 0) dx[cut.column - cut.lead] = from_f32<T>(is * fmaf(exh[g], md, egw[g] + ms));

@@ -99,3 +99,31 @@ def test_layer_norm_gradient_of_rows_with_infinite_elements(dev, rows, D, kind, 
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got[want.isinf()].double(), want[want.isinf()])
     assert torch.equal(dw[1:-1], ref[1][1:-1]) and torch.equal(db[1:-1], ref[2][1:-1])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,D", [(300, 40), (300, 304), (500, 1000), (400, 1001), (300, 515), (200, 8190), (130, 16400), (20, 1000)])
+def test_layer_norm_gradient_of_large_constant_rows(dev, rows, D, kind):
+    """Rows of one value: x - mean is zero, whatever mean times invstd is.  2^123 / sqrt(1e-5) is beyond 32 bits; the sums of D such
+    values are not (a power of two, so that they are exact)."""
+    dy = torch.randn(rows, D, generator=_gen(dev, 55), device=dev).to(TYPES[kind])
+    big = torch.full_like(dy, 2.0 ** 123)
+    mean, invstd = torch.full((rows,), 2.0 ** 123, device=dev), torch.full((rows,), 1e-5 ** -0.5, device=dev)
+    small = torch.zeros_like(dy), torch.zeros_like(mean)
+    for got, want in zip(ops.layer_norm_backward(big, dy, mean, invstd), ops.layer_norm_backward(small[0], dy, small[1], invstd)):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("D", [301, 1000, 2050])
+def test_layer_norm_gradient_with_infinite_elements_of_tensors_that_begin_anywhere(dev, D, kind):
+    """single elements: x and grad_out begin unequally far behind an aligned address"""
+    g = _gen(dev, 56)
+    flat = torch.randn(2, 400 * D + 8, generator=g, device=dev).to(TYPES[kind])
+    x, dy = flat[0, 1:400 * D + 1].view(400, D), flat[1, 2:400 * D + 2].view(400, D)
+    _, mean, invstd = ops.layer_norm(x)
+    dy[::3, -1] = float("inf")
+    dx = ops.layer_norm_backward(x, dy, mean, invstd)[0]
+    exact = lm.layer_norm_backward(x, dy, mean, invstd, None)[0]
+    assert torch.equal(dx.isnan(), exact.isnan()) and torch.equal(dx[exact.isinf()].double(), exact[exact.isinf()])
+    assert exact.isinf().any() and dx[1::3].isfinite().all()
