@@ -592,6 +592,9 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* m, const void* fro
                  : "memory");
 }
 constexpr unsigned long long kTileWaitNs = 2000000000ull;
+// The computing warps give up on tiles and on peers once each and then go on with NaN, so a piece's results are late by
+// both waits at most; the warp that stores them waits longer, or results that are NaN would not be stored at all.
+constexpr unsigned long long kWrittenWaitNs = kTileWaitNs + kPeerWaitNs + 1000000000ull;
 constexpr int kFwdStages = 3, kBwdStages = 2;
 
 // The warp beside the W computing ones: loads pieces ahead, stores a piece's results when all warps have written them
@@ -603,7 +606,7 @@ __device__ __forceinline__ void move_tiles(int n, int lane, unsigned long long* 
         for (int k = 0; k < STAGES && k < n; ++k) load(k);
         int stage = 0, parity = 0;
         for (int k = 0; k < n; ++k) {
-            if (!mbar_wait(written + stage, parity, kTileWaitNs)) break;      // the others find no more tiles and give up
+            if (!mbar_wait(written + stage, parity, kWrittenWaitNs)) break;   // the others find no more tiles and give up
             store(k);
             bulk_commit();
             if (k + STAGES < n) {
