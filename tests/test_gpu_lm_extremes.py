@@ -4,7 +4,7 @@ import torch
 
 from hfuse_b200 import ops
 from oracle import lm
-from test_gpu_lm import TYPES, _check_rec, _gen, api  # noqa: F401
+from test_gpu_lm import TYPES, _check_rec, _gen, _ids, api  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +127,19 @@ def test_layer_norm_gradient_with_infinite_elements_of_tensors_that_begin_anywhe
     exact = lm.layer_norm_backward(x, dy, mean, invstd, None)[0]
     assert torch.equal(dx.isnan(), exact.isnan()) and torch.equal(dx[exact.isinf()].double(), exact[exact.isinf()])
     assert exact.isinf().any() and dx[1::3].isfinite().all()
+
+
+# ---- sums that are exact in 32 bits -----------------------------------------------------------------------------
+@pytest.mark.parametrize("n,V,D,how,kind", [
+    (200, 3, 40, "even", "bf16"), (1000, 1, 8, "one", "f32"), (1000, 1, 33, "one", "f16"), (8192, 5, 64, "one", "bf16"), (8192, 40, 7, "text", "f32"),
+    (17000, 3, 24, "one", "f32"), (17600, 3, 25, "one", "bf16"), (20000, 2, 64, "even", "f16"), (32769, 2, 64, "one", "bf16"),
+    (40000, 4, 24, "one", "f32"), (40000, 3, 9, "even", "f32"), (70000, 3, 128, "one", "f16"), (70000, 1000, 64, "text", "f32"),
+    (300000, 2, 8, "even", "f32"), (300000, 7, 8, "text", "bf16"), (300000, 50000, 16, "text", "f16"), (1 << 20, 3, 4, "one", "f32")])
+def test_embedding_gradient_without_a_lost_or_doubled_token(dev, n, V, D, how, kind):
+    """Whole numbers up to 8, no sum beyond 2^24: every order of additions gives the same bits, so nothing may be off.
+    Runs of more than 33 chunks and of more than 545, where the join looks for their ends in steps of 512."""
+    ids = _ids(dev, n, V, how, 57)
+    ids[7::1000], ids[11::1300] = -1, V
+    dy = torch.randint(-8, 9, (n, D), generator=_gen(dev, 58), device=dev).to(TYPES[kind])
+    assert torch.equal(ops.embedding_backward(dy, ids, V, 0.5), lm.embedding_backward(dy, ids, V, 0.5).to(TYPES[kind]))
+    assert torch.equal(ops.embedding_backward(dy, ids, V, 2.0, V // 2), lm.embedding_backward(dy, ids, V, 2.0, V // 2).to(TYPES[kind]))
