@@ -34,8 +34,9 @@ using namespace hfuse;
 
 namespace {
 
-// tokens that a thread sums: few tokens need many threads, many tokens leave fewer parts to join with long chunks (65536 tokens of
-// 2048 bf16: 164 instead of 167 us with 64)
+// Tokens that a thread sums: few tokens need many threads, many tokens leave fewer parts to join with long chunks.  With 32 and
+// with 64, into 32000 rows, in a replayed graph: 8193 tokens of 512 bf16 35 and 40 us, 32768 46 and 50, 40960 52 and 51,
+// 65536 54 and 51; of 2048 bf16 8193 tokens 50 and 54, 32768 82 and 78, 65536 114 and 113, 131072 190 and 171.
 constexpr int kChunk = 32, kSmallChunk = 16, kWideChunk = 64;
 constexpr int kTile = 2048;          // tokens a block ranks at a time
 constexpr int kMaxTiles = 128;
@@ -393,8 +394,8 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_scatter(const SortArgs 
 // Up to 8192 tokens: key and position make one 32-bit number, all of them are in every block's shared memory, and a warp
 // finds a token's place by counting the smaller ones.  The other warps write the zeros of the block's share of the rows,
 // which begins at a multiple of 32 rows; its bits (32 KB at most, for all of kSmallRows) are in shared memory too.
-// Counting keeps the arithmetic busy and zeros the memory, so the two hide each other: 15 us for 4099 tokens and the 61 MB of
-// rows that they do not meet in a table of 32000 x 1001 16-bit elements.
+// Counting keeps the arithmetic busy and zeros the memory, so the two hide each other: 18 us (by itself and cold, under ncu) for
+// 4099 tokens and the 61 MB of rows that they do not meet in a table of 32000 x 1001 16-bit elements.
 template <class I>
 __global__ void __launch_bounds__(1024) emb_sort_small(const SortArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -471,8 +472,8 @@ __device__ __forceinline__ void note_crossing(const EmbSumArgs& a, int c, unsign
     a.crossing[is_long ? a.chunks - 1 - k : k] = make_uint2((unsigned)c, id);
 }
 
-// Chunks of the sorted tokens, EV columns to a thread; bound by memory: 102 us for 65536 tokens of 2048 bf16 and the part of the
-// zeros of 128000 rows that the sort left (5.9 TB/s).
+// Chunks of the sorted tokens, EV columns to a thread; bound by memory: 96 us (under ncu) for 65536 tokens of 2048 bf16 and
+// the part of the zeros of 128000 rows that the sort left.
 template <class T, int EV>
 __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
     constexpr int P = (EV + 1) / 2, U = 8;                // U rows of grad_out are under way together
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(256) emb_sum(const EmbSumArgs a) {
 
 // The same for rows that allow narrow accesses only (EV elements of 2 or 4 bytes): a warp takes a chunk and kCols
 // accesses of each lane, a stretch of 32 apart; the chunk's keys and positions are in its lanes.  Bound by the number of
-// accesses: 12 us for 4099 tokens of 1001 16-bit elements.
+// accesses: 13 us (under ncu) for 4099 tokens of 1001 16-bit elements.
 constexpr int kCols = 4;
 template <class T, int EV>
 __global__ void __launch_bounds__(256) emb_sum_narrow(const EmbSumArgs a) {
@@ -624,8 +625,8 @@ __global__ void __launch_bounds__(256) emb_sum_narrow(const EmbSumArgs a) {
 }
 
 // Runs that cross chunks.  Up to kLongRun parts: a warp adds them for 32 accesses of COLS columns.  Longer ones: a block, 32
-// columns, kRuns stretches of the run's parts, the stretches' sums added in order.  10 us for 65536 tokens of 2048 bf16 with the
-// frequencies of text.
+// columns, kRuns stretches of the run's parts, the stretches' sums added in order.  18 us (by itself and cold, under ncu)
+// for 65536 tokens of 2048 bf16 with the frequencies of text.
 constexpr int kRuns = 16;
 template <class T, int COLS>
 __global__ void __launch_bounds__(32 * kRuns) emb_join(const EmbSumArgs a) {

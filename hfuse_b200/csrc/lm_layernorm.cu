@@ -572,8 +572,8 @@ __device__ __forceinline__ float warp_sum4(float a, float b, float c, float d, i
 
 // Teams of warps take two rows at a time, [team][stage][x, dy][row] buffers; the block's teams add up their dw and db in
 // the same memory at the end.  x and dy are read from shared memory twice, which leaves registers for the columns' sums.  8192
-// rows of 2048 floats take 34 us, 5.9 TB/s, bound by memory; 16-bit rows (16384 of 2048: 47 us with the join below) by the latency
-// of 16 warps with two barriers for a pair of rows.
+// rows of 2048 floats take 33 us (under ncu), 6.2 TB/s, bound by memory; 16-bit rows (16384 of 2048: 47 us with the join below, of
+// 1000 elements 32) by the latency of 16 warps with two barriers for a pair of rows.
 template <class T, class W, int EV, int NV, bool PHASED>
 __global__ void __launch_bounds__(512) ln_bwd_rows(const LnBwdArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -863,7 +863,9 @@ __global__ void __launch_bounds__(512) ln_bwd_wide(const LnBwdArgs a) {
 }
 
 // A few rows: one launch without a workspace.  Blocks below `rows` take a row each; dw and db need no row sums, so the
-// blocks above add them up for 32 columns each at the same time, from the same inputs.
+// blocks above add them up for 32 columns each at the same time, from the same inputs.  In a replayed graph, with it and with the
+// kernels for more rows: 256 rows of 1024 bf16 4.4 and 7.3 us, 384 8.1 and 8.4, 512 11.4 and 8.6; 128 rows of 8192 bf16 7.4
+// and 18.7, 1024 32.6 and 30.3.
 constexpr long long kFewRows = 256, kFewElements = 1 << 20;
 template <class T, class W>
 __global__ void __launch_bounds__(512) ln_bwd_few(const LnBwdArgs a) {
@@ -954,7 +956,8 @@ __global__ void __launch_bounds__(256) ln_bwd_cols(const LnBwdArgs a) {
 }
 
 // The slices' (or blocks') sums: 32 columns and 32 runs of slices to a block, the runs added in a fixed order.  Launched
-// as the programmatic dependent of the kernel that makes the sums.  148 blocks' sums of 2048 columns: 4.4 us.
+// as the programmatic dependent of the kernel that makes the sums.  148 blocks' sums of 2048 columns: 7.2 us by itself and cold,
+// under ncu.
 template <class W>
 __global__ void __launch_bounds__(1024) ln_bwd_fold(const LnBwdArgs a) {
     __shared__ float sh[32][33];
@@ -1108,7 +1111,8 @@ int hfuse_layernorm(const void* x, int64_t rows, int D, int64_t ld_x, int dtype,
         if (wide && packs <= 64) return ln_fwd_short_launch<T, W, EV, 2>(a, f.sms, s);
         if (!wide && packs <= 32) return ln_fwd_short_launch<T, W, 1, 1>(a, f.sms, s);
         if (!wide && packs <= 64) return ln_fwd_short_launch<T, W, 1, 2>(a, f.sms, s);
-        // rows that fit shared memory beside their weights.  Few rows are spread over more warps each.
+        // Rows that fit shared memory beside their weights.  Few rows are spread over twice the warps each: 4096 bf16 wide, in a
+        // replayed graph, 296 rows take 4.5 instead of 5.6 us, 592 5.1 and 5.6, 888 6.9 and 6.4, 2368 11.5 and 10.1.
         const bool few = rows < 4LL * f.sms;
         auto team = [&](int nv) { return (int)(((phased ? D / EV : packs) + 32LL * nv - 1) / (32LL * nv)); };
         if (8 * (size_t)D + D * es + 64 <= kRowSmem) {
@@ -1165,7 +1169,7 @@ int hfuse_layernorm_backward(const void* x, int64_t ld_x, const void* grad_out, 
         constexpr int EV = 16 / sizeof(T), NV = 16 / EV;               // 16 columns to a thread
         const long long packs = wide ? D / EV : D;
         int rc;
-        // one launch instead of two: 8.3 instead of 12.1 us a call of a few rows, which is the host's time
+        // one launch instead of two: 8.3 instead of 10 to 12 us a call of a few rows, which is the host's time
         if (rows <= kFewRows && rows * (long long)D <= kFewElements)
             return launch_kernel(ln_bwd_few<T, W>, (int)rows + (want_w ? (D + 31) / 32 : 0), 512, 0, s, false, a);
         if (rows > 0 && packs <= 64) {

@@ -449,7 +449,8 @@ __device__ __forceinline__ void sweep_backward(const T* sd, const float2 (&a)[N]
 
 // ---- staging by cp.async -----------------------------------------------------------------------------------
 // [2 stages][tensors][rows][C], the warps' maps (the barrier at the top of a piece is behind their last reader), next, peers.
-// For single steps (64 x 2048 bf16: 6.8 us, the host's launch), short sequences and strides that tiles do not take.
+// For single steps (64 x 2048 bf16: 7 us a call, which is the host's time; 3.5 us in a replayed graph, of which an empty kernel
+// takes 0.5), short sequences and strides that tiles do not take.
 // 8 x 4096 steps of 2048 bf16 channels took 73 us with it, its gradient's 4 x 8192 steps of 1024 86 us: the staging's
 // instructions are what tiles save.
 template <class T, int CPL, int S, int ALIGN>
@@ -651,7 +652,7 @@ __device__ __forceinline__ void hold_beyond(T* sg, int steps) {
 }
 
 // Bound by memory: 8 x 4096 steps of 2048 bf16 channels in 71 us, 5.7 TB/s (issue slots are next: two blocks of 9 warps to an
-// SM).  Few channels, 65537 steps of 768 floats by clusters of 8: 111 us, 5.4 TB/s.
+// SM).  Few channels, 65537 steps of 768 floats by clusters of 8: 106 to 111 us, 5.5 TB/s.
 template <class T, int CPL, int S>
 __global__ void __launch_bounds__(kWarpsFwd * 32 + 32, 2) rec_fwd_tiles(const RecArgs p, const __grid_constant__ RecTiles m) {
     constexpr int C = 32 * CPL, N = S * CPL / 2, W = kWarpsFwd, rows = W * S, TILE = rows * C;
@@ -877,7 +878,11 @@ bool make_tiles(CUtensorMap& m, const void* at, long long stride_b, long long st
     return encode_tiled()(&m, type, 3, const_cast<void*>(at), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-constexpr int kTileSteps = 512;      // below, the host's time for the maps is worth more than what they save
+// From here on TMA tiles.  Times in a replayed graph, with tiles and by cp.async; the host needs about 1 us more for the maps.
+// Forward they differ little: 8 x 512 steps of 2048 bf16 12.2 and 12.0 us, 768 15.5 and 16.2, 1024 19.3 and 20.6.  The gradient in
+// 16 bits gains: 512 steps 24.0 and 26.0 us, 1024 40 and 51 (already 320 steps 20.6 and 23.0; 128 steps 13.0 and 7.6, since
+// its tile is 256 steps).  In floats it loses up to here, and a little beyond: 8 x 384 steps of 1024 17.2 and 15.8, 1024 35.2 and 32.9.
+constexpr int kTileSteps = 512;
 
 template <class T, int CPL, int ALIGN, bool BWD>
 int rec_launch(RecArgs a, cudaStream_t s) {

@@ -246,7 +246,8 @@ HFUSE_API int hfuse_embedding_backward(const void* grad_out, const void* ids, in
  * the state before every step that is a multiple of HFUSE_RECURRENCE_CHUNK.  A gate of -infinity
  * starts afresh (h_t = x_t), one of +infinity holds the state; both multiply what they leave out by
  * zero, so a state or an x that is infinite or NaN gives NaN all the same.  Of a_t and 1 - a_t, one
- * that is below 2^-126 counts as zero. */
+ * that is below 2^-126 counts as zero.  What an infinite x or state turns into some steps later may be
+ * NaN where step-by-step arithmetic would keep the infinity. */
 #define HFUSE_RECURRENCE_CHUNK 256
 HFUSE_API int64_t hfuse_gated_recurrence_chunks(int64_t T);
 HFUSE_API int hfuse_gated_recurrence(const void* gate, int64_t gate_stride_b, int64_t gate_stride_t, const void* x,
